@@ -653,6 +653,76 @@ void hip_softmax_f16(size_t num_els, size_t num_dims, size_t dim, const size_t* 
 /* f64 (crates/maidenx_cuda/src/nn/activation/softmax.rs:26-31): formed in f64 throughout. */
 void hip_softmax_f64(size_t num_els, size_t num_dims, size_t dim, const size_t* metadata, const double* input, double* output);
 
+/* ---- attention over packed sequences ---------------------------------------------------------------
+ * No counterpart in the reference (its users multiply, softmax and multiply over [L, L] buffers).  Causal attention of
+ * `heads` query heads over `kv_heads` key and value heads (query head h reads key head h / (heads / kv_heads)), over
+ * sequences packed one after the other along the token axis:
+ *   S_ij = scale * q_i . k_j + bias[bucket(i - j)][h]          j <= i, i and j in one sequence
+ *   output_i = sum_j P_ij v_j,   P_ij = exp(S_ij - lse_i),   lse_i = ln sum_j exp S_ij
+ * metadata = tokens, heads, kv_heads, dim, sequences, buckets, max_distance
+ *            | query strides[3] | key strides[3] | value strides[3] | query offset, key offset, value offset
+ *   strides of the token, head and element axis; query [tokens, heads, dim], key and value [tokens, kv_heads, dim]: any
+ *   strides (views of one projection among them); 16-byte aligned rows of neighbouring elements are read fastest.
+ * offsets: device array of sequences + 1 token positions, ascending from >= 0 to <= tokens; sequence s is
+ *   [offsets[s], offsets[s + 1]) and may be empty.  Offsets that do not ascend or leave the tokens are reported by
+ *   hip_get_last_status() like an index out of range (results are then unspecified, nothing outside the tensors is read
+ *   or written).  Being read on the device, they may change between replays of a captured call.
+ * bias: NULL, or a learned table [buckets, heads], contiguous (buckets 2 .. 256, buckets / 2 < max_distance <= 4096): with
+ *   E = buckets / 2, distance n has bucket n below E, else min(buckets - 1, E + floor((buckets - E) * ln(n / E) /
+ *   ln(max_distance / E))), exactly.  -inf takes a pair out; a row whose pairs are all out has an output of zeros and
+ *   lse = -inf, and gives no gradient.  Any finite bias is a bias.
+ * scale: any value, zero and negative ones included.  dim: 1 .. 128.
+ * output [tokens, heads, dim] and lse [heads, tokens] (f32) are contiguous.  Rows of tokens that no sequence holds are
+ *   not written, here and in the gradients.  Outputs must not overlap inputs.
+ * Scores, statistics and sums are f32; P (and dS in the backward pass) are rounded to the tensors' type where they enter a
+ * product, results once.  Same bits on every call.
+ * backward: grad_output [tokens, heads, dim] contiguous; output and lse as the forward call wrote them; each of
+ *   grad_query [tokens, heads, dim], grad_key and grad_value [tokens, kv_heads, dim] (contiguous; sums over the heads that share
+ *   a key head) and grad_bias [buckets, heads] may be NULL. */
+#define MX_DECL_ATTENTION(T, S)                                                                                              \
+    void hip_attention_##S(const size_t* metadata, const int32_t* offsets, const T* query, const T* key, const T* value,     \
+                           const T* bias, float scale, T* output, float* lse);                                               \
+    void hip_attention_backward_##S(const size_t* metadata, const int32_t* offsets, const T* query, const T* key,            \
+                                    const T* value, const T* bias, float scale, const T* output, const float* lse,           \
+                                    const T* grad_output, T* grad_query, T* grad_key, T* grad_value, T* grad_bias);
+MX_DECL_ATTENTION(float, f32)
+MX_DECL_ATTENTION(mx_bf16, bf16)
+MX_DECL_ATTENTION(mx_f16, f16)
+
+/* ---- clipped policy loss ---------------------------------------------------------------------------
+ * No counterpart in the reference (its one loss is MSE).  Over logits x [rows, vocabulary], for every row of weight != 0:
+ *   lse = ln sum_v exp x_v;  lp = x[target] - lse;  r = exp(lp - old_logp);  c = min(max(r, 1 - clip_low), 1 + clip_high)
+ *   loss = sum of weight * (-min(r A, c A) + kl_weight * (exp(ref_logp - lp) - (ref_logp - lp) - 1)),   A = advantage
+ *   d loss / d x_v = g ([v == target] - exp(x_v - lse)),  g = weight * (-[r A <= c A] r A + kl_weight (1 - exp(ref_logp - lp)))
+ * The weights carry the normalisation (1 / tokens, 1 / (sequences * length), ..).  A row of weight zero (a prompt token, padding)
+ * is left out: nothing of it is read - its target may be anything - and logp, lse and its gradient are zero.
+ * metadata = rows, vocabulary | strides of the row and the element axis of the logits | their offset.  target: device indices
+ *   [rows]; one outside [0, vocabulary) in a row that counts leaves the row out and is reported by hip_get_last_status() like an
+ *   index out of range.  old_logp, ref_logp (NULL if kl_weight is 0), advantage, weight: f32 [rows].  clip_low, clip_high >= 0.
+ * loss [1], logp [rows] (lp), lse [rows]: f32.  grad_logits [rows, vocabulary]: contiguous, of the logits' type.
+ *   hip_policy_loss_..           the loss
+ *   hip_policy_loss_backward_..  grad_logits = grad_loss[0] * (d loss / d x) from logp and lse of the forward call; grad_loss NULL: 1
+ *   hip_policy_loss_step_..      both in one pass over the logits (each read once where a row fits a block's registers)
+ * Sums are f32 (the loss f64) in a fixed order; gradients are rounded once.  Same bits on every call. */
+#define MX_DECL_POLICY_LOSS(T, S, I, IS)                                                                                      \
+    void hip_policy_loss_##S##_##IS(const size_t* metadata, const I* target, const T* logits, const float* old_logp,         \
+                                    const float* ref_logp, const float* advantage, const float* weight, float clip_low,      \
+                                    float clip_high, float kl_weight, float* loss, float* logp, float* lse);                 \
+    void hip_policy_loss_backward_##S##_##IS(const size_t* metadata, const I* target, const T* logits, const float* old_logp, \
+                                             const float* ref_logp, const float* advantage, const float* weight,             \
+                                             float clip_low, float clip_high, float kl_weight, const float* logp,            \
+                                             const float* lse, const float* grad_loss, T* grad_logits);                      \
+    void hip_policy_loss_step_##S##_##IS(const size_t* metadata, const I* target, const T* logits, const float* old_logp,    \
+                                         const float* ref_logp, const float* advantage, const float* weight, float clip_low, \
+                                         float clip_high, float kl_weight, const float* grad_loss, float* loss, float* logp, \
+                                         float* lse, T* grad_logits);
+MX_DECL_POLICY_LOSS(float, f32, int32_t, i32)
+MX_DECL_POLICY_LOSS(float, f32, int64_t, i64)
+MX_DECL_POLICY_LOSS(mx_bf16, bf16, int32_t, i32)
+MX_DECL_POLICY_LOSS(mx_bf16, bf16, int64_t, i64)
+MX_DECL_POLICY_LOSS(mx_f16, f16, int32_t, i32)
+MX_DECL_POLICY_LOSS(mx_f16, f16, int64_t, i64)
+
 /* ---- index ops -----------------------------------------------------------------------------------
  * No backend symbol exists for these in the reference: crates/maidenx_tensor/src/ops/indexing.rs runs them
  * as host loops over get / set / add_at_index (index_select :93-124, index_add_ :15-91, gather :315-363,

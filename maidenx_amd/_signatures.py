@@ -163,6 +163,20 @@ def index_signatures(dtypes=("f32", "bf16", "f16", "f64"), wide=INDEX_WIDE_DTYPE
     return sig
 
 
+def language_model_signatures(dtypes=("f32", "bf16", "f16")):
+    """Attention over packed sequences and the clipped policy loss (no counterpart in the reference)."""
+    F = C.c_float
+    sig = {}
+    for dt in dtypes:
+        sig[f"attention_{dt}"] = [P] * 6 + [F, P, P]
+        sig[f"attention_backward_{dt}"] = [P] * 6 + [F] + [P] * 7
+        for it in ("i32", "i64"):
+            sig[f"policy_loss_{dt}_{it}"] = [P] * 7 + [F] * 3 + [P] * 3
+            sig[f"policy_loss_backward_{dt}_{it}"] = [P] * 7 + [F] * 3 + [P] * 4
+            sig[f"policy_loss_step_{dt}_{it}"] = [P] * 7 + [F] * 3 + [P] * 5
+    return sig
+
+
 def extension_signatures():
     """Entry points of the HIP library that have no counterpart symbol in the reference."""
     sig = index_signatures()
@@ -180,6 +194,7 @@ def extension_signatures():
     sig["sgd_step_f32"] = [SZ, P, P, C.c_float]
     sig["conv2d_cols_matmul_f32"] = [P, C.c_int, P, P, SZ, P, P]
     sig["conv2d_col2im_add_f32"] = [SZ, P, P, P]
+    sig.update(language_model_signatures())
     sig.update(cast_signatures())
     sig.update(wide_util_signatures())
     sig.update(wide_unary_signatures())

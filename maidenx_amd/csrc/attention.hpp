@@ -1,0 +1,1035 @@
+// Causal attention over packed sequences with grouped heads and an optional learned relative position bias, forward and
+// backward, in tiles that never leave the chip.
+//
+//   S_ij = scale * q_i . k_j + table[bucket(i - j)][h]     j <= i, both in one sequence [offsets[s], offsets[s + 1])
+//   o_i  = sum_j P_ij v_j,  P_ij = exp(S_ij - lse_i),  lse_i = ln sum_j exp S_ij
+//   dP_ij = do_i . v_j;  D_i = do_i . o_i = sum_j P_ij dP_ij;  dS_ij = P_ij (dP_ij - D_i)
+//   dq_i = scale sum_j dS_ij k_j;  dk_j = scale sum_i dS_ij q_i;  dv_j = sum_i P_ij do_i   (sums over the heads of a group too)
+//   dtable[b][h] = sum of dS_ij over the pairs with bucket(i - j) = b
+//
+// Layout of the products.  All of them are 32 x 32 tiles of the matrix cores, with the fragment of a lane l (half = l / 32)
+//   operand:  row l % 32, eight terms of the sum starting at 8 * half       result:  column l % 32, rows (r % 4) + 8 (r / 4) + 4 half
+// S is formed with the index that the next product does NOT sum over in the columns: S^T = K Q^T where o and dq sum over
+// keys, S = Q K^T where dk and dv sum over queries.  A lane then holds, for its own column, eight values of every half of
+// a 32-row tile, which IS the right operand of the next product once both operands agree on the order of the terms: the
+// left operand (v, k, do, q with the summed index in the rows) is read from LDS transposed, in that order.  So P and dS
+// never travel between lanes, and the softmax statistics of a query are one register of its lane (plus one exchange of halves).
+//
+// Tiles are laid over the packed tokens, not over sequences: a row knows its sequence's first token, tiles that no mask
+// touches skip it, and a batch of short sequences fills its tiles.
+//
+// Rounding: scores, statistics and every accumulator are f32.  P and dS are rounded to the tensors' type where they become an
+// operand of the matrix cores (bf16 and f16; f32 tensors keep f32 there): the error is that of one more rounding of
+// every term, independent from term to term, and the sum over terms is as far off as the rounding of the result itself.
+#pragma once
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+
+#include "mxh.hpp"
+
+namespace mxh {
+
+constexpr int ATTN_MAX_DIM = 128;
+constexpr int ATTN_MAX_BUCKETS = 256;
+constexpr int ATTN_MAX_DISTANCE = 4096;
+constexpr int ATTN_THREADS = 256;
+constexpr int ATTN_ROWS = 128;              // rows (of queries, or of keys in the backward pass for keys) that a block owns: 32 a wave
+constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
+constexpr float ATTN_FLT_MAX = 3.402823466e+38f;
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+template <class E>
+struct AttnView {              // one [tokens, heads, dim] operand
+    const E* p;
+    int64_t token, head, elem; // strides in elements
+    int vec;                   // rows can be read in 16-byte pieces
+};
+template <class E>
+struct AttnArgs {
+    AttnView<E> q, k, v, o, go;
+    const int32_t* offsets;
+    const E* table;            // [buckets, heads], null: no bias
+    int32_t tokens, heads, group, dim, sequences;
+    int32_t buckets, exact_to, max_distance;
+    float scale, scale_log2;   // scale_log2 = |scale| * log2(e); the sign goes into an operand
+    E *out, *gq, *gk, *gv;
+    float *lse, *delta, *partial;
+    int32_t partial_tiles;
+    int* flag;
+    uint16_t borders[ATTN_MAX_BUCKETS / 2];      // distance at which bucket exact_to + 1 + m begins
+};
+
+// ---- element types -----------------------------------------------------------------------------------------------------
+template <class E> struct AttnType;
+template <> struct AttnType<bf16_t> {
+    using Frag = bf16x8_t;
+    static constexpr int CHUNK = 8;       // elements in 16 bytes
+    __device__ static f32x16_t mma(Frag a, Frag b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    __device__ static Frag pack(f32x8_t x) { return __builtin_convertvector(x, bf16x8_t); }
+    __device__ static u32x2_t pack4(f32x4_t x) { return __builtin_bit_cast(u32x2_t, __builtin_convertvector(x, bf16x4_t)); }
+    __device__ static float get(bf16_t x) { return bf2f(x); }
+    __device__ static bf16_t put(float x) { return f2bf(x); }
+    __device__ static float get(Frag f, int e) { return (float)f[e]; }
+};
+template <> struct AttnType<f16_t> {
+    using Frag = f16x8_t;
+    static constexpr int CHUNK = 8;
+    __device__ static f32x16_t mma(Frag a, Frag b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    __device__ static Frag pack(f32x8_t x) { return __builtin_convertvector(x, f16x8_t); }
+    __device__ static u32x2_t pack4(f32x4_t x) { return __builtin_bit_cast(u32x2_t, __builtin_convertvector(x, f16x4_t)); }
+    __device__ static float get(f16_t x) { return h2f(x); }
+    __device__ static f16_t put(float x) { return f2h(x); }
+    __device__ static float get(Frag f, int e) { return (float)f[e]; }
+};
+template <> struct AttnType<float> {
+    using Frag = f32x8_t;
+    static constexpr int CHUNK = 4;
+    // eight products of two terms each: term e of a lane's eight pairs the same index of both operands in either half
+    __device__ static f32x16_t mma(Frag a, Frag b, f32x16_t c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+    __device__ static Frag pack(f32x8_t x) { return x; }
+    __device__ static float get(float x) { return x; }
+    __device__ static float put(float x) { return x; }
+    __device__ static float get(Frag f, int e) { return f[e]; }
+};
+
+__device__ inline float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+// the value of the lane 32 further on (the other half of the same column)
+__device__ inline float attn_other_half(float x) { return __shfl_xor(x, 32, WAVE); }
+
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------------
+// ROWS rows of DP elements at a pitch of a power of two, in 16-byte pieces whose place within a row is XOR-ed with bits
+// of the row: the 16 lanes that a 16-byte read serves together then meet all 64 banks once (32 rows, one piece each),
+// and so do the transposed reads (4 rows, 4 neighbouring pieces each), for which rows 0..3 have to differ in the upper
+// bits of the piece's place.
+template <class E, int DP>
+struct AttnTile {
+    using T = AttnType<E>;
+    using Frag = typename T::Frag;
+    static constexpr int PITCH = (DP <= 32 ? 32 : DP <= 64 ? 64 : 128) * (int)sizeof(E);
+    static constexpr int PIECES = PITCH / 16;                // of a row in LDS
+    static constexpr int DATA = DP * (int)sizeof(E) / 16;    // of a row in memory (a multiple of 4)
+    __device__ static int swizzle(int row) {
+        if constexpr (PIECES >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+        else if constexpr (PIECES == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        else return (row >> 2) & 3;
+    }
+    __device__ static int at(int row, int piece) { return row * PITCH + ((piece ^ swizzle(row)) << 4); }
+    // rows row0 + (lane % 32), elements 16 step + 8 half ..
+    __device__ static Frag rows(const char* tile, int row0, int step, int lane) {
+        const int r = lane & 31, half = lane >> 5;
+        if constexpr (sizeof(E) == 2) {
+            return *(const Frag*)(tile + row0 * PITCH + at(r, 2 * step + half));
+        } else {
+            const f32x4_t a = *(const f32x4_t*)(tile + row0 * PITCH + at(r, 4 * step + 2 * half));
+            const f32x4_t b = *(const f32x4_t*)(tile + row0 * PITCH + at(r, 4 * step + 2 * half + 1));
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+    // column 32 block + (lane % 32), rows row0 + 4 half + (e % 4) + 8 (e / 4): the order in which a result holds its rows
+    __device__ static Frag columns(const char* tile, int row0, int block, int lane) {
+        const int half = lane >> 5;
+        if constexpr (sizeof(E) == 2) {
+            // the hardware's transposed read: 16 lanes bring 4 rows x 16 columns, lane c gets column c
+            const int c = lane & 15, r = 4 * half + (c >> 2), piece = 4 * block + 2 * ((lane >> 4) & 1) + ((c & 3) >> 1);
+            s16x4_t lo, hi;
+            lo = read4(tile + row0 * PITCH + at(r, piece) + (c & 1) * 8);
+            hi = read4(tile + row0 * PITCH + at(r + 8, piece) + (c & 1) * 8);
+            return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int col = 32 * block + (lane & 31);
+            Frag f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = *(const float*)(tile + row0 * PITCH + at(4 * half + (e & 3) + 8 * (e >> 2), col >> 2) + (col & 3) * 4);
+            return f;
+        }
+    }
+    __device__ static s16x4_t read4(const char* p) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p);
+    }
+};
+
+// 16 bytes of a row from element d on, zeros beyond dim
+template <class E>
+__device__ inline u32x4_t attn_piece(const E* row, int d, int dim, int64_t elem, int vec) {
+    constexpr int N = AttnType<E>::CHUNK;
+    u32x4_t r = {0, 0, 0, 0};
+    if (vec) {
+        if (d < dim) r = *(const u32x4_t*)(row + d);
+        return r;
+    }
+    E x[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        x[e] = E{};
+        if (d + e < dim) x[e] = row[(int64_t)(d + e) * elem];
+    }
+    __builtin_memcpy(&r, x, 16);
+    return r;
+}
+
+// A tile of ROWS tokens of one operand on its way from memory to LDS through a block's registers.
+template <class E, int DP, int ROWS>
+struct AttnStage {
+    using L = AttnTile<E, DP>;
+    static constexpr int N = (ROWS * L::DATA + ATTN_THREADS - 1) / ATTN_THREADS;
+    static constexpr bool WHOLE = ROWS * L::DATA % ATTN_THREADS == 0;
+    u32x4_t r[N];
+    // rows outside [lo, hi) become zeros
+    __device__ void load(const AttnView<E>& view, int head, int token0, int lo, int hi, int dim, int tid) {
+        const E* base = view.p + (int64_t)head * view.head;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int idx = u * ATTN_THREADS + tid, row = idx / L::DATA, piece = idx % L::DATA, token = token0 + row;
+            r[u] = u32x4_t{0, 0, 0, 0};
+            if (token >= lo && token < hi && (WHOLE || row < ROWS)) r[u] = attn_piece<E>(base + (int64_t)token * view.token, piece * L::T::CHUNK, dim, view.elem, view.vec);
+        }
+    }
+    __device__ void store(char* tile, int tid) const {
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int idx = u * ATTN_THREADS + tid;
+            if (WHOLE || idx < ROWS * L::DATA) *(u32x4_t*)(tile + L::at(idx / L::DATA, idx % L::DATA)) = r[u];
+        }
+    }
+};
+
+// Row fragments straight from memory, held for the whole loop; `sign` 1, -1 or 0 is multiplied in (exact).
+template <class E, int DP>
+__device__ inline void attn_own_rows(const AttnView<E>& view, int head, int token, bool there, int dim, int lane, float sign, typename AttnType<E>::Frag (&f)[DP / 16]) {
+    using T = AttnType<E>;
+    const E* row = view.p + (int64_t)head * view.head + (int64_t)token * view.token;
+    const uint32_t flip = sizeof(E) == 2 ? 0x80008000u : 0x80000000u;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+        u32x4_t part[sizeof(E) / 2];
+#pragma unroll
+        for (int c = 0; c < (int)sizeof(E) / 2; ++c) {
+            part[c] = u32x4_t{0, 0, 0, 0};
+            if (there && sign != 0.0f) part[c] = attn_piece<E>(row, 16 * s + 8 * (lane >> 5) + c * T::CHUNK, dim, view.elem, view.vec);
+            if (sign < 0.0f) part[c] ^= flip;
+        }
+        __builtin_memcpy(&f[s], part, sizeof(f[s]));
+    }
+}
+
+// ---- sequences -----------------------------------------------------------------------------------------------------------
+// First token of the sequence of `row` and the first token behind it; false if no sequence holds the row.  Offsets that
+// do not ascend give some bounds with first <= row < last <= tokens: never an access outside the tensors.
+__device__ inline bool attn_sequence(const int32_t* offsets, int sequences, int tokens, int row, int lane, int& first, int& last) {
+    int lo = -1, hi = tokens;
+    bool above = false;
+    if (sequences < WAVE) {
+        const int mine = lane <= sequences ? offsets[lane] : -1;
+        for (int e = 0; e <= sequences; ++e) {
+            const int off = __builtin_amdgcn_readlane(mine, e);
+            if (off <= row) { if (off > lo) lo = off; }
+            else { above = true; if (off < hi) hi = off; }
+        }
+    } else {
+        int a = 0, b = sequences + 1;              // offsets[0 .. a) <= row < offsets[b ..)
+        while (a < b) {
+            const int m = (a + b) >> 1;
+            if (offsets[m] <= row) a = m + 1;
+            else b = m;
+        }
+        if (a > 0) lo = offsets[a - 1];
+        if (a <= sequences) { above = true; hi = offsets[a]; }
+        if (hi <= row) hi = row + 1;
+    }
+    first = lo < 0 ? 0 : lo > row ? row : lo;
+    last = hi > tokens ? tokens : hi;
+    return row < tokens && lo >= 0 && above;
+}
+__device__ inline int attn_wave_min(int x) {
+#pragma unroll
+    for (int d = 1; d < WAVE; d <<= 1) { const int o = __shfl_xor(x, d, WAVE); x = o < x ? o : x; }
+    return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ inline int attn_wave_max(int x) { return -attn_wave_min(-x); }
+
+// One wave of the first block looks the offsets over; the host reports what it finds with the next status.
+template <class E>
+__device__ inline void attn_check_offsets(const AttnArgs<E>& a) {
+    if (blockIdx.x != 0 || threadIdx.x >= WAVE) return;
+    bool bad = false;
+    for (int e = threadIdx.x; e <= a.sequences; e += WAVE) {
+        const int off = a.offsets[e];
+        if (off < 0 || off > a.tokens || (e < a.sequences && a.offsets[e + 1] < off)) bad = true;
+    }
+    if (bad) *a.flag = 1;
+}
+
+// tile of rows and head of a block.  The blocks of a tile follow one another (the longest first); with a multiple of eight
+// heads, neighbouring heads - which share their keys - are eight blocks apart: on one XCD, behind one L2.
+__device__ inline void attn_place(int block, int tiles, int heads, bool last_first, int& tile, int& head) {
+    const int t = block / heads, x = block - t * heads;
+    tile = last_first ? tiles - 1 - t : t;
+    head = heads % 8 == 0 ? (x % 8) * (heads / 8) + x / 8 : x;
+}
+
+// ---- the bias ------------------------------------------------------------------------------------------------------------
+template <class E>
+__device__ inline int attn_bucket(const AttnArgs<E>& a, int distance) {
+    if (distance < a.exact_to) return distance;
+    int b = a.exact_to;
+    for (int m = 0; m < a.buckets - a.exact_to - 1; ++m) b += distance >= (int)a.borders[m];
+    return b;
+}
+// by_distance[n], n = 0 .. max_distance: the bias of head h in units of log2, the last for every distance from max_distance on
+template <class E>
+__device__ inline void attn_bias_by_distance(const AttnArgs<E>& a, int head, float* by_distance, int tid) {
+    for (int n = tid; n <= a.max_distance; n += ATTN_THREADS) {
+        const float b = AttnType<E>::get(a.table[(int64_t)attn_bucket(a, n) * a.heads + head]);
+        // a finite bias stays finite: the type's lowest value is a value like any other, only -inf takes a pair out
+        const float x = b * ATTN_LOG2E;
+        by_distance[n] = __builtin_isinf(b) ? b : x > ATTN_FLT_MAX ? ATTN_FLT_MAX : x < -ATTN_FLT_MAX ? -ATTN_FLT_MAX : x;
+    }
+}
+// Adds the bias to scores that a lane holds at distances d0 - (r % 4) - 8 (r / 4), times step (1: rows are keys, -1: queries)
+template <int STEP>
+__device__ inline void attn_add_bias(f32x16_t& s, float c, const float* by_distance, int d0, int max_distance, bool near, float far_bias) {
+    if (near) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            int n = d0 - STEP * ((r & 3) + 8 * (r >> 2));
+            n = n < 0 ? 0 : n > max_distance ? max_distance : n;
+            s[r] = __builtin_fmaf(s[r], c, by_distance[n]);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, far_bias);
+    }
+}
+
+// ---- what a mask hides -----------------------------------------------------------------------------------------------------
+// The matrix cores multiply a weight of zero by whatever the other operand holds: a NaN or an infinity in a row that the mask hides
+// from a column (a later token, another sequence) would become a NaN there.  So a block whose sums are not finite makes them
+// once more (its columns that really see such a row end as they have to), with the tiles that a mask touches term by term:
+// sums[d] += weight * tile[row][d] for the rows that `sees` lets through.  Costs nothing where everything is finite.
+template <class E, int DP, int TILES, class Sees>
+__device__ inline void attn_careful(const char* tile, const f32x16_t (&weight)[TILES], f32x16_t (&sums)[DP / 32], int lane, Sees sees) {
+    using L = AttnTile<E, DP>;
+    const int half = lane >> 5;
+#pragma nounroll
+    for (int row = 0; row < 32 * TILES; ++row) {
+        const int at = (row & 3) + 4 * ((row >> 3) & 3) + 16 * (row >> 5);      // where the lane's half of rows keeps it
+        float mine = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16 * TILES; ++r) mine = r == at ? weight[r >> 4][r & 15] : mine;
+        const float w = __shfl(mine, (lane & 31) | (((row >> 2) & 1) << 5), WAVE);
+        const bool seen = sees(row);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c0 = 32 * d + 8 * g + 4 * half;
+                E x[4];
+                __builtin_memcpy(x, tile + L::at(row, c0 * (int)sizeof(E) / 16) + c0 * (int)sizeof(E) % 16, sizeof(x));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = __builtin_fmaf(w, AttnType<E>::get(x[e]), sums[d][4 * g + e]);
+                    sums[d][4 * g + e] = seen ? y : sums[d][4 * g + e];
+                }
+            }
+    }
+}
+template <int N>
+__device__ inline bool attn_finite(const f32x16_t (&sums)[N]) {
+    bool fine = true;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) fine &= __builtin_fabsf(sums[d][r]) <= ATTN_FLT_MAX;
+    return fine;
+}
+
+// ---- forward -------------------------------------------------------------------------------------------------------------
+template <class E> constexpr int attn_keys() { return sizeof(E) == 4 ? 32 : 64; }     // keys of a tile: 64 KB of LDS for two tiles of keys and values either way
+template <class E, int DP>
+constexpr size_t attn_tile_bytes(int rows) { return (size_t)rows * AttnTile<E, DP>::PITCH; }
+
+template <class E, int DP, bool BIAS>
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles) {
+    using T = AttnType<E>;
+    using L = AttnTile<E, DP>;
+    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int span[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    char* const ktile = lds;
+    char* const vtile = lds + 2 * BN * L::PITCH;
+    float* const by_distance = (float*)(lds + 4 * BN * L::PITCH);
+    attn_check_offsets(a);
+    int tile, head;
+    attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
+    const int kv = head / a.group;
+    const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
+    int first, last;
+    const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
+    const int lo = attn_wave_min(there ? first : 0x7fffffff), hi = attn_wave_max(there ? row + 1 : 0);   // keys this wave needs
+    const int inner = attn_wave_max(there ? first : 0x7fffffff);                                        // from here on all rows share the keys
+    const int top = attn_wave_min(there ? row : -1);                                                   // ... and up to here
+    if (lane == 0) { span[wave] = lo; span[4 + wave] = hi; }
+    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
+    typename T::Frag q[KS];
+    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, q);
+    __syncthreads();
+    int begin = span[0], end = span[4];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        begin = span[w] < begin ? span[w] : begin;
+        end = span[4 + w] > end ? span[4 + w] : end;
+    }
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    if (end <= begin) return;                       // no row of the block is in a sequence
+
+    const int lower = there ? first : -1;           // key j is seen if (unsigned)(j - lower) <= reach
+    const uint32_t reach = there ? (uint32_t)(row - first) : 0;
+    const float c = a.scale_log2;
+    f32x16_t acc[DB];
+    float m, l;
+    int careful = 0;
+    for (;;) {
+    careful = __builtin_amdgcn_readfirstlane(careful);
+    asm volatile("" : "+s"(careful));               // one loop for both ways through it
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
+    m = -INFINITY;
+    l = 0.0f;
+    AttnStage<E, DP, BN> ks, vs;
+    ks.load(a.k, kv, begin, begin, end, a.dim, tid);
+    vs.load(a.v, kv, begin, begin, end, a.dim, tid);
+    ks.store(ktile, tid);
+    vs.store(vtile, tid);
+    __syncthreads();
+    int buf = 0;
+    for (int j0 = begin; j0 < end; j0 += BN, buf ^= 1) {
+        const bool more = j0 + BN < end;
+        if (more) {
+            ks.load(a.k, kv, j0 + BN, begin, end, a.dim, tid);
+            vs.load(a.v, kv, j0 + BN, begin, end, a.dim, tid);
+        }
+        const char* const kt = ktile + buf * BN * L::PITCH;
+        const char* const vt = vtile + buf * BN * L::PITCH;
+        if (j0 < hi && j0 + BN > lo) {
+            f32x16_t s[JB];
+#pragma unroll
+            for (int b = 0; b < JB; ++b) {
+                s[b] = f32x16_t{};
+#pragma unroll
+                for (int k = 0; k < KS; ++k) s[b] = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s[b]);
+            }
+            const int j = j0 + 4 * half;            // key of row 0 of the lane's results
+            if (BIAS) {
+                const bool near = row0 - (j0 + BN - 1) < a.max_distance;
+                const float far_bias = by_distance[a.max_distance];
+#pragma unroll
+                for (int b = 0; b < JB; ++b) attn_add_bias<1>(s[b], c, by_distance, row - j - 32 * b, a.max_distance, near, far_bias);
+            }
+            const bool masked = j0 < inner || j0 + BN - 1 > top;
+            if (masked) {
+#pragma unroll
+                for (int b = 0; b < JB; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if ((uint32_t)(j + 32 * b + (r & 3) + 8 * (r >> 2) - lower) > reach) s[b][r] = -INFINITY;
+            }
+            float best = s[0][0];
+#pragma unroll
+            for (int b = 0; b < JB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
+            best = fmaxf(best, attn_other_half(best));
+            const float cc = BIAS ? 1.0f : c;
+            best = BIAS ? best : best * c;
+            const float next = fmaxf(m, best);
+            if (__any(next > m)) {
+                const float fix = next == -INFINITY ? 1.0f : attn_exp2(m - next);
+                l *= fix;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] *= fix;
+                m = next;
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int b = 0; b < JB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[b][r] = attn_exp2(BIAS ? s[b][r] - base : __builtin_fmaf(s[b][r], cc, -base));
+                    l += s[b][r];
+                }
+            if (careful && masked) {
+                attn_careful<E, DP, JB>(vt, s, acc, lane, [&](int r) { return (uint32_t)(j0 + r - lower) <= reach; });
+            } else
+#pragma unroll
+            for (int b = 0; b < JB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f32x8_t p;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) p[e] = s[b][8 * h + e];
+                    const typename T::Frag pf = T::pack(p);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] = T::mma(L::columns(vt, 32 * b + 16 * h, d, lane), pf, acc[d]);
+                }
+        }
+        if (more) {
+            ks.store(ktile + (buf ^ 1) * BN * L::PITCH, tid);
+            vs.store(vtile + (buf ^ 1) * BN * L::PITCH, tid);
+        }
+        __syncthreads();
+    }
+    if (careful || !__syncthreads_or(!attn_finite(acc))) break;
+    careful = 1;
+    }
+    l += attn_other_half(l);
+    if (!there) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing but -inf: an output of zeros
+    if (half == 0) a.lse[(int64_t)head * a.tokens + row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * ATTN_LN2;
+    E* const out = a.out + ((int64_t)row * a.heads + head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int at = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
+            if (at < a.dim) out[at] = T::put(acc[d][r] * inv);
+        }
+}
+
+// ---- backward: gradients of the queries ------------------------------------------------------------------------------------
+// A block owns 128 queries like the forward kernel.  Writes dq (if wanted) and, for the kernel of the keys, D_i: with a
+// bias the one that makes the row of dS sum to zero (formed from P and dP themselves; the rounding of o in do . o
+// would otherwise enter every pair of the far bucket with the same sign).
+template <class E, int DP, bool BIAS>
+__global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles) {
+    using T = AttnType<E>;
+    using L = AttnTile<E, DP>;
+    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int span[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    char* const ktile = lds;
+    char* const vtile = lds + 2 * BN * L::PITCH;
+    float* const by_distance = (float*)(lds + 4 * BN * L::PITCH);
+    attn_check_offsets(a);
+    int tile, head;
+    attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
+    const int kv = head / a.group;
+    const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
+    int first, last;
+    const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
+    const int lo = attn_wave_min(there ? first : 0x7fffffff), hi = attn_wave_max(there ? row + 1 : 0);
+    const int inner = attn_wave_max(there ? first : 0x7fffffff);
+    const int top = attn_wave_min(there ? row : -1);
+    if (lane == 0) { span[wave] = lo; span[4 + wave] = hi; }
+    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
+    typename T::Frag q[KS], go[KS];
+    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, q);
+    attn_own_rows<E, DP>(a.go, head, there ? row : 0, there, a.dim, lane, 1.0f, go);
+    float delta = 0.0f, lse2 = INFINITY;
+    {
+        typename T::Frag o[KS];
+        attn_own_rows<E, DP>(a.o, head, there ? row : 0, there, a.dim, lane, 1.0f, o);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(T::get(go[k], e), T::get(o[k], e), delta);
+        delta += attn_other_half(delta);
+    }
+    if (there) {
+        const float x = a.lse[(int64_t)head * a.tokens + row];
+        lse2 = x == -INFINITY ? INFINITY : x * ATTN_LOG2E;       // a row of nothing but -inf: P is zero
+    }
+    __syncthreads();
+    int begin = span[0], end = span[4];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        begin = span[w] < begin ? span[w] : begin;
+        end = span[4 + w] > end ? span[4 + w] : end;
+    }
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    if (end <= begin) return;
+    if (!a.gq && !(BIAS && (a.gk || a.partial))) {       // only D_i is wanted, if that
+        if (there && half == 0) a.delta[(int64_t)head * a.tokens + row] = delta;
+        return;
+    }
+    const int lower = there ? first : -1;
+    const uint32_t reach = there ? (uint32_t)(row - first) : 0;
+    const float c = a.scale_log2;
+    f32x16_t acc[DB];
+    float rest;
+    int careful = 0;
+    for (;;) {
+    careful = __builtin_amdgcn_readfirstlane(careful);
+    asm volatile("" : "+s"(careful));
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
+    rest = 0.0f;
+    AttnStage<E, DP, BN> ks, vs;
+    ks.load(a.k, kv, begin, begin, end, a.dim, tid);
+    vs.load(a.v, kv, begin, begin, end, a.dim, tid);
+    ks.store(ktile, tid);
+    vs.store(vtile, tid);
+    __syncthreads();
+    int buf = 0;
+    for (int j0 = begin; j0 < end; j0 += BN, buf ^= 1) {
+        const bool more = j0 + BN < end;
+        if (more) {
+            ks.load(a.k, kv, j0 + BN, begin, end, a.dim, tid);
+            vs.load(a.v, kv, j0 + BN, begin, end, a.dim, tid);
+        }
+        const char* const kt = ktile + buf * BN * L::PITCH;
+        const char* const vt = vtile + buf * BN * L::PITCH;
+        if (j0 < hi && j0 + BN > lo) {
+            const bool masked = j0 < inner || j0 + BN - 1 > top;
+            const bool near = BIAS && row0 - (j0 + BN - 1) < a.max_distance;
+            const float far_bias = BIAS ? by_distance[a.max_distance] : 0.0f;
+#pragma unroll
+            for (int b = 0; b < JB; ++b) {
+                f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+#pragma unroll
+                for (int k = 0; k < KS; ++k) s = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s);
+#pragma unroll
+                for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(vt, 32 * b, k, lane), go[k], dp);
+                const int j = j0 + 32 * b + 4 * half;
+                if (BIAS) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance, near, far_bias);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[r] = attn_exp2(BIAS ? s[r] - lse2 : __builtin_fmaf(s[r], c, -lse2));
+                    s[r] *= dp[r] - delta;
+                    if (masked && (uint32_t)(j + (r & 3) + 8 * (r >> 2) - lower) > reach) s[r] = 0.0f;
+                    if (BIAS) rest += s[r];
+                }
+                if (careful && masked) {
+                    const f32x16_t w[1] = {s};
+                    attn_careful<E, DP, 1>(kt + 32 * b * L::PITCH, w, acc, lane, [&](int r) { return (uint32_t)(j0 + 32 * b + r - lower) <= reach; });
+                } else
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f32x8_t p;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) p[e] = s[8 * h + e];
+                    const typename T::Frag pf = T::pack(p);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] = T::mma(L::columns(kt, 32 * b + 16 * h, d, lane), pf, acc[d]);
+                }
+            }
+        }
+        if (more) {
+            ks.store(ktile + (buf ^ 1) * BN * L::PITCH, tid);
+            vs.store(vtile + (buf ^ 1) * BN * L::PITCH, tid);
+        }
+        __syncthreads();
+    }
+    if (careful || !__syncthreads_or(!attn_finite(acc))) break;
+    careful = 1;
+    }
+    if (BIAS) rest += attn_other_half(rest);
+    if (!there) return;
+    if (half == 0 && a.delta) a.delta[(int64_t)head * a.tokens + row] = BIAS ? delta + rest : delta;
+    if (!a.gq) return;
+    E* const out = a.gq + ((int64_t)row * a.heads + head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int at = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
+            if (at < a.dim) out[at] = T::put(acc[d][r] * a.scale);
+        }
+}
+
+// ---- backward: gradients of the keys, the values and the bias table ----------------------------------------------------------
+// A block owns 128 keys of one key head and walks the queries of every head of its group from there on: the sums over
+// shared heads are made in registers, in a fixed order.
+template <class E, int DP, bool BIAS>
+__global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles) {
+    using T = AttnType<E>;
+    using L = AttnTile<E, DP>;
+    constexpr int BM = 32, DB = DP / 32, KS = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int span[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    char* const qtile = lds;
+    char* const otile = lds + 2 * BM * L::PITCH;
+    float* const stats = (float*)(lds + 4 * BM * L::PITCH);      // [2][lse2 | delta][BM]
+    float* const corner = stats + 4 * BM + wave * (32 * 33 + 64);   // (BIAS) a tile of dS of this wave, and the sums of its diagonals
+    float* const by_distance = stats + 4 * BM + 4 * (32 * 33 + 64);
+    const int kv_heads = a.heads / a.group;
+    int tile, kv;
+    attn_place(blockIdx.x, tiles, kv_heads, false, tile, kv);
+    const int key0 = tile * ATTN_ROWS + wave * 32, key = key0 + (lane & 31);
+    int first, last;
+    const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, key, lane, first, last);
+    const int lo = attn_wave_min(there ? key : 0x7fffffff), hi = attn_wave_max(there ? last : 0);     // queries this wave needs
+    const int inner = attn_wave_max(there ? key : 0x7fffffff), top = attn_wave_min(there ? last : 0); // queries that see every key
+    if (lane == 0) { span[wave] = lo; span[4 + wave] = hi; }
+    typename T::Frag k[KS], v[KS];
+    attn_own_rows<E, DP>(a.k, kv, there ? key : 0, there, a.dim, lane, a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, k);
+    attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
+    __syncthreads();
+    int begin = span[0], end = span[4];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        begin = span[w] < begin ? span[w] : begin;
+        end = span[4 + w] > end ? span[4 + w] : end;
+    }
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+    const uint32_t reach = there ? (uint32_t)(last - key) : 0;       // query i sees the key if (unsigned)(i - key) < reach
+    const float c = a.scale_log2;
+    f32x16_t gk[DB], gv[DB];
+    const int head0 = kv * a.group;
+    const int steps = end > begin ? (end - begin + BM - 1) / BM : 0, total = steps * a.group;
+    AttnStage<E, DP, BM> qs, os;
+    float stat = 0.0f;
+    auto fetch = [&](int n) {
+        const int head = head0 + n / steps, i0 = begin + (n % steps) * BM;
+        qs.load(a.q, head, i0, begin, end, a.dim, tid);
+        os.load(a.go, head, i0, begin, end, a.dim, tid);
+        if (tid < 2 * BM) {
+            const int i = i0 + tid % BM;
+            const bool in = i < end;
+            const float x = in ? (tid < BM ? a.lse : a.delta)[(int64_t)head * a.tokens + i] : 0.0f;
+            stat = tid >= BM ? x : !in || x == -INFINITY ? INFINITY : x * ATTN_LOG2E;
+        }
+    };
+    auto stash = [&](int buf) {
+        qs.store(qtile + buf * BM * L::PITCH, tid);
+        os.store(otile + buf * BM * L::PITCH, tid);
+        if (tid < 2 * BM) stats[buf * 2 * BM + tid] = stat;
+    };
+    float in_bucket[ATTN_MAX_BUCKETS / WAVE] = {0.0f, 0.0f, 0.0f, 0.0f}, far_sum = 0.0f;    // of the head at hand
+    int careful = 0;
+    for (;;) {
+    careful = __builtin_amdgcn_readfirstlane(careful);
+    asm volatile("" : "+s"(careful));
+#pragma unroll
+    for (int d = 0; d < DB; ++d) { gk[d] = f32x16_t{}; gv[d] = f32x16_t{}; }
+    if (total) {
+        fetch(0);
+        stash(0);
+    }
+    if (BIAS) {
+        attn_bias_by_distance(a, head0, by_distance, tid);
+    }
+    __syncthreads();
+    int buf = 0, step = 0, head = head0;
+    for (int n = 0; n < total; ++n, buf ^= 1) {
+        const bool more = n + 1 < total;
+        if (more) fetch(n + 1);
+        const int i0 = begin + step * BM;
+        const char* const qt = qtile + buf * BM * L::PITCH;
+        const char* const ot = otile + buf * BM * L::PITCH;
+        const float* const st = stats + buf * 2 * BM;
+        if (i0 < hi && i0 + BM > lo) {
+            f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+#pragma unroll
+            for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, 0, x, lane), k[x], s);
+#pragma unroll
+            for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, 0, x, lane), v[x], dp);
+            const int i = i0 + 4 * half;
+            const bool masked = i0 < inner || i0 + BM > top;
+            const bool near = BIAS && i0 - (key0 + 31) < a.max_distance;
+            if (BIAS) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance, near, by_distance[a.max_distance]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4_t ls = *(const f32x4_t*)(st + 8 * g + 4 * half), de = *(const f32x4_t*)(st + BM + 8 * g + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * g + e;
+                    float p = attn_exp2(BIAS ? s[r] - ls[e] : __builtin_fmaf(s[r], c, -ls[e]));
+                    float x = p * (dp[r] - de[e]);
+                    if (masked && (uint32_t)(i + e + 8 * g - key) >= reach) p = x = 0.0f;
+                    s[r] = p;
+                    dp[r] = x;
+                }
+            }
+            if (careful && masked) {
+                const f32x16_t pw[1] = {s}, xw[1] = {dp};
+                const auto sees = [&](int r) { return (uint32_t)(i0 + r - key) < reach; };
+                attn_careful<E, DP, 1>(ot, pw, gv, lane, sees);
+                attn_careful<E, DP, 1>(qt, xw, gk, lane, sees);
+            } else
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f32x8_t p, x;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { p[e] = s[8 * h + e]; x[e] = dp[8 * h + e]; }
+                const typename T::Frag pf = T::pack(p), xf = T::pack(x);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) gv[d] = T::mma(L::columns(ot, 16 * h, d, lane), pf, gv[d]);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) gk[d] = T::mma(L::columns(qt, 16 * h, d, lane), xf, gk[d]);
+            }
+            if (BIAS && a.partial) {
+                if (!near) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) far_sum += dp[r];
+                } else {
+                    // The tile of dS by diagonals (distance n = i - key has one value on each), then by buckets: lane b adds
+                    // up what belongs to bucket b (+ 64 u).  Fixed order throughout.
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = dp[r];
+                    __builtin_amdgcn_wave_barrier();
+                    const int n0 = i0 - key0 - 31;                    // distance of diagonal 0
+                    float on = 0.0f;
+                    for (int col = 0; col < 32; ++col) {
+                        const int r = lane + col - 31;                // r - col = lane - 31
+                        if (r >= 0 && r < 32) on += corner[r * 33 + col];
+                    }
+                    corner[32 * 33 + lane] = lane < 63 ? on : 0.0f;
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
+                        const int b = lane + u * WAVE;
+                        if (u * WAVE < a.buckets && b < a.buckets) {
+                            const int from = b <= a.exact_to ? b : (int)a.borders[b - a.exact_to - 1];
+                            const int upto = b + 1 == a.buckets ? 1 << 30 : b + 1 <= a.exact_to ? b + 1 : (int)a.borders[b - a.exact_to];
+                            const int t0 = from - n0 > 0 ? from - n0 : 0, t1 = upto - n0 < 63 ? upto - n0 : 63;
+                            for (int t = t0; t < t1; ++t) in_bucket[u] += corner[32 * 33 + t];
+                        }
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                }
+            }
+        }
+        const bool turn = ++step == steps;
+        if (turn) {
+            step = 0;
+            if (BIAS && a.partial) {
+#pragma unroll
+                for (int d = 32; d > 0; d >>= 1) far_sum += __shfl_xor(far_sum, d, WAVE);
+#pragma unroll
+                for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
+                    const int b = lane + u * WAVE;
+                    if (b < a.buckets) a.partial[((int64_t)head * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = in_bucket[u] + (b + 1 == a.buckets ? far_sum : 0.0f);
+                    in_bucket[u] = 0.0f;
+                }
+                far_sum = 0.0f;
+            }
+            ++head;
+        }
+        if (more) stash(buf ^ 1);
+        __syncthreads();
+        if (BIAS && turn && more) {
+            attn_bias_by_distance(a, head, by_distance, tid);
+            __syncthreads();
+        }
+    }
+    if (careful || !__syncthreads_or(!attn_finite(gk) || !attn_finite(gv))) break;
+    careful = 1;
+    }
+    if (BIAS && a.partial && total == 0)      // no key of the block is in a sequence
+        for (int g = 0; g < a.group; ++g)
+            for (int b = lane; b < a.buckets; b += WAVE) a.partial[((int64_t)(head0 + g) * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = 0.0f;
+    if (!there) return;
+    const int64_t out = ((int64_t)key * kv_heads + kv) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int at = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
+            if (at < a.dim) {
+                if (a.gk) a.gk[out + at] = T::put(gk[d][r] * a.scale);
+                if (a.gv) a.gv[out + at] = T::put(gv[d][r]);
+            }
+        }
+}
+
+// dtable[b][h]: the partial sums of the key tiles, in their order
+template <class E>
+__global__ __launch_bounds__(ATTN_THREADS) void attn_grad_table_kernel(const float* partial, int tiles, int buckets, int heads, E* table) {
+    const int b = blockIdx.x, h = blockIdx.y;
+    __shared__ float sum[ATTN_THREADS / WAVE];
+    float x = 0.0f;
+    for (int t = threadIdx.x; t < tiles; t += ATTN_THREADS) x += partial[((int64_t)h * tiles + t) * buckets + b];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, WAVE);
+    if (threadIdx.x % WAVE == 0) sum[threadIdx.x / WAVE] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) table[(int64_t)b * heads + h] = AttnType<E>::put((sum[0] + sum[1]) + (sum[2] + sum[3]));
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+// attention.hip: least whole distance n with (n / E)^M >= (X / E)^m for m = 1 .. M - 1, exactly
+bool attn_borders(int buckets, int max_distance, uint16_t* borders);
+
+template <class E>
+inline bool attn_view(AttnView<E>& v, const void* base, const size_t* strides, size_t offset, int dim) {
+    v.p = (const E*)base + offset;
+    v.token = (int64_t)strides[0];
+    v.head = (int64_t)strides[1];
+    v.elem = (int64_t)strides[2];
+    constexpr size_t N = AttnType<E>::CHUNK;
+    v.vec = (strides[2] == 1 || dim == 1) && dim % N == 0 && strides[0] % N == 0 && strides[1] % N == 0 && (uintptr_t)v.p % 16 == 0;
+    return true;
+}
+
+// metadata: tokens, heads, kv_heads, dim, sequences, buckets, max_distance | q, k, v strides | q, k, v offsets
+template <class E>
+inline bool attn_arguments(AttnArgs<E>& a, const size_t* md, const int32_t* offsets, const E* q, const E* k, const E* v, const E* table, float scale) {
+    if (!md || !offsets || !q || !k || !v) { set_status(ERR_INVALID, "attention: null argument"); return false; }
+    const size_t tokens = md[0], heads = md[1], kv = md[2], dim = md[3], sequences = md[4];
+    if (heads == 0 || kv == 0 || dim == 0 || heads % kv != 0) { set_status(ERR_INVALID, "attention: heads must be a multiple of kv_heads, and dim positive"); return false; }
+    if (dim > (size_t)ATTN_MAX_DIM) { set_status(ERR_UNSUPPORTED, "attention: head dimension above 128"); return false; }
+    if (tokens >= (1ull << 31) - 1024 || sequences >= (1ull << 31) - 1024 || heads > 65535) { set_status(ERR_TOO_LARGE, "attention: too many tokens, sequences or heads"); return false; }
+    if (((tokens + ATTN_ROWS - 1) / ATTN_ROWS) * heads >= (1ull << 31)) { set_status(ERR_TOO_LARGE, "attention: too many tiles"); return false; }
+    std::memset((void*)&a, 0, sizeof(a));
+    attn_view(a.q, q, md + 7, md[16], (int)dim);
+    attn_view(a.k, k, md + 10, md[17], (int)dim);
+    attn_view(a.v, v, md + 13, md[18], (int)dim);
+    a.offsets = offsets;
+    a.table = table;
+    a.tokens = (int32_t)tokens;
+    a.heads = (int32_t)heads;
+    a.group = (int32_t)(heads / kv);
+    a.dim = (int32_t)dim;
+    a.sequences = (int32_t)sequences;
+    a.scale = scale;
+    a.scale_log2 = (scale == 0.0f ? 1.0f : std::fabs(scale)) * ATTN_LOG2E;
+    if (table) {
+        const size_t buckets = md[5], distance = md[6];
+        if (buckets < 2 || buckets > (size_t)ATTN_MAX_BUCKETS) { set_status(ERR_UNSUPPORTED, "attention: a bias takes 2 to 256 buckets"); return false; }
+        if (distance <= buckets / 2 || distance > (size_t)ATTN_MAX_DISTANCE) { set_status(ERR_UNSUPPORTED, "attention: max_distance lies above buckets / 2 and up to 4096"); return false; }
+        a.buckets = (int32_t)buckets;
+        a.exact_to = (int32_t)(buckets / 2);
+        a.max_distance = (int32_t)distance;
+        if (!attn_borders((int)buckets, (int)distance, a.borders)) return false;
+    }
+    a.flag = index_flag();
+    return a.flag != nullptr;
+}
+
+// more than 64 KB of LDS has to be asked for, once for each kernel and device
+inline bool attn_lds(const void* kernel, size_t bytes, uint64_t& asked) {
+    if (bytes <= 65536) return true;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) { set_status(ERR_INVALID, "attention: bad device"); return false; }
+    if (asked >> dev & 1) return true;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 1024);
+    if (e != hipSuccess) { set_status(ERR_LAUNCH, "attention: LDS size", (int)e); return false; }
+    asked |= 1ull << dev;
+    return true;
+}
+
+template <class E, int DP, bool BIAS>
+inline void attn_forward_launch(const AttnArgs<E>& a) {
+    static uint64_t asked = 0;
+    const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS;
+    const size_t lds = 4 * attn_tile_bytes<E, DP>(attn_keys<E>()) + (BIAS ? ((size_t)a.max_distance + 1) * 4 : 0);
+    auto* kernel = attn_forward_kernel<E, DP, BIAS>;
+    if (!attn_lds((const void*)kernel, lds, asked)) return;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.heads)), dim3(ATTN_THREADS), lds, stream(), a, tiles);
+    MXH_LAUNCH_CHECK("attention");
+}
+template <class E, int DP, bool BIAS>
+inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
+    static uint64_t asked_q = 0, asked_k = 0;
+    const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS;
+    const size_t bias = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
+    {
+        const size_t lds = 4 * attn_tile_bytes<E, DP>(attn_keys<E>()) + bias;
+        auto* kernel = attn_grad_query_kernel<E, DP, BIAS>;
+        if (!attn_lds((const void*)kernel, lds, asked_q)) return;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.heads)), dim3(ATTN_THREADS), lds, stream(), a, tiles);
+        MXH_LAUNCH_CHECK("attention_backward (queries)");
+    }
+    if (a.gk || a.gv || grad_table) {
+        const size_t lds = 4 * attn_tile_bytes<E, DP>(32) + 4 * 32 * 4 + (BIAS ? (size_t)4 * (32 * 33 + 64) * 4 : 0) + bias;
+        auto* kernel = attn_grad_key_kernel<E, DP, BIAS>;
+        if (!attn_lds((const void*)kernel, lds, asked_k)) return;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * (a.heads / a.group))), dim3(ATTN_THREADS), lds, stream(), a, tiles);
+        MXH_LAUNCH_CHECK("attention_backward (keys)");
+    }
+    if (grad_table) {
+        hipLaunchKernelGGL(attn_grad_table_kernel<E>, dim3((unsigned)a.buckets, (unsigned)a.heads), dim3(ATTN_THREADS), 0, stream(), a.partial, a.partial_tiles, a.buckets, a.heads, grad_table);
+        MXH_LAUNCH_CHECK("attention_backward (bias)");
+    }
+}
+// the head dimension is padded with zeros to 32, 64, 96 or 128
+template <class E, class F>
+inline void attn_by_dim(const AttnArgs<E>& a, F&& f) {
+    if (a.dim <= 32) f(std::integral_constant<int, 32>{});
+    else if (a.dim <= 64) f(std::integral_constant<int, 64>{});
+    else if (a.dim <= 96) f(std::integral_constant<int, 96>{});
+    else f(std::integral_constant<int, 128>{});
+}
+
+template <class E>
+inline void attention_entry(const size_t* md, const int32_t* offsets, const E* q, const E* k, const E* v, const E* table, float scale, E* out, float* lse) {
+    AttnArgs<E> a;
+    if (!out || !lse) { set_status(ERR_INVALID, "attention: null output"); return; }
+    if (!attn_arguments(a, md, offsets, q, k, v, table, scale)) return;
+    if (a.tokens == 0 || a.sequences == 0) return;
+    a.out = out;
+    a.lse = lse;
+    attn_by_dim(a, [&](auto dp) {
+        if (table) attn_forward_launch<E, decltype(dp)::value, true>(a);
+        else attn_forward_launch<E, decltype(dp)::value, false>(a);
+    });
+}
+
+template <class E>
+inline void attention_backward_entry(const size_t* md, const int32_t* offsets, const E* q, const E* k, const E* v, const E* table, float scale, const E* out,
+                                     const float* lse, const E* grad_out, E* gq, E* gk, E* gv, E* grad_table) {
+    AttnArgs<E> a;
+    if (!out || !lse || !grad_out) { set_status(ERR_INVALID, "attention_backward: null argument"); return; }
+    if (grad_table && !table) { set_status(ERR_INVALID, "attention_backward: the gradient of a bias that was not given"); return; }
+    if (!attn_arguments(a, md, offsets, q, k, v, table, scale)) return;
+    if (!gq && !gk && !gv && !grad_table) return;
+    const size_t rows[3] = {(size_t)a.heads * a.dim, (size_t)a.dim, 1};
+    attn_view(a.o, out, rows, 0, a.dim);
+    attn_view(a.go, grad_out, rows, 0, a.dim);
+    a.lse = (float*)lse;
+    a.gq = gq;
+    a.gk = gk;
+    a.gv = gv;
+    const bool empty = a.tokens == 0 || a.sequences == 0;
+    if (empty && !grad_table) return;
+    const size_t deltas = ((size_t)a.heads * a.tokens + 63) / 64 * 64;
+    a.partial_tiles = empty ? 0 : 4 * ((a.tokens + ATTN_ROWS - 1) / ATTN_ROWS);
+    const size_t partials = grad_table ? (size_t)a.heads * a.partial_tiles * a.buckets : 0;
+    a.delta = (float*)scratch((deltas + partials) * sizeof(float));
+    if (!a.delta) return;
+    a.partial = grad_table ? a.delta + deltas : nullptr;
+    if (empty) {
+        hipLaunchKernelGGL(attn_grad_table_kernel<E>, dim3((unsigned)a.buckets, (unsigned)a.heads), dim3(ATTN_THREADS), 0, stream(), a.partial, 0, a.buckets, a.heads, grad_table);
+        MXH_LAUNCH_CHECK("attention_backward (bias)");
+        return;
+    }
+    attn_by_dim(a, [&](auto dp) {
+        if (table) attn_backward_launch<E, decltype(dp)::value, true>(a, grad_table);
+        else attn_backward_launch<E, decltype(dp)::value, false>(a, grad_table);
+    });
+}
+
+#define MXH_ATTENTION(E, S)                                                                                                                          \
+    extern "C" void hip_attention_##S(const size_t* metadata, const int32_t* offsets, const E* query, const E* key, const E* value, const E* bias,   \
+                                      float scale, E* output, float* lse) { MXH_API;                                                                 \
+        ::mxh::attention_entry<E>(metadata, offsets, query, key, value, bias, scale, output, lse);                                                   \
+    }                                                                                                                                                \
+    extern "C" void hip_attention_backward_##S(const size_t* metadata, const int32_t* offsets, const E* query, const E* key, const E* value,         \
+                                               const E* bias, float scale, const E* output, const float* lse, const E* grad_output, E* grad_query,   \
+                                               E* grad_key, E* grad_value, E* grad_bias) { MXH_API;                                                  \
+        ::mxh::attention_backward_entry<E>(metadata, offsets, query, key, value, bias, scale, output, lse, grad_output, grad_query, grad_key,        \
+                                           grad_value, grad_bias);                                                                                   \
+    }
+
+}  // namespace mxh

@@ -623,7 +623,7 @@ static void collect_index_flag() {
     if (hipMemcpy(&v, p, sizeof(int), hipMemcpyDeviceToHost) != hipSuccess) return;
     if (v != 0) {
         (void)hipMemset(p, 0, sizeof(int));
-        set_status(ERR_INVALID, "index out of bounds in index_select / index_add_ / gather / scatter_add_ / bincount");
+        set_status(ERR_INVALID, "index out of bounds in index_select / index_add_ / gather / scatter_add_ / bincount, the offsets of attention or the targets of policy_loss");
     }
 }
 

@@ -1,0 +1,287 @@
+"""Attention over packed sequences on the GPU against plain numpy in 64 bits; every bound is derived in language.py."""
+import numpy as np
+import pytest
+
+import maidenx_amd.lib as L
+from helpers import to_float, to_storage
+from language import Attention, borders
+
+pytestmark = pytest.mark.gpu
+ALL = ["f32", "bf16", "f16"]
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("lengths,lead,tail", [([1], 0, 0), ([2], 0, 0), ([31], 0, 0), ([32, 33], 0, 0), ([64, 1, 65], 0, 0), ([129], 0, 0), ([300, 0, 0, 211, 1, 1, 77], 3, 9),
+                                               ([0, 0, 5, 0], 0, 2), ([17] * 40, 1, 0)])
+def test_lengths(hip, dt, lengths, lead, tail):
+    Attention(dt, lengths, 4, 2, 64, lead=lead, tail=tail, seed=len(lengths)).check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("dim", [1, 5, 8, 16, 31, 32, 40, 64, 72, 80, 96, 100, 128])
+def test_head_sizes(hip, dt, dim):
+    Attention(dt, [90, 50], 2, 1, dim, seed=dim).check(hip)
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (6, 2), (8, 8), (8, 1), (16, 4), (5, 5)])
+def test_grouped_heads(hip, heads, kv):
+    Attention("bf16", [70, 150], heads, kv, 32, seed=heads).check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("layout", ["fused", "heads first", "elements first", "odd", "shared"])
+@pytest.mark.parametrize("dim", [64, 24])
+def test_layouts(hip, dt, layout, dim):
+    Attention(dt, [100, 41], 4, 2, dim, layout=layout, seed=5).check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1.0, 1e-6])
+def test_scales(hip, dt, scale):
+    Attention(dt, [70, 20], 2, 2, 32, scale=scale, seed=6).check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("buckets,distance,dim", [(32, 128, 64), (32, 256, 128), (2, 2, 32), (7, 20, 32), (16, 64, 96), (64, 1000, 64), (256, 4096, 32), (3, 4096, 32)])
+def test_bias(hip, dt, buckets, distance, dim):
+    Attention(dt, [333, 1, 160], 4, 2, dim, buckets=buckets, distance=distance, seed=buckets).check(hip)
+
+
+@pytest.mark.parametrize("lengths", [[1], [40], [200, 0, 64], [17] * 30, [700]])
+def test_bias_lengths(hip, lengths):
+    Attention("bf16", lengths, 3, 1, 64, buckets=32, distance=128, lead=2, tail=5, seed=7).check(hip)
+
+
+@pytest.mark.parametrize("buckets,distance", [(32, 256), (32, 128), (20, 640), (256, 4096), (5, 100)])
+def test_buckets_begin_where_the_definition_says(hip, buckets, distance):
+    """q . k is zero, one bucket's bias is 40 above the others: a row's output is the mean of the values in that bucket, and a
+    distance too many or too few moves it by a half.  (Rounding: at most 2^-24 (1500 + 12) of values up to 1500.)"""
+    first = borders(buckets, distance)
+    n = min(first[-1] + 40, 1500)
+    for b in sorted({0, buckets // 2 - 1, buckets // 2, buckets // 2 + 1, max(x for x in range(buckets) if first[x] < n - 1), buckets - 2, buckets - 1}):
+        if first[b] >= n:
+            continue
+        a = Attention("f32", [n], 1, 1, 1, buckets=buckets, distance=distance, seed=b)
+        a.q[:] = 0
+        a.table[:] = 0
+        a.table[b] = 40
+        a.v[:, 0, 0] = np.arange(n)
+        upto = first[b + 1] if b + 1 < buckets else n + 1
+        out, _ = a.forward(hip)
+        rows = np.arange(n)
+        want = rows - (first[b] + np.minimum(upto - 1, rows)) / 2
+        seen = rows >= first[b]
+        assert np.abs(out[seen, 0, 0] - want[seen]).max() < 0.25
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_large_scores(hip, dt):
+    """Scores of some hundreds: one key takes all, sums that a softmax without the running maximum would overflow."""
+    Attention(dt, [150], 2, 1, 64, spread=8.0, scale=0.5, seed=11).check(hip, gradients=dt != "f16")
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("what", ["first", "far", "all"])
+def test_rows_that_a_bias_leaves_empty(hip, dt, what):
+    """A table with -inf: rows whose every pair is out have zeros, lse -inf and no gradient."""
+    a = Attention(dt, [70, 1, 40], 2, 1, 32, buckets=8, distance=16, seed=12)
+    a.table[{"first": slice(0, 1), "far": slice(3, 8), "all": slice(0, 8)}[what]] = -np.inf
+    a.check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_the_lowest_value_is_a_value(hip, dt):
+    """A bias of the type's lowest value on every bucket but those from 4 on: rows near the start have nothing else and are
+    the mean over their keys, since q . k is lost beside it."""
+    a = Attention(dt, [40], 2, 2, 16, buckets=8, distance=16, seed=13)
+    lowest = float(to_float(np.array([{"f32": np.float32(-3.4028234663852886e38).view(np.uint32), "bf16": 0xFF7F, "f16": 0xFBFF}[dt]],
+                                     dtype=np.uint32 if dt == "f32" else np.uint16).view(np.float32 if dt == "f32" else np.uint16), dt)[0])
+    a.table[:4] = lowest
+    out, lse = a.forward(hip)
+    got = to_float(out, dt).astype(np.float64)
+    if dt != "f16":                                          # (-65504 does not drown q . k in f32)
+        for i in range(4):
+            want = a.v[: i + 1].mean(0)
+            assert np.abs(got[i] - want).max() <= 2.0 ** -7 * np.abs(a.v[: i + 1]).max()
+    assert np.isfinite(got).all() and np.isfinite(lse).all()
+    for g in a.backward(hip, out, lse):
+        assert np.isfinite(to_float(g, dt)).all()
+
+
+def test_each_gradient_can_be_left_out(hip):
+    a = Attention("bf16", [100, 60], 4, 2, 64, buckets=16, distance=64, seed=14)
+    out, lse = a.forward(hip)
+    every = a.backward(hip, out, lse)
+    for mask in range(1, 15):
+        want = tuple(bool(mask >> n & 1) for n in range(4))
+        for w, g, e in zip(want, a.backward(hip, out, lse, want), every):
+            assert (g is None) == (not w)
+            if w:
+                assert g.tobytes() == e.tobytes()
+    plain = Attention("f32", [100, 60], 4, 2, 64, seed=14)
+    out, lse = plain.forward(hip)
+    every = plain.backward(hip, out, lse)
+    for mask in range(1, 8):
+        want = tuple(bool(mask >> n & 1) for n in range(3)) + (False,)
+        for w, g, e in zip(want, plain.backward(hip, out, lse, want), every):
+            assert not w or g.tobytes() == e.tobytes()
+
+
+def test_the_same_bits_on_every_call(hip):
+    a = Attention("bf16", [500, 300, 9], 8, 2, 64, buckets=32, distance=128, seed=15)
+    out, lse = a.forward(hip)
+    grads = a.backward(hip, out, lse)
+    for _ in range(3):
+        o, ls = a.forward(hip)
+        assert o.tobytes() == out.tobytes() and ls.tobytes() == lse.tobytes()
+        assert all(x.tobytes() == y.tobytes() for x, y in zip(a.backward(hip, o, ls), grads))
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_a_sequence_does_not_depend_on_its_neighbours(hip, dt):
+    """NaN and infinities all over one sequence and in the rows that belong to none reach no other sequence."""
+    a = Attention(dt, [45, 40, 70], 2, 1, 32, lead=4, tail=7, seed=16)
+    want, bound = a.exact()
+    dirty = np.r_[0:4, 49:89, a.tokens - 7:a.tokens]
+    for t in (a.q, a.k, a.v, a.go):
+        t[dirty[::2]] = np.nan
+        t[dirty[1::2]] = np.inf
+    out, lse = a.forward(hip)
+    gq, gk, gv, _ = a.backward(hip, out, lse)
+    clean = np.r_[4:49, 89:159]
+    for name, got in (("o", out), ("gq", gq), ("gk", gk), ("gv", gv)):
+        a.close(got[clean], want[name][clean], bound[name][clean], name)
+    a.close(lse[:, clean], want["lse"][:, clean], bound["lse"][:, clean], "lse")
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_what_comes_later_does_not_reach_back(hip, dt, bad):
+    """Non-finite keys and values at the end of a sequence (a padded batch) leave the rows before them as they were."""
+    a = Attention(dt, [200, 30], 2, 1, 64, seed=17)
+    want, bound = a.exact()
+    a.v[150:200] = bad
+    a.k[170:200] = bad
+    out, lse = a.forward(hip)
+    rows = np.r_[0:150, 200:230]
+    a.close(out[rows], want["o"][rows], bound["o"][rows], "output")
+    a.close(lse[:, rows], want["lse"][:, rows], bound["lse"][:, rows], "lse")
+
+
+def test_infinite_values_in_view(hip):
+    """An infinite value that a row sees is in its output, as the sum says."""
+    a = Attention("f32", [100], 1, 1, 32, seed=18)
+    a.v[40, 0, 3] = np.inf
+    a.v[60, 0, 4] = -np.inf
+    a.v[70, 0, 5] = np.nan
+    out, _ = a.forward(hip)
+    assert np.isfinite(out[:, 0, :3]).all() and np.isfinite(out[:, 0, 6:]).all()
+    assert np.isfinite(out[:40, 0, 3]).all() and (out[40:, 0, 3] == np.inf).all()
+    assert np.isfinite(out[:60, 0, 4]).all() and (out[60:, 0, 4] == -np.inf).all()
+    assert np.isfinite(out[:70, 0, 5]).all() and np.isnan(out[70:, 0, 5]).all()
+
+
+@pytest.mark.parametrize("offsets", [[0, 50, 40, 90], [-3, 90], [0, 91], [90, 0], [2 ** 31 - 1, 2 ** 31 - 1], [-2 ** 31, 5, 90, 2 ** 31 - 1]] + [[0] + [95] * 70])
+def test_bad_offsets_are_reported(hip, offsets):
+    """Nothing outside the tensors is touched: the kernels keep every bound that they make of offsets within the tokens."""
+    a = Attention("f32", [90], 2, 1, 32, buckets=8, distance=16, seed=19)
+    out, lse = a.forward(hip)
+    a.offsets = np.array(offsets, dtype=np.int32)
+    with pytest.raises(L.HipError, match="offsets of attention"):
+        a.forward(hip)
+    with pytest.raises(L.HipError, match="offsets of attention"):
+        a.backward(hip, out, lse)
+
+
+def test_nothing_to_do(hip):
+    a = Attention("f32", [4], 2, 1, 8, buckets=4, distance=8, seed=20)
+    a.offsets = np.array([0], dtype=np.int32)                # no sequence
+    out, lse = a.forward(hip)
+    assert (out.view(np.uint8) == 0xCD).all() and (lse.view(np.uint8) == 0xCD).all()
+    gq, gk, gv, gt = a.backward(hip, np.zeros_like(out), np.zeros_like(lse))
+    assert all((g.view(np.uint8) == 0xCD).all() for g in (gq, gk, gv)) and (gt == 0).all()
+
+
+def test_many_sequences(hip):
+    """More sequences than a wave has lanes (the search by halves), empty ones among them."""
+    r = np.random.default_rng(21)
+    Attention("bf16", [int(n) for n in r.integers(0, 9, 150)], 2, 1, 32, lead=1, tail=3, seed=21).check(hip)
+
+
+def test_capture_replays_with_new_data(hip):
+    """Forward and backward in a captured graph, replayed over new inputs and other sequence lengths between eager calls."""
+    lib = L.load()
+    problems = [Attention("bf16", lengths, 4, 2, 64, buckets=16, distance=64, seed=22 + i) for i, lengths in enumerate(([150, 50], [20, 100, 80], [200, 0]))]
+    for p in problems:                                        # one number of sequences for all
+        p.offsets = np.concatenate([p.offsets, [200] * (4 - len(p.offsets))]).astype(np.int32)
+    p = problems[0]
+    md, off, q, k, v, table, scale = p.arguments()
+    names = ["off", "q", "k", "v", "table", "go"]
+
+    def inputs(x):
+        a = x.arguments()
+        return dict(zip(names, [a[1].arr, a[2].arr, a[3].arr, a[4].arr, a[5].arr, to_storage(x.go, x.dt).ravel()]))
+    bufs = {n: L.DeviceBuffer.from_numpy(a) for n, a in inputs(p).items()}
+    outs = {n: L.DeviceBuffer(2 * c) for n, c in (("out", 200 * 4 * 64), ("gq", 200 * 4 * 64), ("gk", 200 * 2 * 64), ("gv", 200 * 2 * 64), ("gt", 64))}
+    lse = L.DeviceBuffer(4 * 4 * 200)
+
+    def calls():
+        common = [md, bufs["off"], bufs["q"], bufs["k"], bufs["v"], bufs["table"], scale]
+        L.call("attention_bf16", *common, outs["out"], lse)
+        L.call("attention_backward_bf16", *common, outs["out"], lse, bufs["go"], outs["gq"], outs["gk"], outs["gv"], outs["gt"])
+    calls()
+    L.synchronize()
+    import ctypes as C
+    graph = C.c_void_p()
+    assert lib.hip_graph_begin_capture() == 0
+    calls()
+    assert lib.hip_graph_end_capture(C.byref(graph)) == 0
+    try:
+        for x in problems + problems[:1]:
+            o, ls = x.forward(hip)                            # eager, over the library's own scratch
+            want = [o, *x.backward(hip, o, ls)]
+            for n, a in inputs(x).items():
+                assert lib.hip_memcpy_h2d(bufs[n].ptr, np.ascontiguousarray(a).ctypes.data, a.nbytes) == 0
+            assert lib.hip_graph_launch(graph) == 0
+            L.synchronize()
+            for n, w in zip(("out", "gq", "gk", "gv", "gt"), want):
+                assert outs[n].to_numpy(np.uint16).tobytes() == w.tobytes(), n
+    finally:
+        lib.hip_graph_destroy(graph)
+
+
+def test_on_a_stream_of_the_callers(hip):
+    import ctypes as C
+    lib = L.load()
+    a = Attention("f32", [80, 30], 2, 1, 32, seed=30)
+    out, lse = a.forward(hip)
+    s = C.c_void_p()
+    assert lib.hip_stream_create(C.byref(s)) == 0
+    try:
+        assert lib.hip_set_stream(s) == 0
+        o, ls = a.forward(hip)
+        assert o.tobytes() == out.tobytes() and ls.tobytes() == lse.tobytes()
+    finally:
+        lib.hip_set_stream(None)
+        lib.hip_stream_destroy(s)
+
+
+def test_gradients_are_the_differences(hip):
+    """sum(output * go) in f32, by central differences of size 2^-6: the truncation is below (2^-6)^2 / 6 times the third
+    derivative (for inputs of order one, 1e-3 is generous), the roundings 2^-24 |sum| / 2^-6 are below it."""
+    a = Attention("f32", [12, 5], 2, 1, 8, buckets=4, distance=6, seed=31)
+    out, lse = a.forward(hip)
+    grads = a.backward(hip, out, lse)
+
+    def value():
+        return float((a.forward(hip)[0].astype(np.float64) * a.go).sum())
+    for tensor, grad in ((a.q, grads[0]), (a.k, grads[1]), (a.v, grads[2]), (a.table, grads[3])):
+        flat = tensor.reshape(-1)
+        for i in range(0, flat.size, max(1, flat.size // 9)):
+            kept = flat[i]
+            flat[i] = kept + 2.0 ** -6
+            up = value()
+            flat[i] = kept - 2.0 ** -6
+            down = value()
+            flat[i] = kept
+            assert abs((up - down) * 2.0 ** 5 - grad.reshape(-1)[i]) < 3e-3
