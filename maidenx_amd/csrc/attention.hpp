@@ -33,7 +33,7 @@ namespace mxh {
 constexpr int ATTN_MAX_DIM = 128;
 constexpr int ATTN_MAX_BUCKETS = 256;
 constexpr int ATTN_MAX_DISTANCE = 4096;
-constexpr int ATTN_THREADS = 256;
+constexpr int ATTN_THREADS = 256, ATTN_WAVES = ATTN_THREADS / WAVE;
 constexpr int ATTN_ROWS = 128;              // rows (of queries, or of keys in the backward pass for keys) that a block owns: 32 a wave
 constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
 constexpr float ATTN_FLT_MAX = 3.402823466e+38f;
@@ -182,28 +182,67 @@ __device__ inline u32x4_t attn_piece(const E* row, int d, int dim, int64_t elem,
     return r;
 }
 
-// A tile of ROWS tokens of one operand on its way from memory to LDS through a block's registers.
+// ROWS tokens of one operand, from memory to a tile in LDS.  Rows are whole 16-byte pieces in the usual case: they go
+// straight to LDS (a wave's instruction fills 1 KB in a row; which piece of which row a lane fetches undoes the swizzle), with no
+// register in between, and are waited for a tile later.  The compiler does not know of these loads, so that it does not wait for
+// them before every read of LDS: attn_arrived() does, in front of the barrier that hands a tile over.  Anything else
+// (other strides, heads that are not whole pieces) goes through registers, element by element.
+// A token outside [lo, hi) is replaced by one inside: the mask hides what it brings.
+__device__ inline void attn_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 template <class E, int DP, int ROWS>
 struct AttnStage {
     using L = AttnTile<E, DP>;
-    static constexpr int N = (ROWS * L::DATA + ATTN_THREADS - 1) / ATTN_THREADS;
-    static constexpr bool WHOLE = ROWS * L::DATA % ATTN_THREADS == 0;
-    u32x4_t r[N];
-    // rows outside [lo, hi) become zeros
-    __device__ void load(const AttnView<E>& view, int head, int token0, int lo, int hi, int dim, int tid) {
-        const E* base = view.p + (int64_t)head * view.head;
+    static constexpr int CALLS = ROWS * L::PITCH / 1024;       // wave instructions for a tile
+    static constexpr int N = (CALLS + ATTN_WAVES - 1) / ATTN_WAVES;
+    uint32_t off[N];                                           // bytes from the tile's first token to the lane's piece
+    bool on[N];
+    __device__ void begin(const AttnView<E>& view, int dim, int wave, int lane) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            const int idx = u * ATTN_THREADS + tid, row = idx / L::DATA, piece = idx % L::DATA, token = token0 + row;
-            r[u] = u32x4_t{0, 0, 0, 0};
-            if (token >= lo && token < hi && (WHOLE || row < ROWS)) r[u] = attn_piece<E>(base + (int64_t)token * view.token, piece * L::T::CHUNK, dim, view.elem, view.vec);
+            const int slot = (u * ATTN_WAVES + wave) * 64 + lane, row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row);
+            off[u] = (uint32_t)(row * (int)view.token + piece * L::T::CHUNK) * (uint32_t)sizeof(E);
+            on[u] = piece * L::T::CHUNK < dim && row < ROWS;
         }
     }
-    __device__ void store(char* tile, int tid) const {
+    // pieces that no load brings (dim below DP) have to be zeros: once, for all tiles that lie there later
+    __device__ static void clear(char* tiles, int bytes, int tid) {
+        for (int at = tid * 16; at < bytes; at += ATTN_THREADS * 16) *(u32x4_t*)(tiles + at) = u32x4_t{0, 0, 0, 0};
+    }
+    // every row of the tile is a token inside
+    __device__ void load(const AttnView<E>& view, int head, int token0, int dim, char* tile, int wave, int lane) const {
+        if (!view.vec) return slow(view, head, token0, 0, 0x7fffffff, dim, tile, wave, lane);
+        const E* const base = view.p + (int64_t)head * view.head + (int64_t)token0 * view.token;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+            if (on[u]) fetch(base, off[u], tile, u, wave);
+    }
+    __device__ void load_inside(const AttnView<E>& view, int head, int token0, int lo, int hi, int dim, char* tile, int wave, int lane) const {
+        if (!view.vec) return slow(view, head, token0, lo, hi, dim, tile, wave, lane);
+        const E* const base = view.p + (int64_t)head * view.head + (int64_t)token0 * view.token;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            const int idx = u * ATTN_THREADS + tid;
-            if (WHOLE || idx < ROWS * L::DATA) *(u32x4_t*)(tile + L::at(idx / L::DATA, idx % L::DATA)) = r[u];
+            const int row = ((u * ATTN_WAVES + wave) * 64 + lane) / L::PIECES, token = token0 + row;
+            const int in = token < lo ? lo : token >= hi ? hi - 1 : token;
+            // (within a tile of the first token: 32 bits, as for the others)
+            if (on[u]) fetch(base, off[u] + (uint32_t)(in - token) * (uint32_t)view.token * (uint32_t)sizeof(E), tile, u, wave);
+        }
+    }
+    // (m0, the place in LDS, is read as the load is issued; nothing else in these kernels uses it)
+    __device__ static void fetch(const E* base, uint32_t off, char* tile, int u, int wave) {
+        const uint64_t at = (uint64_t)(uintptr_t)base;
+        const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile + (uint32_t)((u * ATTN_WAVES + wave) * 1024);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                     :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(from) : "memory");
+    }
+    __device__ static void slow(const AttnView<E>& view, int head, int token0, int lo, int hi, int dim, char* tile, int wave, int lane) {
+        const E* const base = view.p + (int64_t)head * view.head;
+#pragma nounroll
+        for (int slot = wave * 64 + lane; slot < ROWS * L::PIECES; slot += ATTN_THREADS) {
+            const int row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row), token = token0 + row;
+            const int in = token < lo ? lo : token >= hi ? hi - 1 : token;
+            *(u32x4_t*)(tile + slot * 16) = attn_piece<E>(base + (int64_t)in * view.token, piece * L::T::CHUNK, dim, view.elem, 0);
         }
     }
 };
@@ -278,8 +317,8 @@ __device__ inline void attn_check_offsets(const AttnArgs<E>& a) {
 // heads, neighbouring heads - which share their keys - are eight blocks apart: on one XCD, behind one L2.
 __device__ inline void attn_place(int block, int tiles, int heads, bool last_first, int& tile, int& head) {
     const int t = block / heads, x = block - t * heads;
-    tile = last_first ? tiles - 1 - t : t;
-    head = heads % 8 == 0 ? (x % 8) * (heads / 8) + x / 8 : x;
+    tile = __builtin_amdgcn_readfirstlane(last_first ? tiles - 1 - t : t);
+    head = __builtin_amdgcn_readfirstlane(heads % 8 == 0 ? (x % 8) * (heads / 8) + x / 8 : x);
 }
 
 // ---- the bias ------------------------------------------------------------------------------------------------------------
@@ -318,11 +357,38 @@ __device__ inline void attn_add_bias(f32x16_t& s, float c, const float* by_dista
 
 // ---- what a mask hides -----------------------------------------------------------------------------------------------------
 // The matrix cores multiply a weight of zero by whatever the other operand holds: a NaN or an infinity in a row that the mask hides
-// from a column (a later token, another sequence) would become a NaN there.  So a block whose sums are not finite makes them
-// once more (its columns that really see such a row end as they have to), with the tiles that a mask touches term by term:
-// sums[d] += weight * tile[row][d] for the rows that `sees` lets through.  Costs nothing where everything is finite.
+// from a column (a later token, another sequence) would become a NaN there.  So the tiles that a mask touches - a few at either end
+// of a block's walk, in a loop of their own - are looked over, and one that holds such a value is added term by term:
+// sums[d] += weight * tile[row][d] for the rows that `sees` lets through.
+template <class E>
+__device__ inline bool attn_finite(u32x4_t x) {
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(E) == 4) {
+            fine &= (x[e] & 0x7F800000u) != 0x7F800000u;
+        } else {
+            const uint32_t exponent = std::is_same<E, bf16_t>::value ? 0x7F80u : 0x7C00u;
+            fine &= (x[e] & exponent) != exponent && (x[e] >> 16 & exponent) != exponent;
+        }
+    }
+    return fine;
+}
+// by all threads of a block, the tile being there: whether it holds such a value.  Two barriers' worth of waiting.
+template <class E>
+__device__ inline bool attn_look_over(const char* tile, int bytes, int* said, int tid, int wave, int lane) {
+    bool fine = true;
+    for (int at = tid * 16; at < bytes; at += ATTN_THREADS * 16) fine &= attn_finite<E>(*(const u32x4_t*)(tile + at));
+    const bool any = __any(!fine);
+    if (lane == 0) said[wave] = any;
+    __syncthreads();
+    int bad = 0;
+#pragma unroll
+    for (int w = 0; w < ATTN_WAVES; ++w) bad |= said[w];
+    return __builtin_amdgcn_readfirstlane(bad) != 0;
+}
 template <class E, int DP, int TILES, class Sees>
-__device__ inline void attn_careful(const char* tile, const f32x16_t (&weight)[TILES], f32x16_t (&sums)[DP / 32], int lane, Sees sees) {
+__device__ inline void attn_add_terms(const char* tile, const f32x16_t (&weight)[TILES], f32x16_t (&sums)[DP / 32], int lane, Sees sees) {
     using L = AttnTile<E, DP>;
     const int half = lane >> 5;
 #pragma nounroll
@@ -345,35 +411,105 @@ __device__ inline void attn_careful(const char* tile, const f32x16_t (&weight)[T
                     const float y = __builtin_fmaf(w, AttnType<E>::get(x[e]), sums[d][4 * g + e]);
                     sums[d][4 * g + e] = seen ? y : sums[d][4 * g + e];
                 }
+                __builtin_amdgcn_sched_barrier(0);       // a few registers at a time
             }
     }
 }
-template <int N>
-__device__ inline bool attn_finite(const f32x16_t (&sums)[N]) {
-    bool fine = true;
+// sums[d] += weight^T tile, the summed index in the rows of both
+template <class E, int DP>
+__device__ inline void attn_add_product(const char* tile, int row0, const f32x16_t& weight, f32x16_t (&sums)[DP / 32], int lane) {
+    using T = AttnType<E>;
 #pragma unroll
-    for (int d = 0; d < N; ++d)
+    for (int h = 0; h < 2; ++h) {
+        f32x8_t p;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) fine &= __builtin_fabsf(sums[d][r]) <= ATTN_FLT_MAX;
-    return fine;
+        for (int e = 0; e < 8; ++e) p[e] = weight[8 * h + e];
+        const typename T::Frag pf = T::pack(p);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) sums[d] = T::mma(AttnTile<E, DP>::columns(tile, row0 + 16 * h, d, lane), pf, sums[d]);
+    }
 }
+
+// The tiles of a block's walk over [begin, end): first those that every row of the block sees whole, [clean, dirty) in steps of
+// STEP, then the rest, in front of them and behind.
+template <int STEP>
+struct AttnWalk {
+    int begin, clean, dirty, nclean, nfront, total;
+    __device__ AttnWalk(int begin_, int end, int from, int upto) : begin(begin_) {
+        clean = from > begin ? begin + (from - begin + STEP - 1) / STEP * STEP : begin;
+        nclean = upto > clean ? (upto - clean) / STEP : 0;
+        if (nclean == 0) clean = begin;
+        dirty = clean + nclean * STEP;
+        nfront = (clean - begin) / STEP;
+        total = nclean + nfront + (end > dirty ? (end - dirty + STEP - 1) / STEP : 0);
+    }
+    __device__ int at(int n) const { return n < nclean ? clean + n * STEP : n < nclean + nfront ? begin + (n - nclean) * STEP : dirty + (n - nclean - nfront) * STEP; }
+};
+
+// What a block has to know of its rows: 32 a wave.
+struct AttnSpan {
+    int begin, end, inner, top;       // the other axis from begin to end; [inner, top) is what every row sees
+    // lo, hi: of a wave's rows (0x7fffffff, 0 for none); inner, top likewise (0, 0x7fffffff for none)
+    __device__ AttnSpan(int lo, int hi, int inner_, int top_, int* shared, int wave, int lane) {
+        if (lane == 0) { shared[wave] = lo; shared[4 + wave] = hi; shared[8 + wave] = inner_; shared[12 + wave] = top_; }
+        __syncthreads();
+        begin = shared[0]; end = shared[4]; inner = shared[8]; top = shared[12];
+#pragma unroll
+        for (int w = 1; w < ATTN_WAVES; ++w) {
+            begin = shared[w] < begin ? shared[w] : begin;
+            end = shared[4 + w] > end ? shared[4 + w] : end;
+            inner = shared[8 + w] > inner ? shared[8 + w] : inner;
+            top = shared[12 + w] < top ? shared[12 + w] : top;
+        }
+        begin = __builtin_amdgcn_readfirstlane(begin);
+        end = __builtin_amdgcn_readfirstlane(end);
+        inner = __builtin_amdgcn_readfirstlane(inner);
+        top = __builtin_amdgcn_readfirstlane(top);
+    }
+};
+
+// rows of a result (index in the columns of the fragments), four neighbouring elements at a time where they lie on their boundaries
+template <class E, int DP>
+__device__ inline void attn_write_row(E* out, const f32x16_t (&sums)[DP / 32], float by, int dim, int half, bool whole) {
+    using T = AttnType<E>;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int at = 32 * d + 8 * g + 4 * half;
+            E x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = T::put(sums[d][4 * g + e] * by);
+            if (whole) {
+                if (at < dim) __builtin_memcpy(__builtin_assume_aligned(out + at, 4 * sizeof(E)), x, sizeof(x));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at + e < dim) out[at + e] = x[e];
+            }
+        }
+}
+template <class E>
+__device__ inline bool attn_whole(const E* out, int dim) { return dim % 4 == 0 && (uintptr_t)out % (4 * sizeof(E)) == 0; }
+
+__device__ inline float attn_sign(float scale) { return scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f; }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
 template <class E> constexpr int attn_keys() { return sizeof(E) == 4 ? 32 : 64; }     // keys of a tile: 64 KB of LDS for two tiles of keys and values either way
 template <class E, int DP>
 constexpr size_t attn_tile_bytes(int rows) { return (size_t)rows * AttnTile<E, DP>::PITCH; }
+// the running maximum may be this much (a factor of 2^8) behind before the sums are rescaled
+constexpr float ATTN_BEHIND = 8.0f;
 
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16;
+    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int span[8];
+    __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    char* const ktile = lds;
-    char* const vtile = lds + 2 * BN * L::PITCH;
-    float* const by_distance = (float*)(lds + 4 * BN * L::PITCH);
+    float* const by_distance = (float*)(lds + 4 * BYTES);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -382,134 +518,116 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
     int first, last;
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
     const int lo = attn_wave_min(there ? first : 0x7fffffff), hi = attn_wave_max(there ? row + 1 : 0);   // keys this wave needs
-    const int inner = attn_wave_max(there ? first : 0x7fffffff);                                        // from here on all rows share the keys
-    const int top = attn_wave_min(there ? row : -1);                                                   // ... and up to here
-    if (lane == 0) { span[wave] = lo; span[4 + wave] = hi; }
-    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
-    typename T::Frag q[KS];
-    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, q);
-    __syncthreads();
-    int begin = span[0], end = span[4];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-        begin = span[w] < begin ? span[w] : begin;
-        end = span[4 + w] > end ? span[4 + w] : end;
+    const AttnSpan all(lo, hi, attn_wave_max(there ? first : 0), attn_wave_min(there ? row + 1 : 0x7fffffff), span, wave, lane);
+    if (all.end <= all.begin) return;               // no row of the block is in a sequence
+    AttnStage<E, DP, BN> ks, vs;
+    ks.begin(a.k, a.dim, wave, lane);
+    vs.begin(a.v, a.dim, wave, lane);
+    const AttnWalk<BN> walk(all.begin, all.end, all.inner, all.top);
+    if (a.dim < DP) {
+        ks.clear(lds, 4 * BYTES, tid);
+        __syncthreads();
     }
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-    if (end <= begin) return;                       // no row of the block is in a sequence
+    auto fetch = [&](int n) {
+        char* const to = lds + (n & 1) * 2 * BYTES;
+        const int j0 = walk.at(n);
+        if (n < walk.nclean) {
+            ks.load(a.k, kv, j0, a.dim, to, wave, lane);
+            vs.load(a.v, kv, j0, a.dim, to + BYTES, wave, lane);
+        } else {
+            ks.load_inside(a.k, kv, j0, all.begin, all.end, a.dim, to, wave, lane);
+            vs.load_inside(a.v, kv, j0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
+        }
+    };
+    fetch(0);
+    typename T::Frag q[KS];
+    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
+    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
 
     const int lower = there ? first : -1;           // key j is seen if (unsigned)(j - lower) <= reach
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
     const float c = a.scale_log2;
     f32x16_t acc[DB];
-    float m, l;
-    int careful = 0;
-    for (;;) {
-    careful = __builtin_amdgcn_readfirstlane(careful);
-    asm volatile("" : "+s"(careful));               // one loop for both ways through it
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
-    m = -INFINITY;
-    l = 0.0f;
-    AttnStage<E, DP, BN> ks, vs;
-    ks.load(a.k, kv, begin, begin, end, a.dim, tid);
-    vs.load(a.v, kv, begin, begin, end, a.dim, tid);
-    ks.store(ktile, tid);
-    vs.store(vtile, tid);
-    __syncthreads();
-    int buf = 0;
-    for (int j0 = begin; j0 < end; j0 += BN, buf ^= 1) {
-        const bool more = j0 + BN < end;
-        if (more) {
-            ks.load(a.k, kv, j0 + BN, begin, end, a.dim, tid);
-            vs.load(a.v, kv, j0 + BN, begin, end, a.dim, tid);
+    float m = -INFINITY, l = 0.0f;
+    auto step = [&](auto masked_, int n) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        const char* const kt = lds + (n & 1) * 2 * BYTES;
+        const char* const vt = kt + BYTES;
+        const int j0 = walk.at(n);
+        bool terms = false;
+        if constexpr (MASKED) {
+            terms = attn_look_over<E>(vt, BYTES, span, tid, wave, lane);
+            if (j0 >= hi || j0 + BN <= lo) return;
         }
-        const char* const kt = ktile + buf * BN * L::PITCH;
-        const char* const vt = vtile + buf * BN * L::PITCH;
-        if (j0 < hi && j0 + BN > lo) {
-            f32x16_t s[JB];
+        f32x16_t s[JB];
 #pragma unroll
-            for (int b = 0; b < JB; ++b) {
-                s[b] = f32x16_t{};
+        for (int b = 0; b < JB; ++b) {
+            s[b] = f32x16_t{};
 #pragma unroll
-                for (int k = 0; k < KS; ++k) s[b] = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s[b]);
-            }
-            const int j = j0 + 4 * half;            // key of row 0 of the lane's results
-            if (BIAS) {
-                const bool near = row0 - (j0 + BN - 1) < a.max_distance;
-                const float far_bias = by_distance[a.max_distance];
+            for (int k = 0; k < KS; ++k) s[b] = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s[b]);
+        }
+        const int j = j0 + 4 * half;                // key of row 0 of the lane's results
+        if (BIAS) {
+            const bool near = row0 - (j0 + BN - 1) < a.max_distance;
+            const float far_bias = by_distance[a.max_distance];
 #pragma unroll
-                for (int b = 0; b < JB; ++b) attn_add_bias<1>(s[b], c, by_distance, row - j - 32 * b, a.max_distance, near, far_bias);
-            }
-            const bool masked = j0 < inner || j0 + BN - 1 > top;
-            if (masked) {
-#pragma unroll
-                for (int b = 0; b < JB; ++b)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if ((uint32_t)(j + 32 * b + (r & 3) + 8 * (r >> 2) - lower) > reach) s[b][r] = -INFINITY;
-            }
-            float best = s[0][0];
+            for (int b = 0; b < JB; ++b) attn_add_bias<1>(s[b], c, by_distance, row - j - 32 * b, a.max_distance, near, far_bias);
+        }
+        if constexpr (MASKED) {
 #pragma unroll
             for (int b = 0; b < JB; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
-            best = fmaxf(best, attn_other_half(best));
-            const float cc = BIAS ? 1.0f : c;
-            best = BIAS ? best : best * c;
-            const float next = fmaxf(m, best);
-            if (__any(next > m)) {
-                const float fix = next == -INFINITY ? 1.0f : attn_exp2(m - next);
-                l *= fix;
+                for (int r = 0; r < 16; ++r)
+                    if ((uint32_t)(j + 32 * b + (r & 3) + 8 * (r >> 2) - lower) > reach) s[b][r] = -INFINITY;
+        }
+        float best = s[0][0];
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] *= fix;
-                m = next;
+        for (int b = 0; b < JB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
+        best = fmaxf(best, attn_other_half(best));
+        if (!BIAS) best *= c;
+        if (__any(best > m + ATTN_BEHIND)) {
+            const float next = fmaxf(m, best), fix = next == -INFINITY ? 1.0f : attn_exp2(m - next);
+            l *= fix;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[d] *= fix;
+            m = next;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int b = 0; b < JB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = attn_exp2(BIAS ? s[b][r] - base : __builtin_fmaf(s[b][r], c, -base));
+                l += s[b][r];
             }
-            const float base = m == -INFINITY ? 0.0f : m;
+        if (MASKED && terms) {
+            attn_add_terms<E, DP, JB>(vt, s, acc, lane, [&](int r) { return (uint32_t)(j0 + r - lower) <= reach; });
+        } else {
 #pragma unroll
-            for (int b = 0; b < JB; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[b][r] = attn_exp2(BIAS ? s[b][r] - base : __builtin_fmaf(s[b][r], cc, -base));
-                    l += s[b][r];
-                }
-            if (careful && masked) {
-                attn_careful<E, DP, JB>(vt, s, acc, lane, [&](int r) { return (uint32_t)(j0 + r - lower) <= reach; });
-            } else
-#pragma unroll
-            for (int b = 0; b < JB; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    f32x8_t p;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = s[b][8 * h + e];
-                    const typename T::Frag pf = T::pack(p);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] = T::mma(L::columns(vt, 32 * b + 16 * h, d, lane), pf, acc[d]);
-                }
+            for (int b = 0; b < JB; ++b) attn_add_product<E, DP>(vt, 32 * b, s[b], acc, lane);
         }
-        if (more) {
-            ks.store(ktile + (buf ^ 1) * BN * L::PITCH, tid);
-            vs.store(vtile + (buf ^ 1) * BN * L::PITCH, tid);
-        }
+    };
+    for (int n = 0; n < walk.nclean; ++n) {
+        attn_arrived();
         __syncthreads();
+        if (n + 1 < walk.total) fetch(n + 1);
+        step(std::false_type{}, n);
     }
-    if (careful || !__syncthreads_or(!attn_finite(acc))) break;
-    careful = 1;
+    for (int n = walk.nclean; n < walk.total; ++n) {
+        attn_arrived();
+        __syncthreads();
+        if (n + 1 < walk.total) fetch(n + 1);
+        step(std::true_type{}, n);
     }
     l += attn_other_half(l);
     if (!there) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing but -inf: an output of zeros
     if (half == 0) a.lse[(int64_t)head * a.tokens + row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * ATTN_LN2;
-    E* const out = a.out + ((int64_t)row * a.heads + head) * a.dim;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int at = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
-            if (at < a.dim) out[at] = T::put(acc[d][r] * inv);
-        }
+    attn_write_row<E, DP>(a.out + ((int64_t)row * a.heads + head) * a.dim, acc, inv, a.dim, half, attn_whole(a.out, a.dim));
 }
 
 // ---- backward: gradients of the queries ------------------------------------------------------------------------------------
@@ -517,16 +635,14 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
 // bias the one that makes the row of dS sum to zero (formed from P and dP themselves; the rounding of o in do . o
 // would otherwise enter every pair of the far bucket with the same sign).
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles) {
+__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16;
+    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int span[8];
+    __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    char* const ktile = lds;
-    char* const vtile = lds + 2 * BN * L::PITCH;
-    float* const by_distance = (float*)(lds + 4 * BN * L::PITCH);
+    float* const by_distance = (float*)(lds + 4 * BYTES);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -535,124 +651,109 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_query_kernel(const 
     int first, last;
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
     const int lo = attn_wave_min(there ? first : 0x7fffffff), hi = attn_wave_max(there ? row + 1 : 0);
-    const int inner = attn_wave_max(there ? first : 0x7fffffff);
-    const int top = attn_wave_min(there ? row : -1);
-    if (lane == 0) { span[wave] = lo; span[4 + wave] = hi; }
-    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
+    const AttnSpan all(lo, hi, attn_wave_max(there ? first : 0), attn_wave_min(there ? row + 1 : 0x7fffffff), span, wave, lane);
+    if (all.end <= all.begin) return;
+    AttnStage<E, DP, BN> ks, vs;
+    ks.begin(a.k, a.dim, wave, lane);
+    vs.begin(a.v, a.dim, wave, lane);
+    const AttnWalk<BN> walk(all.begin, all.end, all.inner, all.top);
+    if (a.dim < DP) {
+        ks.clear(lds, 4 * BYTES, tid);
+        __syncthreads();
+    }
+    auto fetch = [&](int n) {
+        char* const to = lds + (n & 1) * 2 * BYTES;
+        const int j0 = walk.at(n);
+        if (n < walk.nclean) {
+            ks.load(a.k, kv, j0, a.dim, to, wave, lane);
+            vs.load(a.v, kv, j0, a.dim, to + BYTES, wave, lane);
+        } else {
+            ks.load_inside(a.k, kv, j0, all.begin, all.end, a.dim, to, wave, lane);
+            vs.load_inside(a.v, kv, j0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
+        }
+    };
+    const bool walks = a.gq || (BIAS && (a.gk || a.partial));       // else only D_i is wanted, if that
+    if (walks) fetch(0);
     typename T::Frag q[KS], go[KS];
-    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, q);
     attn_own_rows<E, DP>(a.go, head, there ? row : 0, there, a.dim, lane, 1.0f, go);
     float delta = 0.0f, lse2 = INFINITY;
     {
-        typename T::Frag o[KS];
-        attn_own_rows<E, DP>(a.o, head, there ? row : 0, there, a.dim, lane, 1.0f, o);
+        attn_own_rows<E, DP>(a.o, head, there ? row : 0, there, a.dim, lane, 1.0f, q);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(T::get(go[k], e), T::get(o[k], e), delta);
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(T::get(go[k], e), T::get(q[k], e), delta);
         delta += attn_other_half(delta);
     }
+    if (!walks) {
+        if (there && half == 0) a.delta[(int64_t)head * a.tokens + row] = delta;
+        return;
+    }
+    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (there) {
         const float x = a.lse[(int64_t)head * a.tokens + row];
         lse2 = x == -INFINITY ? INFINITY : x * ATTN_LOG2E;       // a row of nothing but -inf: P is zero
     }
-    __syncthreads();
-    int begin = span[0], end = span[4];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-        begin = span[w] < begin ? span[w] : begin;
-        end = span[4 + w] > end ? span[4 + w] : end;
-    }
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-    if (end <= begin) return;
-    if (!a.gq && !(BIAS && (a.gk || a.partial))) {       // only D_i is wanted, if that
-        if (there && half == 0) a.delta[(int64_t)head * a.tokens + row] = delta;
-        return;
-    }
+    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
     const int lower = there ? first : -1;
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
     const float c = a.scale_log2;
     f32x16_t acc[DB];
-    float rest;
-    int careful = 0;
-    for (;;) {
-    careful = __builtin_amdgcn_readfirstlane(careful);
-    asm volatile("" : "+s"(careful));
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
-    rest = 0.0f;
-    AttnStage<E, DP, BN> ks, vs;
-    ks.load(a.k, kv, begin, begin, end, a.dim, tid);
-    vs.load(a.v, kv, begin, begin, end, a.dim, tid);
-    ks.store(ktile, tid);
-    vs.store(vtile, tid);
-    __syncthreads();
-    int buf = 0;
-    for (int j0 = begin; j0 < end; j0 += BN, buf ^= 1) {
-        const bool more = j0 + BN < end;
-        if (more) {
-            ks.load(a.k, kv, j0 + BN, begin, end, a.dim, tid);
-            vs.load(a.v, kv, j0 + BN, begin, end, a.dim, tid);
+    float rest = 0.0f;
+    auto step = [&](auto masked_, int n) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        const char* const kt = lds + (n & 1) * 2 * BYTES;
+        const char* const vt = kt + BYTES;
+        const int j0 = walk.at(n);
+        bool terms = false;
+        if constexpr (MASKED) {
+            terms = attn_look_over<E>(kt, BYTES, span, tid, wave, lane);
+            if (j0 >= hi || j0 + BN <= lo) return;
         }
-        const char* const kt = ktile + buf * BN * L::PITCH;
-        const char* const vt = vtile + buf * BN * L::PITCH;
-        if (j0 < hi && j0 + BN > lo) {
-            const bool masked = j0 < inner || j0 + BN - 1 > top;
-            const bool near = BIAS && row0 - (j0 + BN - 1) < a.max_distance;
-            const float far_bias = BIAS ? by_distance[a.max_distance] : 0.0f;
+        const bool near = BIAS && row0 - (j0 + BN - 1) < a.max_distance;
+        const float far_bias = BIAS ? by_distance[a.max_distance] : 0.0f;
 #pragma unroll
-            for (int b = 0; b < JB; ++b) {
-                f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+        for (int b = 0; b < JB; ++b) {
+            f32x16_t s = f32x16_t{}, dp = f32x16_t{};
 #pragma unroll
-                for (int k = 0; k < KS; ++k) s = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s);
+            for (int k = 0; k < KS; ++k) s = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(vt, 32 * b, k, lane), go[k], dp);
-                const int j = j0 + 32 * b + 4 * half;
-                if (BIAS) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance, near, far_bias);
+            for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(vt, 32 * b, k, lane), go[k], dp);
+            const int j = j0 + 32 * b + 4 * half;
+            if (BIAS) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance, near, far_bias);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[r] = attn_exp2(BIAS ? s[r] - lse2 : __builtin_fmaf(s[r], c, -lse2));
-                    s[r] *= dp[r] - delta;
-                    if (masked && (uint32_t)(j + (r & 3) + 8 * (r >> 2) - lower) > reach) s[r] = 0.0f;
-                    if (BIAS) rest += s[r];
-                }
-                if (careful && masked) {
-                    const f32x16_t w[1] = {s};
-                    attn_careful<E, DP, 1>(kt + 32 * b * L::PITCH, w, acc, lane, [&](int r) { return (uint32_t)(j0 + 32 * b + r - lower) <= reach; });
-                } else
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    f32x8_t p;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = s[8 * h + e];
-                    const typename T::Frag pf = T::pack(p);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] = T::mma(L::columns(kt, 32 * b + 16 * h, d, lane), pf, acc[d]);
-                }
+            for (int r = 0; r < 16; ++r) {
+                s[r] = attn_exp2(BIAS ? s[r] - lse2 : __builtin_fmaf(s[r], c, -lse2));
+                s[r] *= dp[r] - delta;
+                if (MASKED && (uint32_t)(j + (r & 3) + 8 * (r >> 2) - lower) > reach) s[r] = 0.0f;
+                if (BIAS) rest += s[r];
+            }
+            if (MASKED && terms) {
+                const f32x16_t w[1] = {s};
+                attn_add_terms<E, DP, 1>(kt + 32 * b * L::PITCH, w, acc, lane, [&](int r) { return (uint32_t)(j0 + 32 * b + r - lower) <= reach; });
+            } else {
+                attn_add_product<E, DP>(kt, 32 * b, s, acc, lane);
             }
         }
-        if (more) {
-            ks.store(ktile + (buf ^ 1) * BN * L::PITCH, tid);
-            vs.store(vtile + (buf ^ 1) * BN * L::PITCH, tid);
-        }
+    };
+    for (int n = 0; n < walk.nclean; ++n) {
+        attn_arrived();
         __syncthreads();
+        if (n + 1 < walk.total) fetch(n + 1);
+        step(std::false_type{}, n);
     }
-    if (careful || !__syncthreads_or(!attn_finite(acc))) break;
-    careful = 1;
+    for (int n = walk.nclean; n < walk.total; ++n) {
+        attn_arrived();
+        __syncthreads();
+        if (n + 1 < walk.total) fetch(n + 1);
+        step(std::true_type{}, n);
     }
     if (BIAS) rest += attn_other_half(rest);
     if (!there) return;
-    if (half == 0 && a.delta) a.delta[(int64_t)head * a.tokens + row] = BIAS ? delta + rest : delta;
-    if (!a.gq) return;
-    E* const out = a.gq + ((int64_t)row * a.heads + head) * a.dim;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int at = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
-            if (at < a.dim) out[at] = T::put(acc[d][r] * a.scale);
-        }
+    if (half == 0) a.delta[(int64_t)head * a.tokens + row] = BIAS ? delta + rest : delta;
+    if (a.gq) attn_write_row<E, DP>(a.gq + ((int64_t)row * a.heads + head) * a.dim, acc, a.scale, a.dim, half, attn_whole(a.gq, a.dim));
 }
 
 // ---- backward: gradients of the keys, the values and the bias table ----------------------------------------------------------
@@ -662,13 +763,11 @@ template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int BM = 32, DB = DP / 32, KS = DP / 16;
+    constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int span[8];
+    __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    char* const qtile = lds;
-    char* const otile = lds + 2 * BM * L::PITCH;
-    float* const stats = (float*)(lds + 4 * BM * L::PITCH);      // [2][lse2 | delta][BM]
+    float* const stats = (float*)(lds + 4 * BYTES);              // [2][lse2 | delta][BM]
     float* const corner = stats + 4 * BM + wave * (32 * 33 + 64);   // (BIAS) a tile of dS of this wave, and the sums of its diagonals
     float* const by_distance = stats + 4 * BM + 4 * (32 * 33 + 64);
     const int kv_heads = a.heads / a.group;
@@ -678,179 +777,161 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
     int first, last;
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, key, lane, first, last);
     const int lo = attn_wave_min(there ? key : 0x7fffffff), hi = attn_wave_max(there ? last : 0);     // queries this wave needs
-    const int inner = attn_wave_max(there ? key : 0x7fffffff), top = attn_wave_min(there ? last : 0); // queries that see every key
-    if (lane == 0) { span[wave] = lo; span[4 + wave] = hi; }
-    typename T::Frag k[KS], v[KS];
-    attn_own_rows<E, DP>(a.k, kv, there ? key : 0, there, a.dim, lane, a.scale > 0.0f ? 1.0f : a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f, k);
-    attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
-    __syncthreads();
-    int begin = span[0], end = span[4];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-        begin = span[w] < begin ? span[w] : begin;
-        end = span[4 + w] > end ? span[4 + w] : end;
-    }
-    begin = __builtin_amdgcn_readfirstlane(begin);
-    end = __builtin_amdgcn_readfirstlane(end);
-    const uint32_t reach = there ? (uint32_t)(last - key) : 0;       // query i sees the key if (unsigned)(i - key) < reach
-    const float c = a.scale_log2;
-    f32x16_t gk[DB], gv[DB];
+    const AttnSpan all(lo, hi, attn_wave_max(there ? key : 0), attn_wave_min(there ? last : 0x7fffffff), span, wave, lane);
     const int head0 = kv * a.group;
-    const int steps = end > begin ? (end - begin + BM - 1) / BM : 0, total = steps * a.group;
+    if (all.end <= all.begin) {                    // no key of the block is in a sequence
+        if (BIAS && a.partial)
+            for (int g = 0; g < a.group; ++g)
+                for (int b = lane; b < a.buckets; b += WAVE) a.partial[((int64_t)(head0 + g) * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = 0.0f;
+        return;
+    }
     AttnStage<E, DP, BM> qs, os;
+    qs.begin(a.q, a.dim, wave, lane);
+    os.begin(a.go, a.dim, wave, lane);
+    const AttnWalk<BM> walk(all.begin, all.end, all.inner, all.top);
+    if (a.dim < DP) {
+        qs.clear(lds, 4 * BYTES, tid);
+        __syncthreads();
+    }
     float stat = 0.0f;
-    auto fetch = [&](int n) {
-        const int head = head0 + n / steps, i0 = begin + (n % steps) * BM;
-        qs.load(a.q, head, i0, begin, end, a.dim, tid);
-        os.load(a.go, head, i0, begin, end, a.dim, tid);
+    auto fetch = [&](int head, int n, int buf) {
+        char* const to = lds + buf * 2 * BYTES;
+        const int i0 = walk.at(n);
+        if (n < walk.nclean) {
+            qs.load(a.q, head, i0, a.dim, to, wave, lane);
+            os.load(a.go, head, i0, a.dim, to + BYTES, wave, lane);
+        } else {
+            qs.load_inside(a.q, head, i0, all.begin, all.end, a.dim, to, wave, lane);
+            os.load_inside(a.go, head, i0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
+        }
         if (tid < 2 * BM) {
             const int i = i0 + tid % BM;
-            const bool in = i < end;
+            const bool in = i < all.end;
             const float x = in ? (tid < BM ? a.lse : a.delta)[(int64_t)head * a.tokens + i] : 0.0f;
             stat = tid >= BM ? x : !in || x == -INFINITY ? INFINITY : x * ATTN_LOG2E;
         }
     };
-    auto stash = [&](int buf) {
-        qs.store(qtile + buf * BM * L::PITCH, tid);
-        os.store(otile + buf * BM * L::PITCH, tid);
-        if (tid < 2 * BM) stats[buf * 2 * BM + tid] = stat;
-    };
-    float in_bucket[ATTN_MAX_BUCKETS / WAVE] = {0.0f, 0.0f, 0.0f, 0.0f}, far_sum = 0.0f;    // of the head at hand
-    int careful = 0;
-    for (;;) {
-    careful = __builtin_amdgcn_readfirstlane(careful);
-    asm volatile("" : "+s"(careful));
+    fetch(head0, 0, 0);
+    typename T::Frag k[KS], v[KS];
+    attn_own_rows<E, DP>(a.k, kv, there ? key : 0, there, a.dim, lane, attn_sign(a.scale), k);
+    attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
+    const uint32_t reach = there ? (uint32_t)(last - key) : 0;       // query i sees the key if (unsigned)(i - key) < reach
+    const float c = a.scale_log2;
+    f32x16_t gk[DB], gv[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) { gk[d] = f32x16_t{}; gv[d] = f32x16_t{}; }
-    if (total) {
-        fetch(0);
-        stash(0);
-    }
-    if (BIAS) {
-        attn_bias_by_distance(a, head0, by_distance, tid);
-    }
-    __syncthreads();
-    int buf = 0, step = 0, head = head0;
-    for (int n = 0; n < total; ++n, buf ^= 1) {
-        const bool more = n + 1 < total;
-        if (more) fetch(n + 1);
-        const int i0 = begin + step * BM;
-        const char* const qt = qtile + buf * BM * L::PITCH;
-        const char* const ot = otile + buf * BM * L::PITCH;
+    float in_bucket[ATTN_MAX_BUCKETS / WAVE] = {0.0f, 0.0f, 0.0f, 0.0f}, far_sum = 0.0f;    // of the head at hand
+    auto step = [&](auto masked_, int n, int buf) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        const char* const qt = lds + buf * 2 * BYTES;
+        const char* const ot = qt + BYTES;
         const float* const st = stats + buf * 2 * BM;
-        if (i0 < hi && i0 + BM > lo) {
-            f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+        const int i0 = walk.at(n);
+        bool terms = false;
+        if constexpr (MASKED) {
+            terms = attn_look_over<E>(qt, 2 * BYTES, span, tid, wave, lane);
+            if (i0 >= hi || i0 + BM <= lo) return;
+        }
+        f32x16_t s = f32x16_t{}, dp = f32x16_t{};
 #pragma unroll
-            for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, 0, x, lane), k[x], s);
+        for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, 0, x, lane), k[x], s);
 #pragma unroll
-            for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, 0, x, lane), v[x], dp);
-            const int i = i0 + 4 * half;
-            const bool masked = i0 < inner || i0 + BM > top;
-            const bool near = BIAS && i0 - (key0 + 31) < a.max_distance;
-            if (BIAS) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance, near, by_distance[a.max_distance]);
+        for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, 0, x, lane), v[x], dp);
+        const int i = i0 + 4 * half;
+        const bool near = BIAS && i0 - (key0 + 31) < a.max_distance;
+        if (BIAS) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance, near, by_distance[a.max_distance]);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4_t ls = *(const f32x4_t*)(st + 8 * g + 4 * half), de = *(const f32x4_t*)(st + BM + 8 * g + 4 * half);
+        for (int g = 0; g < 4; ++g) {
+            const f32x4_t ls = *(const f32x4_t*)(st + 8 * g + 4 * half), de = *(const f32x4_t*)(st + BM + 8 * g + 4 * half);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * g + e;
-                    float p = attn_exp2(BIAS ? s[r] - ls[e] : __builtin_fmaf(s[r], c, -ls[e]));
-                    float x = p * (dp[r] - de[e]);
-                    if (masked && (uint32_t)(i + e + 8 * g - key) >= reach) p = x = 0.0f;
-                    s[r] = p;
-                    dp[r] = x;
-                }
-            }
-            if (careful && masked) {
-                const f32x16_t pw[1] = {s}, xw[1] = {dp};
-                const auto sees = [&](int r) { return (uint32_t)(i0 + r - key) < reach; };
-                attn_careful<E, DP, 1>(ot, pw, gv, lane, sees);
-                attn_careful<E, DP, 1>(qt, xw, gk, lane, sees);
-            } else
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                f32x8_t p, x;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) { p[e] = s[8 * h + e]; x[e] = dp[8 * h + e]; }
-                const typename T::Frag pf = T::pack(p), xf = T::pack(x);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) gv[d] = T::mma(L::columns(ot, 16 * h, d, lane), pf, gv[d]);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) gk[d] = T::mma(L::columns(qt, 16 * h, d, lane), xf, gk[d]);
-            }
-            if (BIAS && a.partial) {
-                if (!near) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) far_sum += dp[r];
-                } else {
-                    // The tile of dS by diagonals (distance n = i - key has one value on each), then by buckets: lane b adds
-                    // up what belongs to bucket b (+ 64 u).  Fixed order throughout.
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = dp[r];
-                    __builtin_amdgcn_wave_barrier();
-                    const int n0 = i0 - key0 - 31;                    // distance of diagonal 0
-                    float on = 0.0f;
-                    for (int col = 0; col < 32; ++col) {
-                        const int r = lane + col - 31;                // r - col = lane - 31
-                        if (r >= 0 && r < 32) on += corner[r * 33 + col];
-                    }
-                    corner[32 * 33 + lane] = lane < 63 ? on : 0.0f;
-                    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                    for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
-                        const int b = lane + u * WAVE;
-                        if (u * WAVE < a.buckets && b < a.buckets) {
-                            const int from = b <= a.exact_to ? b : (int)a.borders[b - a.exact_to - 1];
-                            const int upto = b + 1 == a.buckets ? 1 << 30 : b + 1 <= a.exact_to ? b + 1 : (int)a.borders[b - a.exact_to];
-                            const int t0 = from - n0 > 0 ? from - n0 : 0, t1 = upto - n0 < 63 ? upto - n0 : 63;
-                            for (int t = t0; t < t1; ++t) in_bucket[u] += corner[32 * 33 + t];
-                        }
-                    }
-                    __builtin_amdgcn_wave_barrier();
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * g + e;
+                float p = attn_exp2(BIAS ? s[r] - ls[e] : __builtin_fmaf(s[r], c, -ls[e]));
+                float x = p * (dp[r] - de[e]);
+                if (MASKED && (uint32_t)(i + e + 8 * g - key) >= reach) p = x = 0.0f;
+                s[r] = p;
+                dp[r] = x;
             }
         }
-        const bool turn = ++step == steps;
-        if (turn) {
-            step = 0;
-            if (BIAS && a.partial) {
+        if (MASKED && terms) {
+            const f32x16_t pw[1] = {s}, xw[1] = {dp};
+            const auto sees = [&](int r) { return (uint32_t)(i0 + r - key) < reach; };
+            attn_add_terms<E, DP, 1>(ot, pw, gv, lane, sees);
+            attn_add_terms<E, DP, 1>(qt, xw, gk, lane, sees);
+        } else {
+            attn_add_product<E, DP>(ot, 0, s, gv, lane);
+            attn_add_product<E, DP>(qt, 0, dp, gk, lane);
+        }
+        if (BIAS && a.partial) {
+            if (!near) {
 #pragma unroll
-                for (int d = 32; d > 0; d >>= 1) far_sum += __shfl_xor(far_sum, d, WAVE);
+                for (int r = 0; r < 16; ++r) far_sum += dp[r];
+            } else {
+                // The tile of dS by diagonals (distance n = i - key has one value on each), then by buckets: lane b adds
+                // up what belongs to bucket b (+ 64 u).  Fixed order throughout.
+#pragma unroll
+                for (int r = 0; r < 16; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = there ? dp[r] : 0.0f;
+                __builtin_amdgcn_wave_barrier();
+                const int n0 = i0 - key0 - 31;                    // distance of diagonal 0
+                float on = 0.0f;
+                for (int col = 0; col < 32; ++col) {
+                    const int r = lane + col - 31;                // r - col = lane - 31
+                    if (r >= 0 && r < 32) on += corner[r * 33 + col];
+                }
+                corner[32 * 33 + lane] = lane < 63 ? on : 0.0f;
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
                     const int b = lane + u * WAVE;
-                    if (b < a.buckets) a.partial[((int64_t)head * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = in_bucket[u] + (b + 1 == a.buckets ? far_sum : 0.0f);
-                    in_bucket[u] = 0.0f;
+                    if (u * WAVE < a.buckets && b < a.buckets) {
+                        const int from = b <= a.exact_to ? b : (int)a.borders[b - a.exact_to - 1];
+                        const int upto = b + 1 == a.buckets ? 1 << 30 : b + 1 <= a.exact_to ? b + 1 : (int)a.borders[b - a.exact_to];
+                        const int t0 = from - n0 > 0 ? from - n0 : 0, t1 = upto - n0 < 63 ? upto - n0 : 63;
+                        for (int t = t0; t < t1; ++t) in_bucket[u] += corner[32 * 33 + t];
+                    }
                 }
-                far_sum = 0.0f;
+                __builtin_amdgcn_wave_barrier();
             }
-            ++head;
         }
-        if (more) stash(buf ^ 1);
-        __syncthreads();
-        if (BIAS && turn && more) {
+    };
+    int buf = 0;
+    for (int head = head0; head < head0 + a.group; ++head) {
+        if (BIAS) {
+            __syncthreads();                        // the table of the head before is not read any more
             attn_bias_by_distance(a, head, by_distance, tid);
+        }
+        auto turn = [&](int n) {
+            if (tid < 2 * BM) stats[buf * 2 * BM + tid] = stat;
+            attn_arrived();
             __syncthreads();
+            if (n + 1 < walk.total) fetch(head, n + 1, buf ^ 1);
+            else if (head + 1 < head0 + a.group) fetch(head + 1, 0, buf ^ 1);
+        };
+        for (int n = 0; n < walk.nclean; ++n, buf ^= 1) {
+            turn(n);
+            step(std::false_type{}, n, buf);
+        }
+        for (int n = walk.nclean; n < walk.total; ++n, buf ^= 1) {
+            turn(n);
+            step(std::true_type{}, n, buf);
+        }
+        if (BIAS && a.partial) {
+            far_sum = there ? far_sum : 0.0f;       // (a column without a key is masked in the tiles of the second loop only)
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) far_sum += __shfl_xor(far_sum, d, WAVE);
+#pragma unroll
+            for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
+                const int b = lane + u * WAVE;
+                if (b < a.buckets) a.partial[((int64_t)head * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = in_bucket[u] + (b + 1 == a.buckets ? far_sum : 0.0f);
+                in_bucket[u] = 0.0f;
+            }
+            far_sum = 0.0f;
         }
     }
-    if (careful || !__syncthreads_or(!attn_finite(gk) || !attn_finite(gv))) break;
-    careful = 1;
-    }
-    if (BIAS && a.partial && total == 0)      // no key of the block is in a sequence
-        for (int g = 0; g < a.group; ++g)
-            for (int b = lane; b < a.buckets; b += WAVE) a.partial[((int64_t)(head0 + g) * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = 0.0f;
     if (!there) return;
     const int64_t out = ((int64_t)key * kv_heads + kv) * a.dim;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int at = 32 * d + (r & 3) + 8 * (r >> 2) + 4 * half;
-            if (at < a.dim) {
-                if (a.gk) a.gk[out + at] = T::put(gk[d][r] * a.scale);
-                if (a.gv) a.gv[out + at] = T::put(gv[d][r]);
-            }
-        }
+    if (a.gk) attn_write_row<E, DP>(a.gk + out, gk, a.scale, a.dim, half, attn_whole(a.gk, a.dim));
+    if (a.gv) attn_write_row<E, DP>(a.gv + out, gv, 1.0f, a.dim, half, attn_whole(a.gv, a.dim));
 }
 
 // dtable[b][h]: the partial sums of the key tiles, in their order
@@ -878,7 +959,8 @@ inline bool attn_view(AttnView<E>& v, const void* base, const size_t* strides, s
     v.head = (int64_t)strides[1];
     v.elem = (int64_t)strides[2];
     constexpr size_t N = AttnType<E>::CHUNK;
-    v.vec = (strides[2] == 1 || dim == 1) && dim % N == 0 && strides[0] % N == 0 && strides[1] % N == 0 && (uintptr_t)v.p % 16 == 0;
+    // a tile of 64 rows is addressed with 32-bit offsets
+    v.vec = (strides[2] == 1 || dim == 1) && dim % N == 0 && strides[0] % N == 0 && strides[1] % N == 0 && (uintptr_t)v.p % 16 == 0 && strides[0] < (1u << 23);
     return true;
 }
 
