@@ -64,8 +64,10 @@ struct AttnArgs {
     int32_t buckets, exact_to, max_distance;
     float scale, scale_log2;   // scale_log2 = |scale| * log2(e); the sign goes into an operand
     E *out, *gq, *gk, *gv;
-    float *lse, *delta, *partial;
-    int32_t partial_tiles;
+    float *lse, *partial;
+    float* stats;              // [heads, tokens]: (lse in units of log2, D)
+    float *part_k, *part_v;    // with more than one part: [parts][tokens, kv_heads, dim] sums in f32
+    int32_t head_parts, query_parts, partial_tiles;
     int* flag;
     uint16_t borders[ATTN_MAX_BUCKETS / 2];      // distance at which bucket exact_to + 1 + m begins
 };
@@ -188,13 +190,26 @@ __device__ inline u32x4_t attn_piece(const E* row, int d, int dim, int64_t elem,
 // them before every read of LDS: attn_arrived() does, in front of the barrier that hands a tile over.  Anything else
 // (other strides, heads that are not whole pieces) goes through registers, element by element.
 // A token outside [lo, hi) is replaced by one inside: the mask hides what it brings.
-__device__ inline void attn_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ inline void attn_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+
+// BYTES (4 or 16) of every lane, from base + off to 64 * BYTES of LDS in a row.  (m0, the place in LDS, is read as the load is
+// issued; nothing else in these kernels uses it.)
+template <int BYTES>
+__device__ inline void attn_load_lds(const void* base, uint32_t off, const void* to) {
+    const uint64_t at = (uint64_t)(uintptr_t)base;
+    const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)const_cast<void*>(to));
+    if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
+}
 
 template <class E, int DP, int ROWS>
 struct AttnStage {
     using L = AttnTile<E, DP>;
     static constexpr int CALLS = ROWS * L::PITCH / 1024;       // wave instructions for a tile
-    static constexpr int N = (CALLS + ATTN_WAVES - 1) / ATTN_WAVES;
+    static constexpr int N = (CALLS + ATTN_WAVES - 1) / ATTN_WAVES;       // of a wave: that many, or (a small tile) none
+    static_assert(CALLS % ATTN_WAVES == 0 || CALLS < ATTN_WAVES, "what a wave waits for is counted");
     uint32_t off[N];                                           // bytes from the tile's first token to the lane's piece
     bool on[N];
     __device__ void begin(const AttnView<E>& view, int dim, int wave, int lane) {
@@ -228,13 +243,8 @@ struct AttnStage {
             if (on[u]) fetch(base, off[u] + (uint32_t)(in - token) * (uint32_t)view.token * (uint32_t)sizeof(E), tile, u, wave);
         }
     }
-    // (m0, the place in LDS, is read as the load is issued; nothing else in these kernels uses it)
     __device__ static void fetch(const E* base, uint32_t off, char* tile, int u, int wave) {
-        const uint64_t at = (uint64_t)(uintptr_t)base;
-        const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
-        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tile + (uint32_t)((u * ATTN_WAVES + wave) * 1024);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                     :: "s"(__builtin_amdgcn_readfirstlane(to)), "v"(off), "s"(from) : "memory");
+        attn_load_lds<16>(base, off, tile + (u * ATTN_WAVES + wave) * 1024);
     }
     __device__ static void slow(const AttnView<E>& view, int head, int token0, int lo, int hi, int dim, char* tile, int wave, int lane) {
         const E* const base = view.p + (int64_t)head * view.head;
@@ -446,6 +456,47 @@ struct AttnWalk {
     __device__ int at(int n) const { return n < nclean ? clean + n * STEP : n < nclean + nfront ? begin + (n - nclean) * STEP : dirty + (n - nclean - nfront) * STEP; }
 };
 
+// The tiles of a walk pass through a ring of `stages` (2 to 4) places in LDS: stages - 1 of them are on their way while one is
+// worked on.  A wave has issued PER loads for each, which come back in order: it waits until only those of the later tiles are
+// out, then meets the others.
+struct AttnRing {
+    int stages, at = 0, to = 0, ahead = 0;
+    __device__ explicit AttnRing(int stages_) : stages(stages_) {}
+    template <class Fetch>
+    __device__ __forceinline__ void fill(Fetch&& fetch) {          // fetch(place): false when there is nothing left
+        while (ahead < stages - 1 && fetch(to)) {
+            ++ahead;
+            to = to + 1 == stages ? 0 : to + 1;
+        }
+    }
+    template <int PER>
+    __device__ void arrived() const {
+        static_assert(3 * PER < 64, "the counter has six bits");
+        if (ahead == 1) attn_wait<0>();
+        else if (ahead == 2) attn_wait<PER>();
+        else attn_wait<2 * PER>();
+        __syncthreads();
+    }
+    __device__ void done() {
+        --ahead;
+        at = at + 1 == stages ? 0 : at + 1;
+    }
+};
+// the tiles [from, upto) of a walk: step(masked, tile, place)
+template <int PER, class Walk, class Fetch, class Step>
+__device__ __forceinline__ void attn_run(const Walk& walk, int from, int upto, AttnRing& ring, Fetch&& fetch, Step&& step) {
+    ring.fill(fetch);
+    auto turn = [&](auto masked, int n) __attribute__((always_inline)) {
+        ring.template arrived<PER>();
+        ring.fill(fetch);
+        step(masked, n, ring.at);
+        ring.done();
+    };
+    int n = from;
+    for (; n < upto && n < walk.nclean; ++n) turn(std::false_type{}, n);
+    for (; n < upto; ++n) turn(std::true_type{}, n);
+}
+
 // What a block has to know of its rows: 32 a wave.
 struct AttnSpan {
     int begin, end, inner, top;       // the other axis from begin to end; [inner, top) is what every row sees
@@ -502,14 +553,14 @@ constexpr size_t attn_tile_bytes(int rows) { return (size_t)rows * AttnTile<E, D
 constexpr float ATTN_BEHIND = 8.0f;
 
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles) {
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    float* const by_distance = (float*)(lds + 4 * BYTES);
+    float* const by_distance = (float*)(lds + stages * 2 * BYTES);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -525,21 +576,25 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
     vs.begin(a.v, a.dim, wave, lane);
     const AttnWalk<BN> walk(all.begin, all.end, all.inner, all.top);
     if (a.dim < DP) {
-        ks.clear(lds, 4 * BYTES, tid);
+        ks.clear(lds, stages * 2 * BYTES, tid);
         __syncthreads();
     }
-    auto fetch = [&](int n) {
-        char* const to = lds + (n & 1) * 2 * BYTES;
-        const int j0 = walk.at(n);
-        if (n < walk.nclean) {
+    AttnRing ring(stages);
+    int next = 0;
+    auto fetch = [&](int place) __attribute__((always_inline)) {
+        if (next == walk.total) return false;
+        char* const to = lds + place * 2 * BYTES;
+        const int j0 = walk.at(next);
+        if (next++ < walk.nclean) {
             ks.load(a.k, kv, j0, a.dim, to, wave, lane);
             vs.load(a.v, kv, j0, a.dim, to + BYTES, wave, lane);
         } else {
             ks.load_inside(a.k, kv, j0, all.begin, all.end, a.dim, to, wave, lane);
             vs.load_inside(a.v, kv, j0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
         }
+        return true;
     };
-    fetch(0);
+    ring.fill(fetch);
     typename T::Frag q[KS];
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
@@ -551,9 +606,9 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
     float m = -INFINITY, l = 0.0f;
-    auto step = [&](auto masked_, int n) {
+    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_)::value;
-        const char* const kt = lds + (n & 1) * 2 * BYTES;
+        const char* const kt = lds + place * 2 * BYTES;
         const char* const vt = kt + BYTES;
         const int j0 = walk.at(n);
         bool terms = false;
@@ -611,18 +666,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
             for (int b = 0; b < JB; ++b) attn_add_product<E, DP>(vt, 32 * b, s[b], acc, lane);
         }
     };
-    for (int n = 0; n < walk.nclean; ++n) {
-        attn_arrived();
-        __syncthreads();
-        if (n + 1 < walk.total) fetch(n + 1);
-        step(std::false_type{}, n);
-    }
-    for (int n = walk.nclean; n < walk.total; ++n) {
-        attn_arrived();
-        __syncthreads();
-        if (n + 1 < walk.total) fetch(n + 1);
-        step(std::true_type{}, n);
-    }
+    attn_run<2 * AttnStage<E, DP, BN>::N>(walk, 0, walk.total, ring, fetch, step);
     l += attn_other_half(l);
     if (!there) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing but -inf: an output of zeros
@@ -631,18 +675,18 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
 }
 
 // ---- backward: gradients of the queries ------------------------------------------------------------------------------------
-// A block owns 128 queries like the forward kernel.  Writes dq (if wanted) and, for the kernel of the keys, D_i: with a
+// A block owns 128 queries like the forward kernel.  Writes dq (if wanted) and, for the kernel of the keys, lse and D_i: with a
 // bias the one that makes the row of dS sum to zero (formed from P and dP themselves; the rounding of o in do . o
 // would otherwise enter every pair of the far bucket with the same sign).
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles) {
+__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    float* const by_distance = (float*)(lds + 4 * BYTES);
+    float* const by_distance = (float*)(lds + stages * 2 * BYTES);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -658,22 +702,26 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
     vs.begin(a.v, a.dim, wave, lane);
     const AttnWalk<BN> walk(all.begin, all.end, all.inner, all.top);
     if (a.dim < DP) {
-        ks.clear(lds, 4 * BYTES, tid);
+        ks.clear(lds, stages * 2 * BYTES, tid);
         __syncthreads();
     }
-    auto fetch = [&](int n) {
-        char* const to = lds + (n & 1) * 2 * BYTES;
-        const int j0 = walk.at(n);
-        if (n < walk.nclean) {
+    AttnRing ring(stages);
+    int next = 0;
+    auto fetch = [&](int place) __attribute__((always_inline)) {
+        if (next == walk.total) return false;
+        char* const to = lds + place * 2 * BYTES;
+        const int j0 = walk.at(next);
+        if (next++ < walk.nclean) {
             ks.load(a.k, kv, j0, a.dim, to, wave, lane);
             vs.load(a.v, kv, j0, a.dim, to + BYTES, wave, lane);
         } else {
             ks.load_inside(a.k, kv, j0, all.begin, all.end, a.dim, to, wave, lane);
             vs.load_inside(a.v, kv, j0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
         }
+        return true;
     };
     const bool walks = a.gq || (BIAS && (a.gk || a.partial));       // else only D_i is wanted, if that
-    if (walks) fetch(0);
+    if (walks) ring.fill(fetch);
     typename T::Frag q[KS], go[KS];
     attn_own_rows<E, DP>(a.go, head, there ? row : 0, there, a.dim, lane, 1.0f, go);
     float delta = 0.0f, lse2 = INFINITY;
@@ -685,15 +733,16 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(T::get(go[k], e), T::get(q[k], e), delta);
         delta += attn_other_half(delta);
     }
-    if (!walks) {
-        if (there && half == 0) a.delta[(int64_t)head * a.tokens + row] = delta;
-        return;
-    }
-    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (there) {
         const float x = a.lse[(int64_t)head * a.tokens + row];
         lse2 = x == -INFINITY ? INFINITY : x * ATTN_LOG2E;       // a row of nothing but -inf: P is zero
     }
+    float* const stat = a.stats + ((int64_t)head * a.tokens + row) * 2;
+    if (!walks) {
+        if (there && half == 0) { stat[0] = lse2; stat[1] = delta; }
+        return;
+    }
+    attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
     const int lower = there ? first : -1;
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
@@ -702,9 +751,9 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
     float rest = 0.0f;
-    auto step = [&](auto masked_, int n) {
+    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_)::value;
-        const char* const kt = lds + (n & 1) * 2 * BYTES;
+        const char* const kt = lds + place * 2 * BYTES;
         const char* const vt = kt + BYTES;
         const int j0 = walk.at(n);
         bool terms = false;
@@ -738,80 +787,78 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
             }
         }
     };
-    for (int n = 0; n < walk.nclean; ++n) {
-        attn_arrived();
-        __syncthreads();
-        if (n + 1 < walk.total) fetch(n + 1);
-        step(std::false_type{}, n);
-    }
-    for (int n = walk.nclean; n < walk.total; ++n) {
-        attn_arrived();
-        __syncthreads();
-        if (n + 1 < walk.total) fetch(n + 1);
-        step(std::true_type{}, n);
-    }
+    attn_run<2 * AttnStage<E, DP, BN>::N>(walk, 0, walk.total, ring, fetch, step);
     if (BIAS) rest += attn_other_half(rest);
     if (!there) return;
-    if (half == 0) a.delta[(int64_t)head * a.tokens + row] = BIAS ? delta + rest : delta;
+    if (half == 0) { stat[0] = lse2; stat[1] = BIAS ? delta + rest : delta; }
     if (a.gq) attn_write_row<E, DP>(a.gq + ((int64_t)row * a.heads + head) * a.dim, acc, a.scale, a.dim, half, attn_whole(a.gq, a.dim));
 }
 
 // ---- backward: gradients of the keys, the values and the bias table ----------------------------------------------------------
-// A block owns 128 keys of one key head and walks the queries of every head of its group from there on: the sums over
-// shared heads are made in registers, in a fixed order.
+// A block owns 128 keys of one key head and walks the queries of the heads of its group from there on: the sums over
+// shared heads are made in registers, in a fixed order.  Where that makes too few blocks for the chip, the heads and then
+// the queries are shared out among several blocks, whose sums a second kernel adds up, in a fixed order too.
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles) {
+__global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    float* const stats = (float*)(lds + 4 * BYTES);              // [2][lse2 | delta][BM]
-    float* const corner = stats + 4 * BM + wave * (32 * 33 + 64);   // (BIAS) a tile of dS of this wave, and the sums of its diagonals
-    float* const by_distance = stats + 4 * BM + 4 * (32 * 33 + 64);
-    const int kv_heads = a.heads / a.group;
+    constexpr int PLACE = 2 * BYTES + ATTN_WAVES * 8 * BM;       // queries, gradients of the output, and a copy of their statistics for each wave
+    float* const corner = (float*)(lds + stages * PLACE) + wave * (32 * 33 + 64);   // (BIAS) a tile of dS of this wave, and the sums of its diagonals
+    float* const by_distance = (float*)(lds + stages * PLACE) + ATTN_WAVES * (32 * 33 + 64);
+    const int kv_heads = a.heads / a.group, parts = a.head_parts * a.query_parts;
     int tile, kv;
-    attn_place(blockIdx.x, tiles, kv_heads, false, tile, kv);
+    attn_place(blockIdx.x, tiles, kv_heads * parts, false, tile, kv);
+    const int part = kv % parts, query_part = part % a.query_parts;
+    kv /= parts;
     const int key0 = tile * ATTN_ROWS + wave * 32, key = key0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, key, lane, first, last);
     const int lo = attn_wave_min(there ? key : 0x7fffffff), hi = attn_wave_max(there ? last : 0);     // queries this wave needs
     const AttnSpan all(lo, hi, attn_wave_max(there ? key : 0), attn_wave_min(there ? last : 0x7fffffff), span, wave, lane);
-    const int head0 = kv * a.group;
-    if (all.end <= all.begin) {                    // no key of the block is in a sequence
-        if (BIAS && a.partial)
-            for (int g = 0; g < a.group; ++g)
-                for (int b = lane; b < a.buckets; b += WAVE) a.partial[((int64_t)(head0 + g) * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = 0.0f;
-        return;
+    const int head0 = kv * a.group + part / a.query_parts * a.group / a.head_parts, heads = a.group / a.head_parts;
+    float* const sums = BIAS && a.partial ? a.partial + ((int64_t)head0 * a.partial_tiles + (query_part * tiles + tile) * ATTN_WAVES + wave) * a.buckets : nullptr;
+    const AttnWalk<BM> walk(all.begin, all.end > all.begin ? all.end : all.begin, all.inner, all.top);
+    const int from = (int)((int64_t)walk.total * query_part / a.query_parts), upto = (int)((int64_t)walk.total * (query_part + 1) / a.query_parts);
+    if (from == upto) {                            // no key of the block is in a sequence, or there are more parts than tiles
+        if (BIAS && sums)
+            for (int g = 0; g < heads; ++g)
+                for (int b = lane; b < a.buckets; b += WAVE) sums[(int64_t)g * a.partial_tiles * a.buckets + b] = 0.0f;
+        if (parts == 1) return;
     }
     AttnStage<E, DP, BM> qs, os;
     qs.begin(a.q, a.dim, wave, lane);
     os.begin(a.go, a.dim, wave, lane);
-    const AttnWalk<BM> walk(all.begin, all.end, all.inner, all.top);
     if (a.dim < DP) {
-        qs.clear(lds, 4 * BYTES, tid);
+        for (int p = 0; p < stages; ++p) qs.clear(lds + p * PLACE, 2 * BYTES, tid);
         __syncthreads();
     }
-    float stat = 0.0f;
-    auto fetch = [&](int head, int n, int buf) {
-        char* const to = lds + buf * 2 * BYTES;
-        const int i0 = walk.at(n);
-        if (n < walk.nclean) {
-            qs.load(a.q, head, i0, a.dim, to, wave, lane);
-            os.load(a.go, head, i0, a.dim, to + BYTES, wave, lane);
+    AttnRing ring(stages);
+    int next_head = head0, next = from;
+    auto fetch = [&](int place) __attribute__((always_inline)) {
+        if (next_head == head0 + heads || from == upto) return false;
+        char* const to = lds + place * PLACE;
+        const int i0 = walk.at(next);
+        const bool clean = next < walk.nclean;
+        if (clean) {
+            qs.load(a.q, next_head, i0, a.dim, to, wave, lane);
+            os.load(a.go, next_head, i0, a.dim, to + BYTES, wave, lane);
         } else {
-            qs.load_inside(a.q, head, i0, all.begin, all.end, a.dim, to, wave, lane);
-            os.load_inside(a.go, head, i0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
+            qs.load_inside(a.q, next_head, i0, all.begin, all.end, a.dim, to, wave, lane);
+            os.load_inside(a.go, next_head, i0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
         }
-        if (tid < 2 * BM) {
-            const int i = i0 + tid % BM;
-            const bool in = i < all.end;
-            const float x = in ? (tid < BM ? a.lse : a.delta)[(int64_t)head * a.tokens + i] : 0.0f;
-            stat = tid >= BM ? x : !in || x == -INFINITY ? INFINITY : x * ATTN_LOG2E;
+        const int i = i0 + (lane >> 1), in = i < all.end ? i : all.end - 1;
+        attn_load_lds<4>(a.stats + ((int64_t)next_head * a.tokens + i0) * 2, (uint32_t)((in - i0) * 8 + (lane & 1) * 4), to + 2 * BYTES + wave * 8 * BM);
+        if (++next == upto) {
+            next = from;
+            ++next_head;
         }
+        return true;
     };
-    fetch(head0, 0, 0);
+    ring.fill(fetch);
     typename T::Frag k[KS], v[KS];
     attn_own_rows<E, DP>(a.k, kv, there ? key : 0, there, a.dim, lane, attn_sign(a.scale), k);
     attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
@@ -821,11 +868,11 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
 #pragma unroll
     for (int d = 0; d < DB; ++d) { gk[d] = f32x16_t{}; gv[d] = f32x16_t{}; }
     float in_bucket[ATTN_MAX_BUCKETS / WAVE] = {0.0f, 0.0f, 0.0f, 0.0f}, far_sum = 0.0f;    // of the head at hand
-    auto step = [&](auto masked_, int n, int buf) {
+    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_)::value;
-        const char* const qt = lds + buf * 2 * BYTES;
+        const char* const qt = lds + place * PLACE;
         const char* const ot = qt + BYTES;
-        const float* const st = stats + buf * 2 * BM;
+        const float* const st = (const float*)(qt + 2 * BYTES) + wave * 2 * BM;      // (lse2, D) of each row
         const int i0 = walk.at(n);
         bool terms = false;
         if constexpr (MASKED) {
@@ -842,12 +889,13 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
         if (BIAS) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance, near, by_distance[a.max_distance]);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const f32x4_t ls = *(const f32x4_t*)(st + 8 * g + 4 * half), de = *(const f32x4_t*)(st + BM + 8 * g + 4 * half);
+            const f32x4_t st01 = *(const f32x4_t*)(st + 16 * g + 8 * half), st23 = *(const f32x4_t*)(st + 16 * g + 8 * half + 4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
-                float p = attn_exp2(BIAS ? s[r] - ls[e] : __builtin_fmaf(s[r], c, -ls[e]));
-                float x = p * (dp[r] - de[e]);
+                const float ls = e < 2 ? st01[2 * e] : st23[2 * e - 4], de = e < 2 ? st01[2 * e + 1] : st23[2 * e - 3];
+                float p = attn_exp2(BIAS ? s[r] - ls : __builtin_fmaf(s[r], c, -ls));
+                float x = p * (dp[r] - de);
                 if (MASKED && (uint32_t)(i + e + 8 * g - key) >= reach) p = x = 0.0f;
                 s[r] = p;
                 dp[r] = x;
@@ -862,7 +910,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
             attn_add_product<E, DP>(ot, 0, s, gv, lane);
             attn_add_product<E, DP>(qt, 0, dp, gk, lane);
         }
-        if (BIAS && a.partial) {
+        if (BIAS && sums) {
             if (!near) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) far_sum += dp[r];
@@ -894,35 +942,20 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
             }
         }
     };
-    int buf = 0;
-    for (int head = head0; head < head0 + a.group; ++head) {
+    for (int g = 0; g < heads; ++g) {
         if (BIAS) {
             __syncthreads();                        // the table of the head before is not read any more
-            attn_bias_by_distance(a, head, by_distance, tid);
+            attn_bias_by_distance(a, head0 + g, by_distance, tid);
         }
-        auto turn = [&](int n) {
-            if (tid < 2 * BM) stats[buf * 2 * BM + tid] = stat;
-            attn_arrived();
-            __syncthreads();
-            if (n + 1 < walk.total) fetch(head, n + 1, buf ^ 1);
-            else if (head + 1 < head0 + a.group) fetch(head + 1, 0, buf ^ 1);
-        };
-        for (int n = 0; n < walk.nclean; ++n, buf ^= 1) {
-            turn(n);
-            step(std::false_type{}, n, buf);
-        }
-        for (int n = walk.nclean; n < walk.total; ++n, buf ^= 1) {
-            turn(n);
-            step(std::true_type{}, n, buf);
-        }
-        if (BIAS && a.partial) {
+        attn_run<2 * AttnStage<E, DP, BM>::N + 1>(walk, from, upto, ring, fetch, step);
+        if (BIAS && sums && from < upto) {
             far_sum = there ? far_sum : 0.0f;       // (a column without a key is masked in the tiles of the second loop only)
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) far_sum += __shfl_xor(far_sum, d, WAVE);
 #pragma unroll
             for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
                 const int b = lane + u * WAVE;
-                if (b < a.buckets) a.partial[((int64_t)head * a.partial_tiles + tile * 4 + wave) * a.buckets + b] = in_bucket[u] + (b + 1 == a.buckets ? far_sum : 0.0f);
+                if (b < a.buckets) sums[(int64_t)g * a.partial_tiles * a.buckets + b] = in_bucket[u] + (b + 1 == a.buckets ? far_sum : 0.0f);
                 in_bucket[u] = 0.0f;
             }
             far_sum = 0.0f;
@@ -930,8 +963,37 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
     }
     if (!there) return;
     const int64_t out = ((int64_t)key * kv_heads + kv) * a.dim;
+    if (parts > 1) {
+        const int64_t size = (int64_t)a.tokens * kv_heads * a.dim;
+        attn_write_row<float, DP>(a.part_k + part * size + out, gk, a.scale, a.dim, half, a.dim % 4 == 0);
+        attn_write_row<float, DP>(a.part_v + part * size + out, gv, 1.0f, a.dim, half, a.dim % 4 == 0);
+        return;
+    }
     if (a.gk) attn_write_row<E, DP>(a.gk + out, gk, a.scale, a.dim, half, attn_whole(a.gk, a.dim));
     if (a.gv) attn_write_row<E, DP>(a.gv + out, gv, 1.0f, a.dim, half, attn_whole(a.gv, a.dim));
+}
+
+// dk and dv from their parts, in order; rows that no sequence holds are left as they are
+template <class E, int N>
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_parts_kernel(const AttnArgs<E> a, int parts, int64_t units, int row) {
+    const int64_t u = (int64_t)blockIdx.x * ATTN_THREADS + threadIdx.x;
+    if (u >= units) return;
+    const int token = (int)(u / (row / N));
+    if (token < a.offsets[0] || token >= a.offsets[a.sequences]) return;
+    const float* const from = blockIdx.y ? a.part_v : a.part_k;
+    E* const to = blockIdx.y ? a.gv : a.gk;
+    if (!to) return;
+    float x[N] = {};
+    for (int p = 0; p < parts; ++p) {
+        float y[N];
+        __builtin_memcpy(y, __builtin_assume_aligned(from + ((int64_t)p * units + u) * N, N * 4), sizeof(y));
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] += y[e];
+    }
+    E z[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e] = AttnType<E>::put(x[e]);
+    __builtin_memcpy(__builtin_assume_aligned(to + u * N, N * sizeof(E)), z, sizeof(z));
 }
 
 // dtable[b][h]: the partial sums of the key tiles, in their order
@@ -1011,34 +1073,57 @@ inline bool attn_lds(const void* kernel, size_t bytes, uint64_t& asked) {
     return true;
 }
 
+// Places of the ring: where a CU has one block at a time (256 CUs), as many as help (four) and fit, so that the time a tile takes
+// to arrive is spread over three steps; where it has two, what leaves room for both.
+inline int attn_stages(size_t place, size_t rest, unsigned blocks) {
+    const size_t room = (blocks <= 256 ? 160 * 1024 : 80 * 1024) - 512 - rest;
+    const size_t n = room / place;
+    return n >= 4 ? 4 : n >= 3 ? 3 : 2;
+}
 template <class E, int DP, bool BIAS>
 inline void attn_forward_launch(const AttnArgs<E>& a) {
     static uint64_t asked = 0;
     const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS;
-    const size_t lds = 4 * attn_tile_bytes<E, DP>(attn_keys<E>()) + (BIAS ? ((size_t)a.max_distance + 1) * 4 : 0);
+    const size_t place = 2 * attn_tile_bytes<E, DP>(attn_keys<E>()), rest = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
+    const unsigned blocks = (unsigned)(tiles * a.heads);
+    const int stages = attn_stages(place, rest, blocks);
     auto* kernel = attn_forward_kernel<E, DP, BIAS>;
-    if (!attn_lds((const void*)kernel, lds, asked)) return;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.heads)), dim3(ATTN_THREADS), lds, stream(), a, tiles);
+    if (!attn_lds((const void*)kernel, stages * place + rest, asked)) return;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + rest, stream(), a, tiles, stages);
     MXH_LAUNCH_CHECK("attention");
 }
 template <class E, int DP, bool BIAS>
 inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
     static uint64_t asked_q = 0, asked_k = 0;
-    const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS;
+    const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS, kv = a.heads / a.group;
     const size_t bias = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
     {
-        const size_t lds = 4 * attn_tile_bytes<E, DP>(attn_keys<E>()) + bias;
+        const size_t place = 2 * attn_tile_bytes<E, DP>(attn_keys<E>());
+        const unsigned blocks = (unsigned)(tiles * a.heads);
+        const int stages = attn_stages(place, bias, blocks);
         auto* kernel = attn_grad_query_kernel<E, DP, BIAS>;
-        if (!attn_lds((const void*)kernel, lds, asked_q)) return;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * a.heads)), dim3(ATTN_THREADS), lds, stream(), a, tiles);
+        if (!attn_lds((const void*)kernel, stages * place + bias, asked_q)) return;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + bias, stream(), a, tiles, stages);
         MXH_LAUNCH_CHECK("attention_backward (queries)");
     }
     if (a.gk || a.gv || grad_table) {
-        const size_t lds = 4 * attn_tile_bytes<E, DP>(32) + 4 * 32 * 4 + (BIAS ? (size_t)4 * (32 * 33 + 64) * 4 : 0) + bias;
+        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = (BIAS ? (size_t)ATTN_WAVES * (32 * 33 + 64) * 4 : 0) + bias;
+        const int parts = a.head_parts * a.query_parts;
+        const unsigned blocks = (unsigned)(tiles * kv * parts);
+        const int stages = attn_stages(place, rest, blocks);
         auto* kernel = attn_grad_key_kernel<E, DP, BIAS>;
-        if (!attn_lds((const void*)kernel, lds, asked_k)) return;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * (a.heads / a.group))), dim3(ATTN_THREADS), lds, stream(), a, tiles);
+        if (!attn_lds((const void*)kernel, stages * place + rest, asked_k)) return;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + rest, stream(), a, tiles, stages);
         MXH_LAUNCH_CHECK("attention_backward (keys)");
+        if (parts > 1 && (a.gk || a.gv)) {
+            const int row = kv * a.dim;
+            const bool whole = row % 4 == 0 && (uintptr_t)a.gk % (4 * sizeof(E)) == 0 && (uintptr_t)a.gv % (4 * sizeof(E)) == 0;
+            const int64_t units = (int64_t)a.tokens * row / (whole ? 4 : 1);
+            const dim3 grid(cdiv((size_t)units, (size_t)ATTN_THREADS), 2);
+            if (whole) hipLaunchKernelGGL((attn_join_parts_kernel<E, 4>), grid, dim3(ATTN_THREADS), 0, stream(), a, parts, units, row);
+            else hipLaunchKernelGGL((attn_join_parts_kernel<E, 1>), grid, dim3(ATTN_THREADS), 0, stream(), a, parts, units, row);
+            MXH_LAUNCH_CHECK("attention_backward (parts)");
+        }
     }
     if (grad_table) {
         hipLaunchKernelGGL(attn_grad_table_kernel<E>, dim3((unsigned)a.buckets, (unsigned)a.heads), dim3(ATTN_THREADS), 0, stream(), a.partial, a.partial_tiles, a.buckets, a.heads, grad_table);
@@ -1085,12 +1170,21 @@ inline void attention_backward_entry(const size_t* md, const int32_t* offsets, c
     a.gv = gv;
     const bool empty = a.tokens == 0 || a.sequences == 0;
     if (empty && !grad_table) return;
-    const size_t deltas = ((size_t)a.heads * a.tokens + 63) / 64 * 64;
-    a.partial_tiles = empty ? 0 : 4 * ((a.tokens + ATTN_ROWS - 1) / ATTN_ROWS);
+    // parts of the kernel of the keys: until there are two blocks for every CU, first the heads of a group, then the queries
+    // (eight tiles of them at least)
+    const size_t tiles = cdiv((size_t)a.tokens, (size_t)ATTN_ROWS), kv = (size_t)(a.heads / a.group);
+    a.head_parts = a.query_parts = 1;
+    while (a.head_parts < a.group && (tiles * kv * a.head_parts < 512 || a.group % a.head_parts != 0)) ++a.head_parts;
+    while (tiles * kv * a.head_parts * a.query_parts < 512 && (size_t)a.tokens / 32 / a.query_parts >= 16) a.query_parts *= 2;
+    const int parts = a.head_parts * a.query_parts;
+    const size_t stats = ((size_t)a.heads * a.tokens * 2 + 63) / 64 * 64, sums = parts > 1 ? ((size_t)a.tokens * kv * a.dim + 63) / 64 * 64 * parts : 0;
+    a.partial_tiles = empty ? 0 : (int)(ATTN_WAVES * tiles) * a.query_parts;
     const size_t partials = grad_table ? (size_t)a.heads * a.partial_tiles * a.buckets : 0;
-    a.delta = (float*)scratch((deltas + partials) * sizeof(float));
-    if (!a.delta) return;
-    a.partial = grad_table ? a.delta + deltas : nullptr;
+    a.stats = (float*)scratch((stats + 2 * sums + partials) * sizeof(float));
+    if (!a.stats) return;
+    a.part_k = a.stats + stats;
+    a.part_v = a.part_k + sums;
+    a.partial = grad_table ? a.part_v + sums : nullptr;
     if (empty) {
         hipLaunchKernelGGL(attn_grad_table_kernel<E>, dim3((unsigned)a.buckets, (unsigned)a.heads), dim3(ATTN_THREADS), 0, stream(), a.partial, 0, a.buckets, a.heads, grad_table);
         MXH_LAUNCH_CHECK("attention_backward (bias)");
