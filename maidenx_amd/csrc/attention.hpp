@@ -189,7 +189,7 @@ __device__ inline u32x4_t attn_piece(const E* row, int d, int dim, int64_t elem,
 // register in between, and are waited for a tile later.  The compiler does not know of these loads, so that it does not wait for
 // them before every read of LDS: attn_arrived() does, in front of the barrier that hands a tile over.  Anything else
 // (other strides, heads that are not whole pieces) goes through registers, element by element.
-// A token outside [lo, hi) is replaced by one inside: the mask hides what it brings.
+// A token behind the last one that counts is replaced by that one: the mask hides what it brings.
 template <int N>
 __device__ inline void attn_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
@@ -199,63 +199,54 @@ template <int BYTES>
 __device__ inline void attn_load_lds(const void* base, uint32_t off, const void* to) {
     const uint64_t at = (uint64_t)(uintptr_t)base;
     const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
-    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)const_cast<void*>(to));
+    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)to);      // (the low half of an address in LDS)
     if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
     else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
 }
 
-template <class E, int DP, int ROWS>
+// GROUP waves move the tiles of their own ring; `wave` is a wave's number among them.
+template <class E, int DP, int ROWS, int GROUP>
 struct AttnStage {
     using L = AttnTile<E, DP>;
     static constexpr int CALLS = ROWS * L::PITCH / 1024;       // wave instructions for a tile
-    static constexpr int N = (CALLS + ATTN_WAVES - 1) / ATTN_WAVES;       // of a wave: that many, or (a small tile) none
-    static_assert(CALLS % ATTN_WAVES == 0 || CALLS < ATTN_WAVES, "what a wave waits for is counted");
+    static constexpr int N = (CALLS + GROUP - 1) / GROUP;      // of a wave: that many, or (a small tile) none
+    static_assert(CALLS % GROUP == 0 || CALLS < GROUP, "what a wave waits for is counted");
     uint32_t off[N];                                           // bytes from the tile's first token to the lane's piece
     bool on[N];
     __device__ void begin(const AttnView<E>& view, int dim, int wave, int lane) {
 #pragma unroll
         for (int u = 0; u < N; ++u) {
-            const int slot = (u * ATTN_WAVES + wave) * 64 + lane, row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row);
+            const int slot = (u * GROUP + wave) * 64 + lane, row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row);
             off[u] = (uint32_t)(row * (int)view.token + piece * L::T::CHUNK) * (uint32_t)sizeof(E);
             on[u] = piece * L::T::CHUNK < dim && row < ROWS;
         }
     }
-    // pieces that no load brings (dim below DP) have to be zeros: once, for all tiles that lie there later
-    __device__ static void clear(char* tiles, int bytes, int tid) {
-        for (int at = tid * 16; at < bytes; at += ATTN_THREADS * 16) *(u32x4_t*)(tiles + at) = u32x4_t{0, 0, 0, 0};
-    }
-    // every row of the tile is a token inside
-    __device__ void load(const AttnView<E>& view, int head, int token0, int dim, char* tile, int wave, int lane) const {
-        if (!view.vec) return slow(view, head, token0, 0, 0x7fffffff, dim, tile, wave, lane);
+    // `inside`: every row of the tile is a token of [lo, hi); token0 is
+    __device__ __forceinline__ void load(const AttnView<E>& view, int head, int token0, bool inside, int hi, int dim, char* tile, int wave, int lane) const {
         const E* const base = view.p + (int64_t)head * view.head + (int64_t)token0 * view.token;
+        if (view.vec) {
 #pragma unroll
-        for (int u = 0; u < N; ++u)
-            if (on[u]) fetch(base, off[u], tile, u, wave);
-    }
-    __device__ void load_inside(const AttnView<E>& view, int head, int token0, int lo, int hi, int dim, char* tile, int wave, int lane) const {
-        if (!view.vec) return slow(view, head, token0, lo, hi, dim, tile, wave, lane);
-        const E* const base = view.p + (int64_t)head * view.head + (int64_t)token0 * view.token;
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int row = ((u * ATTN_WAVES + wave) * 64 + lane) / L::PIECES, token = token0 + row;
-            const int in = token < lo ? lo : token >= hi ? hi - 1 : token;
-            // (within a tile of the first token: 32 bits, as for the others)
-            if (on[u]) fetch(base, off[u] + (uint32_t)(in - token) * (uint32_t)view.token * (uint32_t)sizeof(E), tile, u, wave);
-        }
-    }
-    __device__ static void fetch(const E* base, uint32_t off, char* tile, int u, int wave) {
-        attn_load_lds<16>(base, off, tile + (u * ATTN_WAVES + wave) * 1024);
-    }
-    __device__ static void slow(const AttnView<E>& view, int head, int token0, int lo, int hi, int dim, char* tile, int wave, int lane) {
-        const E* const base = view.p + (int64_t)head * view.head;
+            for (int u = 0; u < N; ++u) {
+                uint32_t from = off[u];
+                if (!inside) {                 // (a row before the last one of the tile's: 32 bits, as for the others)
+                    const int row = ((u * GROUP + wave) * 64 + lane) / L::PIECES, beyond = token0 + row - (hi - 1);
+                    from -= beyond > 0 ? (uint32_t)beyond * (uint32_t)view.token * (uint32_t)sizeof(E) : 0u;
+                }
+                if (on[u]) attn_load_lds<16>(base, from, tile + (u * GROUP + wave) * 1024);
+            }
+        } else {
 #pragma nounroll
-        for (int slot = wave * 64 + lane; slot < ROWS * L::PIECES; slot += ATTN_THREADS) {
-            const int row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row), token = token0 + row;
-            const int in = token < lo ? lo : token >= hi ? hi - 1 : token;
-            *(u32x4_t*)(tile + slot * 16) = attn_piece<E>(base + (int64_t)in * view.token, piece * L::T::CHUNK, dim, view.elem, 0);
+            for (int slot = wave * 64 + lane; slot < ROWS * L::PIECES; slot += GROUP * 64) {
+                const int row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row), in = token0 + row < hi ? row : hi - 1 - token0;
+                *(u32x4_t*)(tile + slot * 16) = attn_piece<E>(base + (int64_t)in * view.token, piece * L::T::CHUNK, dim, view.elem, 0);
+            }
         }
     }
 };
+// pieces that no load brings (dim below DP) have to be zeros: once, for all tiles that lie there later
+__device__ inline void attn_clear(char* tiles, int bytes, int tid, int threads) {
+    for (int at = tid * 16; at < bytes; at += threads * 16) *(u32x4_t*)(tiles + at) = u32x4_t{0, 0, 0, 0};
+}
 
 // Row fragments straight from memory, held for the whole loop; `sign` 1, -1 or 0 is multiplied in (exact).
 template <class E, int DP>
@@ -304,13 +295,6 @@ __device__ inline bool attn_sequence(const int32_t* offsets, int sequences, int 
     last = hi > tokens ? tokens : hi;
     return row < tokens && lo >= 0 && above;
 }
-__device__ inline int attn_wave_min(int x) {
-#pragma unroll
-    for (int d = 1; d < WAVE; d <<= 1) { const int o = __shfl_xor(x, d, WAVE); x = o < x ? o : x; }
-    return __builtin_amdgcn_readfirstlane(x);
-}
-__device__ inline int attn_wave_max(int x) { return -attn_wave_min(-x); }
-
 // One wave of the first block looks the offsets over; the host reports what it finds with the next status.
 template <class E>
 __device__ inline void attn_check_offsets(const AttnArgs<E>& a) {
@@ -341,8 +325,8 @@ __device__ inline int attn_bucket(const AttnArgs<E>& a, int distance) {
 }
 // by_distance[n], n = 0 .. max_distance: the bias of head h in units of log2, the last for every distance from max_distance on
 template <class E>
-__device__ inline void attn_bias_by_distance(const AttnArgs<E>& a, int head, float* by_distance, int tid) {
-    for (int n = tid; n <= a.max_distance; n += ATTN_THREADS) {
+__device__ inline void attn_bias_by_distance(const AttnArgs<E>& a, int head, float* by_distance, int tid, int threads) {
+    for (int n = tid; n <= a.max_distance; n += threads) {
         const float b = AttnType<E>::get(a.table[(int64_t)attn_bucket(a, n) * a.heads + head]);
         // a finite bias stays finite: the type's lowest value is a value like any other, only -inf takes a pair out
         const float x = b * ATTN_LOG2E;
@@ -384,17 +368,18 @@ __device__ inline bool attn_finite(u32x4_t x) {
     }
     return fine;
 }
-// by all threads of a block, the tile being there: whether it holds such a value.  Two barriers' worth of waiting.
-template <class E>
-__device__ inline bool attn_look_over(const char* tile, int bytes, int* said, int tid, int wave, int lane) {
+// by the GROUP waves of a ring (tid among their threads), the tile being there: whether it holds such a value.  All waves of the block
+// come along.
+template <class E, int GROUP>
+__device__ inline bool attn_look_over(const char* tile, int bytes, int* said, int tid, int lane) {
     bool fine = true;
-    for (int at = tid * 16; at < bytes; at += ATTN_THREADS * 16) fine &= attn_finite<E>(*(const u32x4_t*)(tile + at));
+    for (int at = tid * 16; at < bytes; at += GROUP * 64 * 16) fine &= attn_finite<E>(*(const u32x4_t*)(tile + at));
     const bool any = __any(!fine);
-    if (lane == 0) said[wave] = any;
+    if (lane == 0) said[tid >> 6] = any;
     __syncthreads();
     int bad = 0;
 #pragma unroll
-    for (int w = 0; w < ATTN_WAVES; ++w) bad |= said[w];
+    for (int w = 0; w < GROUP; ++w) bad |= said[w];
     return __builtin_amdgcn_readfirstlane(bad) != 0;
 }
 template <class E, int DP, int TILES, class Sees>
@@ -496,28 +481,90 @@ __device__ __forceinline__ void attn_run(const Walk& walk, int from, int upto, A
     for (; n < upto && n < walk.nclean; ++n) turn(std::false_type{}, n);
     for (; n < upto; ++n) turn(std::true_type{}, n);
 }
-
-// What a block has to know of its rows: 32 a wave.
-struct AttnSpan {
-    int begin, end, inner, top;       // the other axis from begin to end; [inner, top) is what every row sees
-    // lo, hi: of a wave's rows (0x7fffffff, 0 for none); inner, top likewise (0, 0x7fffffff for none)
-    __device__ AttnSpan(int lo, int hi, int inner_, int top_, int* shared, int wave, int lane) {
-        if (lane == 0) { shared[wave] = lo; shared[4 + wave] = hi; shared[8 + wave] = inner_; shared[12 + wave] = top_; }
-        __syncthreads();
-        begin = shared[0]; end = shared[4]; inner = shared[8]; top = shared[12];
-#pragma unroll
-        for (int w = 1; w < ATTN_WAVES; ++w) {
-            begin = shared[w] < begin ? shared[w] : begin;
-            end = shared[4 + w] > end ? shared[4 + w] : end;
-            inner = shared[8 + w] > inner ? shared[8 + w] : inner;
-            top = shared[12 + w] < top ? shared[12 + w] : top;
-        }
-        begin = __builtin_amdgcn_readfirstlane(begin);
-        end = __builtin_amdgcn_readfirstlane(end);
-        inner = __builtin_amdgcn_readfirstlane(inner);
-        top = __builtin_amdgcn_readfirstlane(top);
+// A walk in rounds: in each, KG groups of waves take a tile of their own (every KG-th), all clean or none.  A group that is left without one in the
+// last round fetches one that it does not need: every wave counts the same loads.
+template <class Walk, int KG>
+struct AttnRounds {
+    const Walk& walk;
+    int group, clean, total;
+    __device__ AttnRounds(const Walk& walk_, int group_)
+        : walk(walk_), group(group_), clean((walk_.nclean + KG - 1) / KG), total(clean + (walk_.total - walk_.nclean + KG - 1) / KG) {}
+    __device__ int tile(int round) const { return round < clean ? round * KG + group : walk.nclean + (round - clean) * KG + group; }
+    __device__ int nearest(int round) const {
+        const int n = tile(round), last = (round < clean ? walk.nclean : walk.total) - 1;
+        return n < last ? n : last;
     }
 };
+template <int PER, class Rounds, class Fetch, class Step>
+__device__ __forceinline__ void attn_run_rounds(const Rounds& rounds, AttnRing& ring, Fetch&& fetch, Step&& step) {
+    auto turn = [&](auto masked, int round) __attribute__((always_inline)) {
+        ring.template arrived<PER>();
+        ring.fill(fetch);
+        step(masked, round, ring.at);
+        ring.done();
+    };
+    int round = 0;
+    for (; round < rounds.clean; ++round) turn(std::false_type{}, round);
+    for (; round < rounds.total; ++round) turn(std::true_type{}, round);
+}
+
+// What a wave has to know of its 32 rows, and a block of all its rows: the other axis from begin to end; [inner, top) is what
+// every row sees.  Rows see keys [first, row], keys are seen by queries [key, last): both ends ascend from row to row.
+struct AttnSpan {
+    int lo, hi, inner, top;
+    __device__ AttnSpan(bool there, int from, int upto) {         // what a lane's row sees
+        const uint32_t rows = (uint32_t)__ballot(there);           // (the halves of a wave say the same)
+        if (rows == 0) { lo = inner = 0; hi = 0; top = 0x7fffffff; return; }
+        const int a = __builtin_ctz(rows), b = 31 - __builtin_clz(rows);
+        lo = __builtin_amdgcn_readlane(from, a);
+        inner = __builtin_amdgcn_readlane(from, b);
+        top = __builtin_amdgcn_readlane(upto, a);
+        hi = __builtin_amdgcn_readlane(upto, b);
+    }
+    template <int WAVES>                                           // of the rows of WAVES waves
+    __device__ AttnSpan of_block(int* shared, int wave, int lane) const {
+        if (lane == 0) { shared[4 * wave] = hi > lo ? lo : 0x7fffffff; shared[4 * wave + 1] = hi; shared[4 * wave + 2] = inner; shared[4 * wave + 3] = top; }
+        __syncthreads();
+        AttnSpan all = *this;
+        all.lo = 0x7fffffff;
+        all.hi = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            all.lo = shared[4 * w] < all.lo ? shared[4 * w] : all.lo;
+            all.hi = shared[4 * w + 1] > all.hi ? shared[4 * w + 1] : all.hi;
+            all.inner = shared[4 * w + 2] > all.inner ? shared[4 * w + 2] : all.inner;
+            all.top = shared[4 * w + 3] < all.top ? shared[4 * w + 3] : all.top;
+        }
+        all.lo = __builtin_amdgcn_readfirstlane(all.lo);
+        all.hi = __builtin_amdgcn_readfirstlane(all.hi);
+        all.inner = __builtin_amdgcn_readfirstlane(all.inner);
+        all.top = __builtin_amdgcn_readfirstlane(all.top);
+        return all;
+    }
+};
+
+// Sums of another group of waves for the same rows, through LDS: `count` registers of a wave, four at a time.
+template <int DB>
+__device__ inline void attn_leave(float* to, const f32x16_t (&sums)[DB], float x, float y, int lane) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) *(f32x4_t*)(to + ((4 * d + g) * 64 + lane) * 4) = f32x4_t{sums[d][4 * g], sums[d][4 * g + 1], sums[d][4 * g + 2], sums[d][4 * g + 3]};
+    to[DB * 1024 + lane] = x;
+    to[DB * 1024 + 64 + lane] = y;
+}
+template <int DB>
+__device__ inline void attn_take(const float* from, f32x16_t (&sums)[DB], float by, float from_by, int lane) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4_t x = *(const f32x4_t*)(from + ((4 * d + g) * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[d][4 * g + e] = __builtin_fmaf(x[e], from_by, sums[d][4 * g + e] * by);
+        }
+}
+template <int DB> constexpr int attn_left() { return DB * 1024 + 128; }       // floats of a wave
 
 // rows of a result (index in the columns of the fragments), four neighbouring elements at a time where they lie on their boundaries
 template <class E, int DP>
@@ -552,15 +599,17 @@ constexpr size_t attn_tile_bytes(int rows) { return (size_t)rows * AttnTile<E, D
 // the running maximum may be this much (a factor of 2^8) behind before the sums are rescaled
 constexpr float ATTN_BEHIND = 8.0f;
 
-template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles, int stages) {
+template <class E, int DP, bool BIAS, int KG>
+__global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
+    constexpr int RG = ATTN_ROWS / 32, BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int span[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    float* const by_distance = (float*)(lds + stages * 2 * BYTES);
+    __shared__ int span[4 * RG * KG];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, group = __builtin_amdgcn_readfirstlane(tid / (64 * RG)), wave = __builtin_amdgcn_readfirstlane(tid / 64 % RG);
+    char* const mine = lds + group * stages * 2 * BYTES;         // the group's ring
+    int* const said = span + group * RG;
+    float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -568,36 +617,32 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
     const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
-    const int lo = attn_wave_min(there ? first : 0x7fffffff), hi = attn_wave_max(there ? row + 1 : 0);   // keys this wave needs
-    const AttnSpan all(lo, hi, attn_wave_max(there ? first : 0), attn_wave_min(there ? row + 1 : 0x7fffffff), span, wave, lane);
-    if (all.end <= all.begin) return;               // no row of the block is in a sequence
-    AttnStage<E, DP, BN> ks, vs;
+    const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
+    if (all.hi <= all.lo) return;                   // no row of the block is in a sequence
+    AttnStage<E, DP, BN, RG> ks, vs;
     ks.begin(a.k, a.dim, wave, lane);
     vs.begin(a.v, a.dim, wave, lane);
-    const AttnWalk<BN> walk(all.begin, all.end, all.inner, all.top);
+    const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
+    const AttnRounds<AttnWalk<BN>, KG> rounds(walk, group);
     if (a.dim < DP) {
-        ks.clear(lds, stages * 2 * BYTES, tid);
+        attn_clear(lds, KG * stages * 2 * BYTES, tid, 64 * RG * KG);
         __syncthreads();
     }
     AttnRing ring(stages);
     int next = 0;
     auto fetch = [&](int place) __attribute__((always_inline)) {
-        if (next == walk.total) return false;
-        char* const to = lds + place * 2 * BYTES;
-        const int j0 = walk.at(next);
-        if (next++ < walk.nclean) {
-            ks.load(a.k, kv, j0, a.dim, to, wave, lane);
-            vs.load(a.v, kv, j0, a.dim, to + BYTES, wave, lane);
-        } else {
-            ks.load_inside(a.k, kv, j0, all.begin, all.end, a.dim, to, wave, lane);
-            vs.load_inside(a.v, kv, j0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
-        }
+        if (next == rounds.total) return false;
+        char* const to = mine + place * 2 * BYTES;
+        const int j0 = walk.at(rounds.nearest(next));
+        const bool inside = next++ < rounds.clean;
+        ks.load(a.k, kv, j0, inside, all.hi, a.dim, to, wave, lane);
+        vs.load(a.v, kv, j0, inside, all.hi, a.dim, to + BYTES, wave, lane);
         return true;
     };
     ring.fill(fetch);
     typename T::Frag q[KS];
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
-    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
+    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
 
     const int lower = there ? first : -1;           // key j is seen if (unsigned)(j - lower) <= reach
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
@@ -606,15 +651,17 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
     float m = -INFINITY, l = 0.0f;
-    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
+    auto step = [&](auto masked_, int round, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_)::value;
-        const char* const kt = lds + place * 2 * BYTES;
+        const char* const kt = mine + place * 2 * BYTES;
         const char* const vt = kt + BYTES;
-        const int j0 = walk.at(n);
+        const int n = rounds.tile(round), j0 = walk.at(n);
+        const bool idle = KG > 1 && n >= (MASKED ? walk.total : walk.nclean);
+        if (!MASKED && idle) return;
         bool terms = false;
         if constexpr (MASKED) {
-            terms = attn_look_over<E>(vt, BYTES, span, tid, wave, lane);
-            if (j0 >= hi || j0 + BN <= lo) return;
+            terms = attn_look_over<E, RG>(vt, BYTES, said, tid % (64 * RG), lane);
+            if (idle || j0 >= own.hi || j0 + BN <= own.lo) return;
         }
         f32x16_t s[JB];
 #pragma unroll
@@ -666,7 +713,22 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
             for (int b = 0; b < JB; ++b) attn_add_product<E, DP>(vt, 32 * b, s[b], acc, lane);
         }
     };
-    attn_run<2 * AttnStage<E, DP, BN>::N>(walk, 0, walk.total, ring, fetch, step);
+    attn_run_rounds<2 * AttnStage<E, DP, BN, RG>::N>(rounds, ring, fetch, step);
+    if constexpr (KG > 1) {
+        __syncthreads();                            // the rings are not needed any more
+        float* const left = (float*)lds;
+        if (group > 0) attn_leave<DB>(left + ((group - 1) * RG + wave) * attn_left<DB>(), acc, m, l, lane);
+        __syncthreads();
+        if (group > 0) return;
+        for (int g = 1; g < KG; ++g) {
+            const float* const from = left + ((g - 1) * RG + wave) * attn_left<DB>();
+            const float m2 = from[DB * 1024 + lane], l2 = from[DB * 1024 + 64 + lane], next = fmaxf(m, m2);
+            const float by = next == -INFINITY ? 1.0f : attn_exp2(m - next), by2 = next == -INFINITY ? 1.0f : attn_exp2(m2 - next);
+            attn_take<DB>(from, acc, by, by2, lane);
+            l = __builtin_fmaf(l2, by2, l * by);
+            m = next;
+        }
+    }
     l += attn_other_half(l);
     if (!there) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing but -inf: an output of zeros
@@ -678,15 +740,17 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_forward_kernel(const Att
 // A block owns 128 queries like the forward kernel.  Writes dq (if wanted) and, for the kernel of the keys, lse and D_i: with a
 // bias the one that makes the row of dS sum to zero (formed from P and dP themselves; the rounding of o in do . o
 // would otherwise enter every pair of the far bucket with the same sign).
-template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
+template <class E, int DP, bool BIAS, int KG>
+__global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
+    constexpr int RG = ATTN_ROWS / 32, BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ int span[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    float* const by_distance = (float*)(lds + stages * 2 * BYTES);
+    __shared__ int span[4 * RG * KG];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, group = __builtin_amdgcn_readfirstlane(tid / (64 * RG)), wave = __builtin_amdgcn_readfirstlane(tid / 64 % RG);
+    char* const mine = lds + group * stages * 2 * BYTES;         // the group's ring
+    int* const said = span + group * RG;
+    float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -694,30 +758,26 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
     const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
-    const int lo = attn_wave_min(there ? first : 0x7fffffff), hi = attn_wave_max(there ? row + 1 : 0);
-    const AttnSpan all(lo, hi, attn_wave_max(there ? first : 0), attn_wave_min(there ? row + 1 : 0x7fffffff), span, wave, lane);
-    if (all.end <= all.begin) return;
-    AttnStage<E, DP, BN> ks, vs;
+    const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
+    if (all.hi <= all.lo) return;
+    AttnStage<E, DP, BN, RG> ks, vs;
     ks.begin(a.k, a.dim, wave, lane);
     vs.begin(a.v, a.dim, wave, lane);
-    const AttnWalk<BN> walk(all.begin, all.end, all.inner, all.top);
+    const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
+    const AttnRounds<AttnWalk<BN>, KG> rounds(walk, group);
     if (a.dim < DP) {
-        ks.clear(lds, stages * 2 * BYTES, tid);
+        attn_clear(lds, KG * stages * 2 * BYTES, tid, 64 * RG * KG);
         __syncthreads();
     }
     AttnRing ring(stages);
     int next = 0;
     auto fetch = [&](int place) __attribute__((always_inline)) {
-        if (next == walk.total) return false;
-        char* const to = lds + place * 2 * BYTES;
-        const int j0 = walk.at(next);
-        if (next++ < walk.nclean) {
-            ks.load(a.k, kv, j0, a.dim, to, wave, lane);
-            vs.load(a.v, kv, j0, a.dim, to + BYTES, wave, lane);
-        } else {
-            ks.load_inside(a.k, kv, j0, all.begin, all.end, a.dim, to, wave, lane);
-            vs.load_inside(a.v, kv, j0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
-        }
+        if (next == rounds.total) return false;
+        char* const to = mine + place * 2 * BYTES;
+        const int j0 = walk.at(rounds.nearest(next));
+        const bool inside = next++ < rounds.clean;
+        ks.load(a.k, kv, j0, inside, all.hi, a.dim, to, wave, lane);
+        vs.load(a.v, kv, j0, inside, all.hi, a.dim, to + BYTES, wave, lane);
         return true;
     };
     const bool walks = a.gq || (BIAS && (a.gk || a.partial));       // else only D_i is wanted, if that
@@ -739,11 +799,11 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
     }
     float* const stat = a.stats + ((int64_t)head * a.tokens + row) * 2;
     if (!walks) {
-        if (there && half == 0) { stat[0] = lse2; stat[1] = delta; }
+        if (there && half == 0 && group == 0) { stat[0] = lse2; stat[1] = delta; }
         return;
     }
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
-    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid);
+    if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
     const int lower = there ? first : -1;
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
     const float c = a.scale_log2;
@@ -751,15 +811,17 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
     float rest = 0.0f;
-    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
+    auto step = [&](auto masked_, int round, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_)::value;
-        const char* const kt = lds + place * 2 * BYTES;
+        const char* const kt = mine + place * 2 * BYTES;
         const char* const vt = kt + BYTES;
-        const int j0 = walk.at(n);
+        const int n = rounds.tile(round), j0 = walk.at(n);
+        const bool idle = KG > 1 && n >= (MASKED ? walk.total : walk.nclean);
+        if (!MASKED && idle) return;
         bool terms = false;
         if constexpr (MASKED) {
-            terms = attn_look_over<E>(kt, BYTES, span, tid, wave, lane);
-            if (j0 >= hi || j0 + BN <= lo) return;
+            terms = attn_look_over<E, RG>(kt, BYTES, said, tid % (64 * RG), lane);
+            if (idle || j0 >= own.hi || j0 + BN <= own.lo) return;
         }
         const bool near = BIAS && row0 - (j0 + BN - 1) < a.max_distance;
         const float far_bias = BIAS ? by_distance[a.max_distance] : 0.0f;
@@ -787,7 +849,19 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
             }
         }
     };
-    attn_run<2 * AttnStage<E, DP, BN>::N>(walk, 0, walk.total, ring, fetch, step);
+    attn_run_rounds<2 * AttnStage<E, DP, BN, RG>::N>(rounds, ring, fetch, step);
+    if constexpr (KG > 1) {
+        __syncthreads();
+        float* const left = (float*)lds;
+        if (group > 0) attn_leave<DB>(left + ((group - 1) * RG + wave) * attn_left<DB>(), acc, rest, 0.0f, lane);
+        __syncthreads();
+        if (group > 0) return;
+        for (int g = 1; g < KG; ++g) {
+            const float* const from = left + ((g - 1) * RG + wave) * attn_left<DB>();
+            attn_take<DB>(from, acc, 1.0f, 1.0f, lane);
+            rest += from[DB * 1024 + lane];
+        }
+    }
     if (BIAS) rest += attn_other_half(rest);
     if (!there) return;
     if (half == 0) { stat[0] = lse2; stat[1] = BIAS ? delta + rest : delta; }
@@ -799,7 +873,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 4 && DP > 64 ? 1 : 2) vo
 // shared heads are made in registers, in a fixed order.  Where that makes too few blocks for the chip, the heads and then
 // the queries are shared out among several blocks, whose sums a second kernel adds up, in a fixed order too.
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
+__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH;
@@ -817,11 +891,10 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
     const int key0 = tile * ATTN_ROWS + wave * 32, key = key0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, key, lane, first, last);
-    const int lo = attn_wave_min(there ? key : 0x7fffffff), hi = attn_wave_max(there ? last : 0);     // queries this wave needs
-    const AttnSpan all(lo, hi, attn_wave_max(there ? key : 0), attn_wave_min(there ? last : 0x7fffffff), span, wave, lane);
+    const AttnSpan own(there, key, last), all = own.of_block<ATTN_WAVES>(span, wave, lane);      // queries
     const int head0 = kv * a.group + part / a.query_parts * a.group / a.head_parts, heads = a.group / a.head_parts;
     float* const sums = BIAS && a.partial ? a.partial + ((int64_t)head0 * a.partial_tiles + (query_part * tiles + tile) * ATTN_WAVES + wave) * a.buckets : nullptr;
-    const AttnWalk<BM> walk(all.begin, all.end > all.begin ? all.end : all.begin, all.inner, all.top);
+    const AttnWalk<BM> walk(all.lo, all.hi > all.lo ? all.hi : all.lo, all.inner, all.top);
     const int from = (int)((int64_t)walk.total * query_part / a.query_parts), upto = (int)((int64_t)walk.total * (query_part + 1) / a.query_parts);
     if (from == upto) {                            // no key of the block is in a sequence, or there are more parts than tiles
         if (BIAS && sums)
@@ -829,11 +902,11 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
                 for (int b = lane; b < a.buckets; b += WAVE) sums[(int64_t)g * a.partial_tiles * a.buckets + b] = 0.0f;
         if (parts == 1) return;
     }
-    AttnStage<E, DP, BM> qs, os;
+    AttnStage<E, DP, BM, ATTN_WAVES> qs, os;
     qs.begin(a.q, a.dim, wave, lane);
     os.begin(a.go, a.dim, wave, lane);
     if (a.dim < DP) {
-        for (int p = 0; p < stages; ++p) qs.clear(lds + p * PLACE, 2 * BYTES, tid);
+        for (int p = 0; p < stages; ++p) attn_clear(lds + p * PLACE, 2 * BYTES, tid, ATTN_THREADS);
         __syncthreads();
     }
     AttnRing ring(stages);
@@ -842,15 +915,10 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
         if (next_head == head0 + heads || from == upto) return false;
         char* const to = lds + place * PLACE;
         const int i0 = walk.at(next);
-        const bool clean = next < walk.nclean;
-        if (clean) {
-            qs.load(a.q, next_head, i0, a.dim, to, wave, lane);
-            os.load(a.go, next_head, i0, a.dim, to + BYTES, wave, lane);
-        } else {
-            qs.load_inside(a.q, next_head, i0, all.begin, all.end, a.dim, to, wave, lane);
-            os.load_inside(a.go, next_head, i0, all.begin, all.end, a.dim, to + BYTES, wave, lane);
-        }
-        const int i = i0 + (lane >> 1), in = i < all.end ? i : all.end - 1;
+        const bool inside = next < walk.nclean;
+        qs.load(a.q, next_head, i0, inside, all.hi, a.dim, to, wave, lane);
+        os.load(a.go, next_head, i0, inside, all.hi, a.dim, to + BYTES, wave, lane);
+        const int i = i0 + (lane >> 1), in = i < all.hi ? i : all.hi - 1;
         attn_load_lds<4>(a.stats + ((int64_t)next_head * a.tokens + i0) * 2, (uint32_t)((in - i0) * 8 + (lane & 1) * 4), to + 2 * BYTES + wave * 8 * BM);
         if (++next == upto) {
             next = from;
@@ -876,8 +944,8 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
         const int i0 = walk.at(n);
         bool terms = false;
         if constexpr (MASKED) {
-            terms = attn_look_over<E>(qt, 2 * BYTES, span, tid, wave, lane);
-            if (i0 >= hi || i0 + BM <= lo) return;
+            terms = attn_look_over<E, ATTN_WAVES>(qt, 2 * BYTES, span, tid, lane);
+            if (i0 >= own.hi || i0 + BM <= own.lo) return;
         }
         f32x16_t s = f32x16_t{}, dp = f32x16_t{};
 #pragma unroll
@@ -945,9 +1013,9 @@ __global__ __launch_bounds__(ATTN_THREADS, 1) void attn_grad_key_kernel(const At
     for (int g = 0; g < heads; ++g) {
         if (BIAS) {
             __syncthreads();                        // the table of the head before is not read any more
-            attn_bias_by_distance(a, head0 + g, by_distance, tid);
+            attn_bias_by_distance(a, head0 + g, by_distance, tid, ATTN_THREADS);
         }
-        attn_run<2 * AttnStage<E, DP, BM>::N + 1>(walk, from, upto, ring, fetch, step);
+        attn_run<2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1>(walk, from, upto, ring, fetch, step);
         if (BIAS && sums && from < upto) {
             far_sum = there ? far_sum : 0.0f;       // (a column without a key is masked in the tiles of the second loop only)
 #pragma unroll
@@ -1063,7 +1131,7 @@ inline bool attn_arguments(AttnArgs<E>& a, const size_t* md, const int32_t* offs
 
 // more than 64 KB of LDS has to be asked for, once for each kernel and device
 inline bool attn_lds(const void* kernel, size_t bytes, uint64_t& asked) {
-    if (bytes <= 65536) return true;
+    if (bytes <= 60 * 1024) return true;
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) { set_status(ERR_INVALID, "attention: bad device"); return false; }
     if (asked >> dev & 1) return true;
@@ -1073,44 +1141,53 @@ inline bool attn_lds(const void* kernel, size_t bytes, uint64_t& asked) {
     return true;
 }
 
-// Places of the ring: where a CU has one block at a time (256 CUs), as many as help (four) and fit, so that the time a tile takes
-// to arrive is spread over three steps; where it has two, what leaves room for both.
-inline int attn_stages(size_t place, size_t rest, unsigned blocks) {
-    const size_t room = (blocks <= 256 ? 160 * 1024 : 80 * 1024) - 512 - rest;
-    const size_t n = room / place;
+// Places of a ring: as many as help (four) and fit beside `rest`, `blocks` sharing a CU's LDS, `rings` a block's.
+inline int attn_stages(size_t place, size_t rest, int rings, int blocks) {
+    const size_t n = (160 * 1024 / blocks - 512 - rest) / (place * rings);
     return n >= 4 ? 4 : n >= 3 ? 3 : 2;
 }
+template <int KG, class Kernel, class E>
+inline void attn_row_launch(Kernel* kernel, const AttnArgs<E>& a, int tiles, size_t place, size_t rest, uint64_t& asked, const char* what) {
+    const unsigned blocks = (unsigned)(tiles * a.heads);
+    const int stages = attn_stages(place, rest, KG, KG > 1 || blocks <= 256 ? 1 : 2);
+    const size_t lds = KG * stages * place + rest;
+    if (!attn_lds((const void*)kernel, lds, asked)) return;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_ROWS * 2 * KG), lds, stream(), a, tiles, stages);
+    MXH_LAUNCH_CHECK(what);
+}
+// Up to two rounds of two blocks for every CU, the time is that of the longest walks: two groups of waves share each
+// (one block of 512 threads to a CU; f32 heads above 64 take too many registers for that).
+template <class E, int DP>
+inline bool attn_two_groups(const AttnArgs<E>& a, int tiles) { return !(sizeof(E) == 4 && DP > 64) && (int64_t)tiles * a.heads <= 1024; }
+
 template <class E, int DP, bool BIAS>
 inline void attn_forward_launch(const AttnArgs<E>& a) {
-    static uint64_t asked = 0;
+    static uint64_t asked[2] = {0, 0};
     const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS;
     const size_t place = 2 * attn_tile_bytes<E, DP>(attn_keys<E>()), rest = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
-    const unsigned blocks = (unsigned)(tiles * a.heads);
-    const int stages = attn_stages(place, rest, blocks);
-    auto* kernel = attn_forward_kernel<E, DP, BIAS>;
-    if (!attn_lds((const void*)kernel, stages * place + rest, asked)) return;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + rest, stream(), a, tiles, stages);
-    MXH_LAUNCH_CHECK("attention");
+    if constexpr (!(sizeof(E) == 4 && DP > 64))
+        if (attn_two_groups<E, DP>(a, tiles)) return attn_row_launch<2>(attn_forward_kernel<E, DP, BIAS, 2>, a, tiles, place, rest, asked[1], "attention");
+    attn_row_launch<1>(attn_forward_kernel<E, DP, BIAS, 1>, a, tiles, place, rest, asked[0], "attention");
 }
 template <class E, int DP, bool BIAS>
 inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
-    static uint64_t asked_q = 0, asked_k = 0;
+    static uint64_t asked_q[2] = {0, 0}, asked_k = 0;
     const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS, kv = a.heads / a.group;
     const size_t bias = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
     {
         const size_t place = 2 * attn_tile_bytes<E, DP>(attn_keys<E>());
-        const unsigned blocks = (unsigned)(tiles * a.heads);
-        const int stages = attn_stages(place, bias, blocks);
-        auto* kernel = attn_grad_query_kernel<E, DP, BIAS>;
-        if (!attn_lds((const void*)kernel, stages * place + bias, asked_q)) return;
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + bias, stream(), a, tiles, stages);
-        MXH_LAUNCH_CHECK("attention_backward (queries)");
+        bool two = false;
+        if constexpr (!(sizeof(E) == 4 && DP > 64)) {
+            two = attn_two_groups<E, DP>(a, tiles);
+            if (two) attn_row_launch<2>(attn_grad_query_kernel<E, DP, BIAS, 2>, a, tiles, place, bias, asked_q[1], "attention_backward (queries)");
+        }
+        if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias, asked_q[0], "attention_backward (queries)");
     }
     if (a.gk || a.gv || grad_table) {
         const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = (BIAS ? (size_t)ATTN_WAVES * (32 * 33 + 64) * 4 : 0) + bias;
         const int parts = a.head_parts * a.query_parts;
         const unsigned blocks = (unsigned)(tiles * kv * parts);
-        const int stages = attn_stages(place, rest, blocks);
+        const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && DP <= 64 && blocks > 256 ? 2 : 1);
         auto* kernel = attn_grad_key_kernel<E, DP, BIAS>;
         if (!attn_lds((const void*)kernel, stages * place + rest, asked_k)) return;
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + rest, stream(), a, tiles, stages);
