@@ -323,30 +323,39 @@ __device__ inline int attn_bucket(const AttnArgs<E>& a, int distance) {
     for (int m = 0; m < a.buckets - a.exact_to - 1; ++m) b += distance >= (int)a.borders[m];
     return b;
 }
-// by_distance[n], n = 0 .. max_distance: the bias of head h in units of log2, the last for every distance from max_distance on
+// in units of log2; a finite bias stays finite: the type's lowest value is a value like any other, only -inf takes a pair out
+template <class E>
+__device__ inline float attn_bias(const AttnArgs<E>& a, int head, int bucket) {
+    const float b = AttnType<E>::get(a.table[(int64_t)bucket * a.heads + head]), x = b * ATTN_LOG2E;
+    return __builtin_isinf(b) ? b : x > ATTN_FLT_MAX ? ATTN_FLT_MAX : x < -ATTN_FLT_MAX ? -ATTN_FLT_MAX : x;
+}
+// by_distance[n], n = 0 .. max_distance: the bias of a head, the last for every distance from max_distance on
 template <class E>
 __device__ inline void attn_bias_by_distance(const AttnArgs<E>& a, int head, float* by_distance, int tid, int threads) {
-    for (int n = tid; n <= a.max_distance; n += threads) {
-        const float b = AttnType<E>::get(a.table[(int64_t)attn_bucket(a, n) * a.heads + head]);
-        // a finite bias stays finite: the type's lowest value is a value like any other, only -inf takes a pair out
-        const float x = b * ATTN_LOG2E;
-        by_distance[n] = __builtin_isinf(b) ? b : x > ATTN_FLT_MAX ? ATTN_FLT_MAX : x < -ATTN_FLT_MAX ? -ATTN_FLT_MAX : x;
+    for (int n = tid; n <= a.max_distance; n += threads) by_distance[n] = attn_bias(a, head, attn_bucket(a, n));
+}
+// Every distance from max_distance on has one bias: a tile of such pairs starts its product there (in units of the product),
+// and costs nothing.  Where that cannot be represented - a bias near the type's limits - the tile goes the way of a near one.
+struct AttnFar {
+    float start;
+    bool apart;
+    __device__ AttnFar(float bias, float c) : start(bias / c), apart(!(__builtin_fabsf(bias) < 1e30f * c) && bias != -INFINITY) {}
+};
+// The scores, in units of log2, that a lane holds at distances d0 - (r % 4) - 8 (r / 4), times STEP (1: rows are keys, -1: queries)
+template <int STEP>
+__device__ inline void attn_add_bias(f32x16_t& s, float c, const float* by_distance, int d0, int max_distance) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        int n = d0 - STEP * ((r & 3) + 8 * (r >> 2));
+        n = n < 0 ? 0 : n > max_distance ? max_distance : n;
+        s[r] = __builtin_fmaf(s[r], c, by_distance[n]);
     }
 }
-// Adds the bias to scores that a lane holds at distances d0 - (r % 4) - 8 (r / 4), times step (1: rows are keys, -1: queries)
-template <int STEP>
-__device__ inline void attn_add_bias(f32x16_t& s, float c, const float* by_distance, int d0, int max_distance, bool near, float far_bias) {
-    if (near) {
+__device__ inline f32x16_t attn_start(float x) {
+    f32x16_t s;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            int n = d0 - STEP * ((r & 3) + 8 * (r >> 2));
-            n = n < 0 ? 0 : n > max_distance ? max_distance : n;
-            s[r] = __builtin_fmaf(s[r], c, by_distance[n]);
-        }
-    } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, far_bias);
-    }
+    for (int r = 0; r < 16; ++r) s[r] = x;
+    return s;
 }
 
 // ---- what a mask hides -----------------------------------------------------------------------------------------------------
@@ -643,6 +652,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     typename T::Frag q[KS];
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
+    const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_log2);
 
     const int lower = there ? first : -1;           // key j is seen if (unsigned)(j - lower) <= reach
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
@@ -664,19 +674,19 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
             if (idle || j0 >= own.hi || j0 + BN <= own.lo) return;
         }
         f32x16_t s[JB];
+        const bool near = BIAS && (far.apart || row0 - (j0 + BN - 1) < a.max_distance);
 #pragma unroll
         for (int b = 0; b < JB; ++b) {
-            s[b] = f32x16_t{};
+            s[b] = attn_start(BIAS && !near ? far.start : 0.0f);
 #pragma unroll
             for (int k = 0; k < KS; ++k) s[b] = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s[b]);
         }
         const int j = j0 + 4 * half;                // key of row 0 of the lane's results
-        if (BIAS) {
-            const bool near = row0 - (j0 + BN - 1) < a.max_distance;
-            const float far_bias = by_distance[a.max_distance];
+        if (BIAS && near) {
 #pragma unroll
-            for (int b = 0; b < JB; ++b) attn_add_bias<1>(s[b], c, by_distance, row - j - 32 * b, a.max_distance, near, far_bias);
+            for (int b = 0; b < JB; ++b) attn_add_bias<1>(s[b], c, by_distance, row - j - 32 * b, a.max_distance);
         }
+        const float cc = BIAS && near ? 1.0f : c;   // what is left to multiply the scores by
         if constexpr (MASKED) {
 #pragma unroll
             for (int b = 0; b < JB; ++b)
@@ -690,7 +700,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 #pragma unroll
             for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
         best = fmaxf(best, attn_other_half(best));
-        if (!BIAS) best *= c;
+        best *= cc;
         if (__any(best > m + ATTN_BEHIND)) {
             const float next = fmaxf(m, best), fix = next == -INFINITY ? 1.0f : attn_exp2(m - next);
             l *= fix;
@@ -703,7 +713,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
         for (int b = 0; b < JB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[b][r] = attn_exp2(BIAS ? s[b][r] - base : __builtin_fmaf(s[b][r], c, -base));
+                s[b][r] = attn_exp2(__builtin_fmaf(s[b][r], cc, -base));
                 l += s[b][r];
             }
         if (MASKED && terms) {
@@ -804,6 +814,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     }
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
+    const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_log2);
     const int lower = there ? first : -1;
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
     const float c = a.scale_log2;
@@ -823,20 +834,20 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
             terms = attn_look_over<E, RG>(kt, BYTES, said, tid % (64 * RG), lane);
             if (idle || j0 >= own.hi || j0 + BN <= own.lo) return;
         }
-        const bool near = BIAS && row0 - (j0 + BN - 1) < a.max_distance;
-        const float far_bias = BIAS ? by_distance[a.max_distance] : 0.0f;
+        const bool near = BIAS && (far.apart || row0 - (j0 + BN - 1) < a.max_distance);
+        const float cc = BIAS && near ? 1.0f : c;
 #pragma unroll
         for (int b = 0; b < JB; ++b) {
-            f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+            f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
 #pragma unroll
             for (int k = 0; k < KS; ++k) s = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s);
 #pragma unroll
             for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(vt, 32 * b, k, lane), go[k], dp);
             const int j = j0 + 32 * b + 4 * half;
-            if (BIAS) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance, near, far_bias);
+            if (BIAS && near) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[r] = attn_exp2(BIAS ? s[r] - lse2 : __builtin_fmaf(s[r], c, -lse2));
+                s[r] = attn_exp2(__builtin_fmaf(s[r], cc, -lse2));
                 s[r] *= dp[r] - delta;
                 if (MASKED && (uint32_t)(j + (r & 3) + 8 * (r >> 2) - lower) > reach) s[r] = 0.0f;
                 if (BIAS) rest += s[r];
@@ -869,6 +880,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 }
 
 // ---- backward: gradients of the keys, the values and the bias table ----------------------------------------------------------
+__host__ __device__ inline int attn_corner(int max_distance) { return 16 * 33 + max_distance + 63; }      // floats of a wave
 // A block owns 128 keys of one key head and walks the queries of the heads of its group from there on: the sums over
 // shared heads are made in registers, in a fixed order.  Where that makes too few blocks for the chip, the heads and then
 // the queries are shared out among several blocks, whose sums a second kernel adds up, in a fixed order too.
@@ -881,8 +893,9 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     constexpr int PLACE = 2 * BYTES + ATTN_WAVES * 8 * BM;       // queries, gradients of the output, and a copy of their statistics for each wave
-    float* const corner = (float*)(lds + stages * PLACE) + wave * (32 * 33 + 64);   // (BIAS) a tile of dS of this wave, and the sums of its diagonals
-    float* const by_distance = (float*)(lds + stages * PLACE) + ATTN_WAVES * (32 * 33 + 64);
+    float* const by_distance = (float*)(lds + stages * PLACE);   // (BIAS)
+    // (its gradient) half a tile of dS of this wave, and its sums of dS for every distance
+    float* const corner = by_distance + a.max_distance + 1 + wave * attn_corner(a.max_distance), *const on_distance = corner + 16 * 33;
     const int kv_heads = a.heads / a.group, parts = a.head_parts * a.query_parts;
     int tile, kv;
     attn_place(blockIdx.x, tiles, kv_heads * parts, false, tile, kv);
@@ -935,7 +948,8 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     f32x16_t gk[DB], gv[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) { gk[d] = f32x16_t{}; gv[d] = f32x16_t{}; }
-    float in_bucket[ATTN_MAX_BUCKETS / WAVE] = {0.0f, 0.0f, 0.0f, 0.0f}, far_sum = 0.0f;    // of the head at hand
+    float far_sum = 0.0f;                          // of the head at hand, from max_distance on
+    AttnFar far(0.0f, 1.0f);
     auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_)::value;
         const char* const qt = lds + place * PLACE;
@@ -947,14 +961,15 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             terms = attn_look_over<E, ATTN_WAVES>(qt, 2 * BYTES, span, tid, lane);
             if (i0 >= own.hi || i0 + BM <= own.lo) return;
         }
-        f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+        const bool near = BIAS && (far.apart || i0 - (key0 + 31) < a.max_distance);
+        const float cc = BIAS && near ? 1.0f : c;
+        f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
 #pragma unroll
         for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, 0, x, lane), k[x], s);
 #pragma unroll
         for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, 0, x, lane), v[x], dp);
         const int i = i0 + 4 * half;
-        const bool near = BIAS && i0 - (key0 + 31) < a.max_distance;
-        if (BIAS) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance, near, by_distance[a.max_distance]);
+        if (BIAS && near) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4_t st01 = *(const f32x4_t*)(st + 16 * g + 8 * half), st23 = *(const f32x4_t*)(st + 16 * g + 8 * half + 4);
@@ -962,7 +977,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
                 const float ls = e < 2 ? st01[2 * e] : st23[2 * e - 4], de = e < 2 ? st01[2 * e + 1] : st23[2 * e - 3];
-                float p = attn_exp2(BIAS ? s[r] - ls : __builtin_fmaf(s[r], c, -ls));
+                float p = attn_exp2(__builtin_fmaf(s[r], cc, -ls));
                 float x = p * (dp[r] - de);
                 if (MASKED && (uint32_t)(i + e + 8 * g - key) >= reach) p = x = 0.0f;
                 s[r] = p;
@@ -979,34 +994,28 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             attn_add_product<E, DP>(qt, 0, dp, gk, lane);
         }
         if (BIAS && sums) {
-            if (!near) {
+            if (i0 - (key0 + 31) >= a.max_distance) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) far_sum += dp[r];
             } else {
-                // The tile of dS by diagonals (distance n = i - key has one value on each), then by buckets: lane b adds
-                // up what belongs to bucket b (+ 64 u).  Fixed order throughout.
-#pragma unroll
-                for (int r = 0; r < 16; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = there ? dp[r] : 0.0f;
-                __builtin_amdgcn_wave_barrier();
-                const int n0 = i0 - key0 - 31;                    // distance of diagonal 0
+                // The tile of dS by diagonals - a distance has one value on each - 16 rows at a time: lane t adds up the
+                // diagonal of distance i0 - key0 - 31 + t, and adds it to that distance's sum.  Fixed order throughout.
                 float on = 0.0f;
-                for (int col = 0; col < 32; ++col) {
-                    const int r = lane + col - 31;                // r - col = lane - 31
-                    if (r >= 0 && r < 32) on += corner[r * 33 + col];
-                }
-                corner[32 * 33 + lane] = lane < 63 ? on : 0.0f;
-                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
-                    const int b = lane + u * WAVE;
-                    if (u * WAVE < a.buckets && b < a.buckets) {
-                        const int from = b <= a.exact_to ? b : (int)a.borders[b - a.exact_to - 1];
-                        const int upto = b + 1 == a.buckets ? 1 << 30 : b + 1 <= a.exact_to ? b + 1 : (int)a.borders[b - a.exact_to];
-                        const int t0 = from - n0 > 0 ? from - n0 : 0, t1 = upto - n0 < 63 ? upto - n0 : 63;
-                        for (int t = t0; t < t1; ++t) in_bucket[u] += corner[32 * 33 + t];
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = there ? dp[8 * h + r] : 0.0f;
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int col = 16 * h + r + 31 - lane;
+                        const float x = corner[r * 33 + (col & 31)];
+                        on += col >= 0 && col < 32 ? x : 0.0f;
                     }
+                    __builtin_amdgcn_wave_barrier();
                 }
-                __builtin_amdgcn_wave_barrier();
+                const int n = i0 - key0 - 31 + lane;
+                if (n >= 0 && lane < 63) on_distance[n] += on;
             }
         }
     };
@@ -1014,17 +1023,21 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         if (BIAS) {
             __syncthreads();                        // the table of the head before is not read any more
             attn_bias_by_distance(a, head0 + g, by_distance, tid, ATTN_THREADS);
+            far = AttnFar(attn_bias(a, head0 + g, a.buckets - 1), c);
+            if (sums)
+                for (int n = lane; n < a.max_distance + 63; n += WAVE) on_distance[n] = 0.0f;
         }
         attn_run<2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1>(walk, from, upto, ring, fetch, step);
         if (BIAS && sums && from < upto) {
             far_sum = there ? far_sum : 0.0f;       // (a column without a key is masked in the tiles of the second loop only)
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) far_sum += __shfl_xor(far_sum, d, WAVE);
-#pragma unroll
-            for (int u = 0; u < ATTN_MAX_BUCKETS / WAVE; ++u) {
-                const int b = lane + u * WAVE;
-                if (b < a.buckets) sums[(int64_t)g * a.partial_tiles * a.buckets + b] = in_bucket[u] + (b + 1 == a.buckets ? far_sum : 0.0f);
-                in_bucket[u] = 0.0f;
+            for (int b = lane; b < a.buckets; b += WAVE) {       // a bucket's distances, in order
+                const int begins = b <= a.exact_to ? b : (int)a.borders[b - a.exact_to - 1];
+                const int ends = b + 1 == a.buckets ? a.max_distance + 63 : b + 1 <= a.exact_to ? b + 1 : (int)a.borders[b - a.exact_to];
+                float x = b + 1 == a.buckets ? far_sum : 0.0f;
+                for (int n = begins; n < ends; ++n) x += on_distance[n];
+                sums[(int64_t)g * a.partial_tiles * a.buckets + b] = x;
             }
             far_sum = 0.0f;
         }
@@ -1143,8 +1156,8 @@ inline bool attn_lds(const void* kernel, size_t bytes, uint64_t& asked) {
 
 // Places of a ring: as many as help (four) and fit beside `rest`, `blocks` sharing a CU's LDS, `rings` a block's.
 inline int attn_stages(size_t place, size_t rest, int rings, int blocks) {
-    const size_t n = (160 * 1024 / blocks - 512 - rest) / (place * rings);
-    return n >= 4 ? 4 : n >= 3 ? 3 : 2;
+    const int64_t room = 160 * 1024 / blocks - 512 - (int64_t)rest, n = room / (int64_t)(place * rings);
+    return n >= 4 ? 4 : n >= 3 ? 3 : n >= 2 || blocks == 1 ? 2 : attn_stages(place, rest, rings, 1);
 }
 template <int KG, class Kernel, class E>
 inline void attn_row_launch(Kernel* kernel, const AttnArgs<E>& a, int tiles, size_t place, size_t rest, uint64_t& asked, const char* what) {
@@ -1155,10 +1168,11 @@ inline void attn_row_launch(Kernel* kernel, const AttnArgs<E>& a, int tiles, siz
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_ROWS * 2 * KG), lds, stream(), a, tiles, stages);
     MXH_LAUNCH_CHECK(what);
 }
-// Up to two rounds of two blocks for every CU, the time is that of the longest walks: two groups of waves share each
-// (one block of 512 threads to a CU; f32 heads above 64 take too many registers for that).
+// Up to two blocks for every CU, the time is that of the longest walks: two groups of waves share each (one block of 512
+// threads to a CU).  Beyond, they are ahead no more: 4096 tokens in one sequence, 16 heads of 128 (512 blocks): 93 against 110 us
+// forward, 32 heads: 185 against 161 us.  f32 heads above 64 take too many registers for it.
 template <class E, int DP>
-inline bool attn_two_groups(const AttnArgs<E>& a, int tiles) { return !(sizeof(E) == 4 && DP > 64) && (int64_t)tiles * a.heads <= 1024; }
+inline bool attn_two_groups(const AttnArgs<E>& a, int tiles) { return !(sizeof(E) == 4 && DP > 64) && (int64_t)tiles * a.heads <= 512; }
 
 template <class E, int DP, bool BIAS>
 inline void attn_forward_launch(const AttnArgs<E>& a) {
@@ -1184,7 +1198,7 @@ inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
         if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias, asked_q[0], "attention_backward (queries)");
     }
     if (a.gk || a.gv || grad_table) {
-        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = (BIAS ? (size_t)ATTN_WAVES * (32 * 33 + 64) * 4 : 0) + bias;
+        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
         const int parts = a.head_parts * a.query_parts;
         const unsigned blocks = (unsigned)(tiles * kv * parts);
         const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && DP <= 64 && blocks > 256 ? 2 : 1);
