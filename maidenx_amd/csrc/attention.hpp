@@ -450,46 +450,36 @@ struct AttnWalk {
     __device__ int at(int n) const { return n < nclean ? clean + n * STEP : n < nclean + nfront ? begin + (n - nclean) * STEP : dirty + (n - nclean - nfront) * STEP; }
 };
 
-// The tiles of a walk pass through a ring of `stages` (2 to 4) places in LDS: stages - 1 of them are on their way while one is
-// worked on.  A wave has issued PER loads for each, which come back in order: it waits until only those of the later tiles are
-// out, then meets the others.
+// The tiles of a walk pass through a ring of `stages` (2 to 4) places in LDS: the place of a tile that is done with takes the next
+// one behind those on their way.  A wave has issued PER loads for each, which come back in order: it waits until only those of the
+// later tiles are out, then meets the others.
 struct AttnRing {
-    int stages, at = 0, to = 0, ahead = 0;
+    int stages, at = 0, to = 0, ahead = 0;         // ahead: fetched and not done with
     __device__ explicit AttnRing(int stages_) : stages(stages_) {}
     template <class Fetch>
     __device__ __forceinline__ void fill(Fetch&& fetch) {          // fetch(place): false when there is nothing left
-        while (ahead < stages - 1 && fetch(to)) {
+        while (ahead < stages && fetch(to)) {
             ++ahead;
             to = to + 1 == stages ? 0 : to + 1;
         }
     }
+    // the tile at `at` (or the `extra`-th after it) has come, and the one before it is done with by all waves
     template <int PER>
-    __device__ void arrived() const {
+    __device__ __forceinline__ void arrived(int extra = 0) const {
         static_assert(3 * PER < 64, "the counter has six bits");
-        if (ahead == 1) attn_wait<0>();
-        else if (ahead == 2) attn_wait<PER>();
-        else attn_wait<2 * PER>();
+        const int later = ahead - 1 - extra;
+        if (later <= 0) attn_wait<0>();
+        else if (later == 1) attn_wait<PER>();
+        else if (later == 2) attn_wait<2 * PER>();
+        else attn_wait<3 * PER>();
         __syncthreads();
     }
+    __device__ int after() const { return at + 1 == stages ? 0 : at + 1; }
     __device__ void done() {
         --ahead;
         at = at + 1 == stages ? 0 : at + 1;
     }
 };
-// the tiles [from, upto) of a walk: step(masked, tile, place)
-template <int PER, class Walk, class Fetch, class Step>
-__device__ __forceinline__ void attn_run(const Walk& walk, int from, int upto, AttnRing& ring, Fetch&& fetch, Step&& step) {
-    ring.fill(fetch);
-    auto turn = [&](auto masked, int n) __attribute__((always_inline)) {
-        ring.template arrived<PER>();
-        ring.fill(fetch);
-        step(masked, n, ring.at);
-        ring.done();
-    };
-    int n = from;
-    for (; n < upto && n < walk.nclean; ++n) turn(std::false_type{}, n);
-    for (; n < upto; ++n) turn(std::true_type{}, n);
-}
 // A walk in rounds: in each, KG groups of waves take a tile of their own (every KG-th), all clean or none.  A group that is left without one in the
 // last round fetches one that it does not need: every wave counts the same loads.
 template <class Walk, int KG>
@@ -888,7 +878,7 @@ template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH;
+    constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH, PER = 2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
@@ -950,26 +940,28 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     for (int d = 0; d < DB; ++d) { gk[d] = f32x16_t{}; gv[d] = f32x16_t{}; }
     float far_sum = 0.0f;                          // of the head at hand, from max_distance on
     AttnFar far(0.0f, 1.0f);
-    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_)::value;
-        const char* const qt = lds + place * PLACE;
-        const char* const ot = qt + BYTES;
-        const float* const st = (const float*)(qt + 2 * BYTES) + wave * 2 * BM;      // (lse2, D) of each row
-        const int i0 = walk.at(n);
-        bool terms = false;
-        if constexpr (MASKED) {
-            terms = attn_look_over<E, ATTN_WAVES>(qt, 2 * BYTES, span, tid, lane);
-            if (i0 >= own.hi || i0 + BM <= own.lo) return;
-        }
-        const bool near = BIAS && (far.apart || i0 - (key0 + 31) < a.max_distance);
-        const float cc = BIAS && near ? 1.0f : c;
-        f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
+    const auto is_near = [&](int i0) { return BIAS && (far.apart || i0 - (key0 + 31) < a.max_distance); };
+    const auto tile_of = [&](int place) { return lds + place * PLACE; };
+    // S and dP of a tile, rows in order
+    auto scores = [&](int n, int place, f32x16_t& s, f32x16_t& dp) __attribute__((always_inline)) {
+        s = attn_start(BIAS && !is_near(walk.at(n)) ? far.start : 0.0f);
+        dp = f32x16_t{};
+        const char* const qt = tile_of(place);
 #pragma unroll
         for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, 0, x, lane), k[x], s);
 #pragma unroll
-        for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, 0, x, lane), v[x], dp);
-        const int i = i0 + 4 * half;
-        if (BIAS && near) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance);
+        for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(qt + BYTES, 0, x, lane), v[x], dp);
+    };
+    auto bias = [&](int n, f32x16_t& s) __attribute__((always_inline)) {
+        const int i0 = walk.at(n);
+        if (is_near(i0)) attn_add_bias<-1>(s, c, by_distance, i0 + 4 * half - key, a.max_distance);
+    };
+    // ... become P and dS
+    auto weights = [&](auto masked_, int n, int place, f32x16_t& s, f32x16_t& dp) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        const float* const st = (const float*)(tile_of(place) + 2 * BYTES) + wave * 2 * BM;      // (lse2, D) of each row
+        const int i0 = walk.at(n), i = i0 + 4 * half;
+        const float cc = is_near(i0) ? 1.0f : c;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4_t st01 = *(const f32x4_t*)(st + 16 * g + 8 * half), st23 = *(const f32x4_t*)(st + 16 * g + 8 * half + 4);
@@ -984,40 +976,88 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
                 dp[r] = x;
             }
         }
-        if (MASKED && terms) {
+    };
+    auto by_bucket = [&](int n, const f32x16_t& dp) __attribute__((always_inline)) {
+        if (!BIAS || !sums) return;
+        const int i0 = walk.at(n);
+        if (i0 - (key0 + 31) >= a.max_distance) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) far_sum += dp[r];
+        } else {
+            // The tile of dS by diagonals - a distance has one value on each - 16 rows at a time: lane t adds up the
+            // diagonal of distance i0 - key0 - 31 + t, and adds it to that distance's sum.  Fixed order throughout.
+            float on = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = there ? dp[8 * h + r] : 0.0f;
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int col = 16 * h + r + 31 - lane;
+                    const float x = corner[r * 33 + (col & 31)];
+                    on += col >= 0 && col < 32 ? x : 0.0f;
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+            const int d = i0 - key0 - 31 + lane;
+            if (d >= 0 && lane < 63) on_distance[d] += on;
+        }
+    };
+    auto products = [&](int place, const f32x16_t& s, const f32x16_t& dp) __attribute__((always_inline)) {
+        attn_add_product<E, DP>(tile_of(place) + BYTES, 0, s, gv, lane);
+        attn_add_product<E, DP>(tile_of(place), 0, dp, gk, lane);
+    };
+    auto masked_step = [&](int n, int place) __attribute__((always_inline)) {
+        const char* const qt = tile_of(place);
+        const int i0 = walk.at(n);
+        const bool terms = attn_look_over<E, ATTN_WAVES>(qt, 2 * BYTES, span, tid, lane);
+        if (i0 >= own.hi || i0 + BM <= own.lo) return;
+        f32x16_t s, dp;
+        scores(n, place, s, dp);
+        bias(n, s);
+        weights(std::true_type{}, n, place, s, dp);
+        if (terms) {
             const f32x16_t pw[1] = {s}, xw[1] = {dp};
             const auto sees = [&](int r) { return (uint32_t)(i0 + r - key) < reach; };
-            attn_add_terms<E, DP, 1>(ot, pw, gv, lane, sees);
+            attn_add_terms<E, DP, 1>(qt + BYTES, pw, gv, lane, sees);
             attn_add_terms<E, DP, 1>(qt, xw, gk, lane, sees);
         } else {
-            attn_add_product<E, DP>(ot, 0, s, gv, lane);
-            attn_add_product<E, DP>(qt, 0, dp, gk, lane);
+            products(place, s, dp);
         }
-        if (BIAS && sums) {
-            if (i0 - (key0 + 31) >= a.max_distance) {
+        by_bucket(n, dp);
+    };
+    // The clean tiles [from, upto): while the vector unit makes the weights of one, the matrix cores are at the scores of the next.
+    auto clean_tiles = [&](int n, int until) __attribute__((always_inline)) {
+        if (n >= until) return;
+        f32x16_t s, dp;
+        ring.template arrived<PER>();
+        ring.fill(fetch);
+        scores(n, ring.at, s, dp);
+        for (; n + 1 < until; ++n) {
+            ring.template arrived<PER>(1);
+            ring.fill(fetch);
+            f32x16_t s1, dp1;
+            bias(n, s);
+            scores(n + 1, ring.after(), s1, dp1);
+            weights(std::false_type{}, n, ring.at, s, dp);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) far_sum += dp[r];
-            } else {
-                // The tile of dS by diagonals - a distance has one value on each - 16 rows at a time: lane t adds up the
-                // diagonal of distance i0 - key0 - 31 + t, and adds it to that distance's sum.  Fixed order throughout.
-                float on = 0.0f;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = there ? dp[8 * h + r] : 0.0f;
-                    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int col = 16 * h + r + 31 - lane;
-                        const float x = corner[r * 33 + (col & 31)];
-                        on += col >= 0 && col < 32 ? x : 0.0f;
-                    }
-                    __builtin_amdgcn_wave_barrier();
-                }
-                const int n = i0 - key0 - 31 + lane;
-                if (n >= 0 && lane < 63) on_distance[n] += on;
+            for (int x = 0; x < 2 * KS; ++x) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
+                __builtin_amdgcn_sched_group_barrier(0x002, 96 / (2 * KS), 0);      // the vector unit meanwhile
             }
+            products(ring.at, s, dp);
+            by_bucket(n, dp);
+            ring.done();
+            s = s1;
+            dp = dp1;
         }
+        bias(n, s);
+        weights(std::false_type{}, n, ring.at, s, dp);
+        products(ring.at, s, dp);
+        by_bucket(n, dp);
+        ring.done();
     };
     for (int g = 0; g < heads; ++g) {
         if (BIAS) {
@@ -1027,7 +1067,13 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             if (sums)
                 for (int n = lane; n < a.max_distance + 63; n += WAVE) on_distance[n] = 0.0f;
         }
-        attn_run<2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1>(walk, from, upto, ring, fetch, step);
+        clean_tiles(from, upto < walk.nclean ? upto : walk.nclean);
+        for (int n = from > walk.nclean ? from : walk.nclean; n < upto; ++n) {
+            ring.template arrived<PER>();
+            ring.fill(fetch);
+            masked_step(n, ring.at);
+            ring.done();
+        }
         if (BIAS && sums && from < upto) {
             far_sum = there ? far_sum : 0.0f;       // (a column without a key is masked in the tiles of the second loop only)
 #pragma unroll

@@ -23,6 +23,14 @@ def test_head_sizes(hip, dt, dim):
     Attention(dt, [90, 50], 2, 1, dim, seed=dim).check(hip)
 
 
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("heads,kv,buckets", [(2, 1, 0), (2, 2, 16), (90, 90, 0), (96, 8, 32)])
+def test_long_walks(hip, dt, dim, heads, kv, buckets):
+    """Many tiles to a block, with few blocks and with more than two for every CU (other numbers of waves and places)."""
+    Attention(dt, [790, 11], heads, kv, dim, buckets=buckets, distance=100 if buckets else 0, seed=dim + heads).check(hip)
+
+
 @pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (6, 2), (8, 8), (8, 1), (16, 4), (5, 5)])
 def test_grouped_heads(hip, heads, kv):
     Attention("bf16", [70, 150], heads, kv, 32, seed=heads).check(hip)
