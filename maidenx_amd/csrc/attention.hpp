@@ -131,39 +131,55 @@ struct AttnTile {
         else return (row >> 2) & 3;
     }
     __device__ static int at(int row, int piece) { return row * PITCH + ((piece ^ swizzle(row)) << 4); }
-    // rows row0 + (lane % 32), elements 16 step + 8 half ..
-    __device__ static Frag rows(const char* tile, int row0, int step, int lane) {
-        const int r = lane & 31, half = lane >> 5;
+    // Where the fragments of a tile lie, for a lane.  A swizzle is made of bits of the row, so what is known when the
+    // kernel is compiled (step, block, the row within 16) is an exclusive or and an offset to one register for each kind of
+    // fragment; the tiles lie on multiples of their pitch.
+    struct Lane {
+        uint32_t rows, columns;
+        __device__ explicit Lane(int lane) {
+            const int r = lane & 31, half = lane >> 5;
+            rows = at(r, sizeof(E) == 2 ? half : 2 * half);
+            if constexpr (sizeof(E) == 2) {
+                const int c = lane & 15;
+                columns = at(4 * half + (c >> 2), 2 * ((lane >> 4) & 1) + ((c & 3) >> 1)) + (c & 1) * 8;
+            } else {
+                columns = at(4 * half, (lane & 31) >> 2) + (lane & 3) * 4;
+            }
+        }
+    };
+    template <class V>
+    __device__ static V read(uint32_t from) { return *(__attribute__((address_space(3))) const V*)(uintptr_t)from; }
+    // rows row0 + (lane % 32), elements 16 step + 8 half ..  (row0: a multiple of 32; base: the tile in LDS)
+    __device__ static Frag rows(uint32_t base, const Lane& l, int row0, int step) {
+        const uint32_t at = base + l.rows;
         if constexpr (sizeof(E) == 2) {
-            return *(const Frag*)(tile + row0 * PITCH + at(r, 2 * step + half));
+            return read<Frag>((at ^ (step << 5)) + row0 * PITCH);
         } else {
-            const f32x4_t a = *(const f32x4_t*)(tile + row0 * PITCH + at(r, 4 * step + 2 * half));
-            const f32x4_t b = *(const f32x4_t*)(tile + row0 * PITCH + at(r, 4 * step + 2 * half + 1));
+            const f32x4_t a = read<f32x4_t>((at ^ (step << 6)) + row0 * PITCH), b = read<f32x4_t>((at ^ (step << 6 | 16)) + row0 * PITCH);
             return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
-    // column 32 block + (lane % 32), rows row0 + 4 half + (e % 4) + 8 (e / 4): the order in which a result holds its rows
-    __device__ static Frag columns(const char* tile, int row0, int block, int lane) {
-        const int half = lane >> 5;
+    // column 32 block + (lane % 32), rows row0 + 4 half + (e % 4) + 8 (e / 4): the order in which a result holds its rows (row0: a
+    // multiple of 16)
+    __device__ static Frag columns(uint32_t base, const Lane& l, int row0, int block) {
+        const uint32_t at = base + l.columns;
         if constexpr (sizeof(E) == 2) {
             // the hardware's transposed read: 16 lanes bring 4 rows x 16 columns, lane c gets column c
-            const int c = lane & 15, r = 4 * half + (c >> 2), piece = 4 * block + 2 * ((lane >> 4) & 1) + ((c & 3) >> 1);
-            s16x4_t lo, hi;
-            lo = read4(tile + row0 * PITCH + at(r, piece) + (c & 1) * 8);
-            hi = read4(tile + row0 * PITCH + at(r + 8, piece) + (c & 1) * 8);
+            const s16x4_t lo = read4((at ^ (block << 6)) + row0 * PITCH), hi = read4((at ^ (block << 6 | swizzle(8) << 4)) + (row0 + 8) * PITCH);
             return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const int col = 32 * block + (lane & 31);
             Frag f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = *(const float*)(tile + row0 * PITCH + at(4 * half + (e & 3) + 8 * (e >> 2), col >> 2) + (col & 3) * 4);
+            for (int e = 0; e < 8; ++e) {
+                const int r = (e & 3) + 8 * (e >> 2);
+                f[e] = read<float>((at ^ (block << 7 | swizzle(r) << 4)) + (row0 + r) * PITCH);
+            }
             return f;
         }
     }
-    __device__ static s16x4_t read4(const char* p) {
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p);
-    }
+    __device__ static s16x4_t read4(uint32_t from) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)from); }
 };
+__device__ inline uint32_t attn_in_lds(const void* p) { return (uint32_t)(uintptr_t)p; }      // the low half of an address in LDS
 
 // 16 bytes of a row from element d on, zeros beyond dim
 template <class E>
@@ -199,7 +215,7 @@ template <int BYTES>
 __device__ inline void attn_load_lds(const void* base, uint32_t off, const void* to) {
     const uint64_t at = (uint64_t)(uintptr_t)base;
     const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
-    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)to);      // (the low half of an address in LDS)
+    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane((int)attn_in_lds(to));
     if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
     else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
 }
@@ -224,7 +240,10 @@ struct AttnStage {
     // `inside`: every row of the tile is a token of [lo, hi); token0 is
     __device__ __forceinline__ void load(const AttnView<E>& view, int head, int token0, bool inside, int hi, int dim, char* tile, int wave, int lane) const {
         const E* const base = view.p + (int64_t)head * view.head + (int64_t)token0 * view.token;
-        if (view.vec) {
+        if (view.vec && inside && dim == DP && CALLS % GROUP == 0) {       // the usual case, without a look at the lanes
+#pragma unroll
+            for (int u = 0; u < N; ++u) attn_load_lds<16>(base, off[u], tile + (u * GROUP + wave) * 1024);
+        } else if (view.vec) {
 #pragma unroll
             for (int u = 0; u < N; ++u) {
                 uint32_t from = off[u];
@@ -421,7 +440,7 @@ __device__ inline void attn_add_terms(const char* tile, const f32x16_t (&weight)
 }
 // sums[d] += weight^T tile, the summed index in the rows of both
 template <class E, int DP>
-__device__ inline void attn_add_product(const char* tile, int row0, const f32x16_t& weight, f32x16_t (&sums)[DP / 32], int lane) {
+__device__ inline void attn_add_product(uint32_t tile, const typename AttnTile<E, DP>::Lane& l, int row0, const f32x16_t& weight, f32x16_t (&sums)[DP / 32]) {
     using T = AttnType<E>;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -430,7 +449,7 @@ __device__ inline void attn_add_product(const char* tile, int row0, const f32x16
         for (int e = 0; e < 8; ++e) p[e] = weight[8 * h + e];
         const typename T::Frag pf = T::pack(p);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) sums[d] = T::mma(AttnTile<E, DP>::columns(tile, row0 + 16 * h, d, lane), pf, sums[d]);
+        for (int d = 0; d < DP / 32; ++d) sums[d] = T::mma(AttnTile<E, DP>::columns(tile, l, row0 + 16 * h, d), pf, sums[d]);
     }
 }
 
@@ -463,18 +482,17 @@ struct AttnRing {
             to = to + 1 == stages ? 0 : to + 1;
         }
     }
-    // the tile at `at` (or the `extra`-th after it) has come, and the one before it is done with by all waves
+    // the tile at `at` has come, and the one before it is done with by all waves
     template <int PER>
-    __device__ __forceinline__ void arrived(int extra = 0) const {
+    __device__ __forceinline__ void arrived() const {
         static_assert(3 * PER < 64, "the counter has six bits");
-        const int later = ahead - 1 - extra;
+        const int later = ahead - 1;
         if (later <= 0) attn_wait<0>();
         else if (later == 1) attn_wait<PER>();
         else if (later == 2) attn_wait<2 * PER>();
         else attn_wait<3 * PER>();
         __syncthreads();
     }
-    __device__ int after() const { return at + 1 == stages ? 0 : at + 1; }
     __device__ void done() {
         --ahead;
         at = at + 1 == stages ? 0 : at + 1;
@@ -603,10 +621,11 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int RG = ATTN_ROWS / 32, BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[4 * RG * KG];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, group = __builtin_amdgcn_readfirstlane(tid / (64 * RG)), wave = __builtin_amdgcn_readfirstlane(tid / 64 % RG);
     char* const mine = lds + group * stages * 2 * BYTES;         // the group's ring
+    const typename L::Lane at(lane);
     int* const said = span + group * RG;
     float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
     attn_check_offsets(a);
@@ -669,7 +688,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
         for (int b = 0; b < JB; ++b) {
             s[b] = attn_start(BIAS && !near ? far.start : 0.0f);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) s[b] = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s[b]);
+            for (int k = 0; k < KS; ++k) s[b] = T::mma(L::rows(attn_in_lds(kt), at, 32 * b, k), q[k], s[b]);
         }
         const int j = j0 + 4 * half;                // key of row 0 of the lane's results
         if (BIAS && near) {
@@ -710,7 +729,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
             attn_add_terms<E, DP, JB>(vt, s, acc, lane, [&](int r) { return (uint32_t)(j0 + r - lower) <= reach; });
         } else {
 #pragma unroll
-            for (int b = 0; b < JB; ++b) attn_add_product<E, DP>(vt, 32 * b, s[b], acc, lane);
+            for (int b = 0; b < JB; ++b) attn_add_product<E, DP>(attn_in_lds(vt), at, 32 * b, s[b], acc);
         }
     };
     attn_run_rounds<2 * AttnStage<E, DP, BN, RG>::N>(rounds, ring, fetch, step);
@@ -745,10 +764,11 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int RG = ATTN_ROWS / 32, BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[4 * RG * KG];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, group = __builtin_amdgcn_readfirstlane(tid / (64 * RG)), wave = __builtin_amdgcn_readfirstlane(tid / 64 % RG);
     char* const mine = lds + group * stages * 2 * BYTES;         // the group's ring
+    const typename L::Lane at(lane);
     int* const said = span + group * RG;
     float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
     attn_check_offsets(a);
@@ -830,9 +850,9 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
         for (int b = 0; b < JB; ++b) {
             f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
 #pragma unroll
-            for (int k = 0; k < KS; ++k) s = T::mma(L::rows(kt, 32 * b, k, lane), q[k], s);
+            for (int k = 0; k < KS; ++k) s = T::mma(L::rows(attn_in_lds(kt), at, 32 * b, k), q[k], s);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(vt, 32 * b, k, lane), go[k], dp);
+            for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(attn_in_lds(vt), at, 32 * b, k), go[k], dp);
             const int j = j0 + 32 * b + 4 * half;
             if (BIAS && near) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance);
 #pragma unroll
@@ -846,7 +866,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
                 const f32x16_t w[1] = {s};
                 attn_add_terms<E, DP, 1>(kt + 32 * b * L::PITCH, w, acc, lane, [&](int r) { return (uint32_t)(j0 + 32 * b + r - lower) <= reach; });
             } else {
-                attn_add_product<E, DP>(kt, 32 * b, s, acc, lane);
+                attn_add_product<E, DP>(attn_in_lds(kt), at, 32 * b, s, acc);
             }
         }
     };
@@ -870,20 +890,27 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 }
 
 // ---- backward: gradients of the keys, the values and the bias table ----------------------------------------------------------
+// Two sums, keys and values of 32 rows of 128 elements take 192 registers of a wave, more than leaves room for a second wave on
+// its SIMD - and one wave alone cannot issue fast enough (4096 tokens, 32 heads of 128: 400 us): there the values stay in LDS.
+template <class E, int DP> constexpr bool attn_values_stay() { return sizeof(E) == 2 && DP > 64; }
 __host__ __device__ inline int attn_corner(int max_distance) { return 16 * 33 + max_distance + 63; }      // floats of a wave
 // A block owns 128 keys of one key head and walks the queries of the heads of its group from there on: the sums over
 // shared heads are made in registers, in a fixed order.  Where that makes too few blocks for the chip, the heads and then
 // the queries are shared out among several blocks, whose sums a second kernel adds up, in a fixed order too.
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
+__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH, PER = 2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     constexpr int PLACE = 2 * BYTES + ATTN_WAVES * 8 * BM;       // queries, gradients of the output, and a copy of their statistics for each wave
-    float* const by_distance = (float*)(lds + stages * PLACE);   // (BIAS)
+    constexpr bool STAY = attn_values_stay<E, DP>();             // the values of the block's keys are in LDS, too
+    char* const vtile = lds + stages * PLACE;
+    const uint32_t vrows = attn_in_lds(vtile + wave * 32 * L::PITCH);
+    const typename L::Lane at(lane);
+    float* const by_distance = (float*)(vtile + (STAY ? ATTN_ROWS * L::PITCH : 0));   // (BIAS)
     // (its gradient) half a tile of dS of this wave, and its sums of dS for every distance
     float* const corner = by_distance + a.max_distance + 1 + wave * attn_corner(a.max_distance), *const on_distance = corner + 16 * 33;
     const int kv_heads = a.heads / a.group, parts = a.head_parts * a.query_parts;
@@ -910,7 +937,13 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     os.begin(a.go, a.dim, wave, lane);
     if (a.dim < DP) {
         for (int p = 0; p < stages; ++p) attn_clear(lds + p * PLACE, 2 * BYTES, tid, ATTN_THREADS);
+        if (STAY) attn_clear(vtile, ATTN_ROWS * L::PITCH, tid, ATTN_THREADS);
         __syncthreads();
+    }
+    if constexpr (STAY) {                          // (waited for with the first tile, whose loads come later)
+        AttnStage<E, DP, ATTN_ROWS, ATTN_WAVES> vs;
+        vs.begin(a.v, a.dim, wave, lane);
+        vs.load(a.v, kv, tile * ATTN_ROWS, false, a.tokens, a.dim, vtile, wave, lane);
     }
     AttnRing ring(stages);
     int next_head = head0, next = from;
@@ -930,9 +963,9 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         return true;
     };
     ring.fill(fetch);
-    typename T::Frag k[KS], v[KS];
+    typename T::Frag k[KS], v[STAY ? 1 : KS];
     attn_own_rows<E, DP>(a.k, kv, there ? key : 0, there, a.dim, lane, attn_sign(a.scale), k);
-    attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
+    if constexpr (!STAY) attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
     const uint32_t reach = there ? (uint32_t)(last - key) : 0;       // query i sees the key if (unsigned)(i - key) < reach
     const float c = a.scale_log2;
     f32x16_t gk[DB], gv[DB];
@@ -946,11 +979,14 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     auto scores = [&](int n, int place, f32x16_t& s, f32x16_t& dp) __attribute__((always_inline)) {
         s = attn_start(BIAS && !is_near(walk.at(n)) ? far.start : 0.0f);
         dp = f32x16_t{};
-        const char* const qt = tile_of(place);
+        const uint32_t qt = attn_in_lds(tile_of(place));
 #pragma unroll
-        for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, 0, x, lane), k[x], s);
+        for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, at, 0, x), k[x], s);
 #pragma unroll
-        for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(qt + BYTES, 0, x, lane), v[x], dp);
+        for (int x = 0; x < KS; ++x) {
+            if constexpr (STAY) dp = T::mma(L::rows(qt + BYTES, at, 0, x), L::rows(vrows, at, 0, x), dp);
+            else dp = T::mma(L::rows(qt + BYTES, at, 0, x), v[x], dp);
+        }
     };
     auto bias = [&](int n, f32x16_t& s) __attribute__((always_inline)) {
         const int i0 = walk.at(n);
@@ -1005,8 +1041,8 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         }
     };
     auto products = [&](int place, const f32x16_t& s, const f32x16_t& dp) __attribute__((always_inline)) {
-        attn_add_product<E, DP>(tile_of(place) + BYTES, 0, s, gv, lane);
-        attn_add_product<E, DP>(tile_of(place), 0, dp, gk, lane);
+        attn_add_product<E, DP>(attn_in_lds(tile_of(place)) + BYTES, at, 0, s, gv);
+        attn_add_product<E, DP>(attn_in_lds(tile_of(place)), at, 0, dp, gk);
     };
     auto masked_step = [&](int n, int place) __attribute__((always_inline)) {
         const char* const qt = tile_of(place);
@@ -1027,37 +1063,13 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         }
         by_bucket(n, dp);
     };
-    // The clean tiles [from, upto): while the vector unit makes the weights of one, the matrix cores are at the scores of the next.
-    auto clean_tiles = [&](int n, int until) __attribute__((always_inline)) {
-        if (n >= until) return;
+    auto clean_step = [&](int n, int place) __attribute__((always_inline)) {
         f32x16_t s, dp;
-        ring.template arrived<PER>();
-        ring.fill(fetch);
-        scores(n, ring.at, s, dp);
-        for (; n + 1 < until; ++n) {
-            ring.template arrived<PER>(1);
-            ring.fill(fetch);
-            f32x16_t s1, dp1;
-            bias(n, s);
-            scores(n + 1, ring.after(), s1, dp1);
-            weights(std::false_type{}, n, ring.at, s, dp);
-#pragma unroll
-            for (int x = 0; x < 2 * KS; ++x) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
-                __builtin_amdgcn_sched_group_barrier(0x002, 96 / (2 * KS), 0);      // the vector unit meanwhile
-            }
-            products(ring.at, s, dp);
-            by_bucket(n, dp);
-            ring.done();
-            s = s1;
-            dp = dp1;
-        }
+        scores(n, place, s, dp);
         bias(n, s);
-        weights(std::false_type{}, n, ring.at, s, dp);
-        products(ring.at, s, dp);
+        weights(std::false_type{}, n, place, s, dp);
+        products(place, s, dp);
         by_bucket(n, dp);
-        ring.done();
     };
     for (int g = 0; g < heads; ++g) {
         if (BIAS) {
@@ -1067,8 +1079,14 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             if (sums)
                 for (int n = lane; n < a.max_distance + 63; n += WAVE) on_distance[n] = 0.0f;
         }
-        clean_tiles(from, upto < walk.nclean ? upto : walk.nclean);
-        for (int n = from > walk.nclean ? from : walk.nclean; n < upto; ++n) {
+        int n = from;
+        for (; n < upto && n < walk.nclean; ++n) {
+            ring.template arrived<PER>();
+            ring.fill(fetch);
+            clean_step(n, ring.at);
+            ring.done();
+        }
+        for (; n < upto; ++n) {
             ring.template arrived<PER>();
             ring.fill(fetch);
             masked_step(n, ring.at);
@@ -1244,10 +1262,10 @@ inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
         if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias, asked_q[0], "attention_backward (queries)");
     }
     if (a.gk || a.gv || grad_table) {
-        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
+        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = (attn_values_stay<E, DP>() ? attn_tile_bytes<E, DP>(ATTN_ROWS) : 0) + bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
         const int parts = a.head_parts * a.query_parts;
         const unsigned blocks = (unsigned)(tiles * kv * parts);
-        const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && DP <= 64 && blocks > 256 ? 2 : 1);
+        const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && blocks > 256 ? 2 : 1);
         auto* kernel = attn_grad_key_kernel<E, DP, BIAS>;
         if (!attn_lds((const void*)kernel, stages * place + rest, asked_k)) return;
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + rest, stream(), a, tiles, stages);
