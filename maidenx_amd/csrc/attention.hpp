@@ -165,14 +165,14 @@ struct AttnTile {
         const uint32_t at = base + l.columns;
         if constexpr (sizeof(E) == 2) {
             // the hardware's transposed read: 16 lanes bring 4 rows x 16 columns, lane c gets column c
-            const s16x4_t lo = read4((at ^ (block << 6)) + row0 * PITCH), hi = read4((at ^ (block << 6 | swizzle(8) << 4)) + (row0 + 8) * PITCH);
+            const s16x4_t lo = read4((at ^ (block << 6)) + row0 * PITCH), hi = read4((at ^ (block << 6 ^ swizzle(8) << 4)) + (row0 + 8) * PITCH);
             return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             Frag f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int r = (e & 3) + 8 * (e >> 2);
-                f[e] = read<float>((at ^ (block << 7 | swizzle(r) << 4)) + (row0 + r) * PITCH);
+                f[e] = read<float>((at ^ (block << 7 ^ swizzle(r) << 4)) + (row0 + r) * PITCH);
             }
             return f;
         }
@@ -209,49 +209,62 @@ __device__ inline u32x4_t attn_piece(const E* row, int d, int dim, int64_t elem,
 template <int N>
 __device__ inline void attn_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
+// the lane's number, found where it is asked for
+__device__ inline int attn_lane() {
+    int lane;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+    return lane;
+}
 // BYTES (4 or 16) of every lane, from base + off to 64 * BYTES of LDS in a row.  (m0, the place in LDS, is read as the load is
 // issued; nothing else in these kernels uses it.)
 template <int BYTES>
-__device__ inline void attn_load_lds(const void* base, uint32_t off, const void* to) {
+__device__ __forceinline__ void attn_load_lds(const void* base, uint32_t off, uint32_t to) {
     const uint64_t at = (uint64_t)(uintptr_t)base;
     const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
-    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane((int)attn_in_lds(to));
+    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane((int)to);
     if constexpr (BYTES == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
     else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
 }
 
-// GROUP waves move the tiles of their own ring; `wave` is a wave's number among them.
-template <class E, int DP, int ROWS, int GROUP>
+// GROUP waves move the tiles of their own ring; `wave` is a wave's number among them.  KEEP: a lane's offset stays in a register.
+template <class E, int DP, int ROWS, int GROUP, bool KEEP = true>
 struct AttnStage {
     using L = AttnTile<E, DP>;
     static constexpr int CALLS = ROWS * L::PITCH / 1024;       // wave instructions for a tile
     static constexpr int N = (CALLS + GROUP - 1) / GROUP;      // of a wave: that many, or (a small tile) none
     static_assert(CALLS % GROUP == 0 || CALLS < GROUP, "what a wave waits for is counted");
-    uint32_t off[N];                                           // bytes from the tile's first token to the lane's piece
-    bool on[N];
-    __device__ void begin(const AttnView<E>& view, int dim, int wave, int lane) {
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int slot = (u * GROUP + wave) * 64 + lane, row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row);
-            off[u] = (uint32_t)(row * (int)view.token + piece * L::T::CHUNK) * (uint32_t)sizeof(E);
-            on[u] = piece * L::T::CHUNK < dim && row < ROWS;
-        }
+    // A wave's instructions bring rows that are STRIDE apart: where the swizzle is the same for them, one offset serves all, and
+    // the rest is in the base.
+    static constexpr int STRIDE = GROUP * 64 / L::PIECES;
+    static constexpr bool ALIKE = STRIDE % 16 == 0;
+    __device__ static int row_of(int u, int wave, int lane) { return ((u * GROUP + wave) * 64 + lane) / L::PIECES; }
+    __device__ static int piece_of(int u, int wave, int lane) { return (lane % L::PIECES) ^ L::swizzle(row_of(u, wave, lane)); }
+    // bytes from the tile's first token to the lane's piece
+    __device__ static uint32_t offset(const AttnView<E>& view, int u, int wave, int lane) {
+        return ((uint32_t)row_of(u, wave, lane) * (uint32_t)view.token + piece_of(u, wave, lane) * L::T::CHUNK) * (uint32_t)sizeof(E);
     }
-    // `inside`: every row of the tile is a token of [lo, hi); token0 is
-    __device__ __forceinline__ void load(const AttnView<E>& view, int head, int token0, bool inside, int hi, int dim, char* tile, int wave, int lane) const {
-        const E* const base = view.p + (int64_t)head * view.head + (int64_t)token0 * view.token;
-        if (view.vec && inside && dim == DP && CALLS % GROUP == 0) {       // the usual case, without a look at the lanes
+    // whether every lane brings a piece of every tile that lies within the walk: then a tile's loads are plain() ones
+    __device__ static bool plainly(const AttnView<E>& view, int dim) { return view.vec && dim == DP && CALLS % GROUP == 0; }
+    uint32_t kept;
+    __device__ __forceinline__ AttnStage(const AttnView<E>& view, int wave, int lane) : kept(offset(view, 0, wave, lane)) {}
+    // (Without KEEP the offset is made anew each time: where registers are short it is the first thing that the compiler puts in
+    // memory, and a load from there waits for every tile on its way.)
+    __device__ __forceinline__ void plain(const AttnView<E>& view, const E* base, uint32_t tile, int wave) const {
+        const int lane = attn_lane();
+        const uint32_t first = KEEP ? kept : offset(view, 0, wave, lane);
 #pragma unroll
-            for (int u = 0; u < N; ++u) attn_load_lds<16>(base, off[u], tile + (u * GROUP + wave) * 1024);
-        } else if (view.vec) {
+        for (int u = 0; u < N; ++u)
+            attn_load_lds<16>(ALIKE ? base + u * STRIDE * view.token : base, ALIKE ? first : offset(view, u, wave, lane), tile + (u * GROUP + wave) * 1024);
+    }
+    // any tile that begins at a token before hi
+    __device__ static __forceinline__ void load(const AttnView<E>& view, int head, int token0, int hi, int dim, char* tile, int wave, int lane) {
+        const E* const base = view.p + (int64_t)head * view.head + (int64_t)token0 * view.token;
+        if (view.vec) {
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-                uint32_t from = off[u];
-                if (!inside) {                 // (a row before the last one of the tile's: 32 bits, as for the others)
-                    const int row = ((u * GROUP + wave) * 64 + lane) / L::PIECES, beyond = token0 + row - (hi - 1);
-                    from -= beyond > 0 ? (uint32_t)beyond * (uint32_t)view.token * (uint32_t)sizeof(E) : 0u;
-                }
-                if (on[u]) attn_load_lds<16>(base, from, tile + (u * GROUP + wave) * 1024);
+                const int row = row_of(u, wave, lane), piece = piece_of(u, wave, lane), in = token0 + row < hi ? row : hi - 1 - token0;
+                const uint32_t from = (uint32_t)(in * (int)view.token + piece * L::T::CHUNK) * (uint32_t)sizeof(E);
+                if (piece * L::T::CHUNK < dim && row < ROWS) attn_load_lds<16>(base, from, attn_in_lds(tile) + (u * GROUP + wave) * 1024);
             }
         } else {
 #pragma nounroll
@@ -289,7 +302,7 @@ __device__ inline void attn_own_rows(const AttnView<E>& view, int head, int toke
 // ---- sequences -----------------------------------------------------------------------------------------------------------
 // First token of the sequence of `row` and the first token behind it; false if no sequence holds the row.  Offsets that
 // do not ascend give some bounds with first <= row < last <= tokens: never an access outside the tensors.
-__device__ inline bool attn_sequence(const int32_t* offsets, int sequences, int tokens, int row, int lane, int& first, int& last) {
+__device__ __forceinline__ bool attn_sequence(const int32_t* offsets, int sequences, int tokens, int row, int lane, int& first, int& last) {
     int lo = -1, hi = tokens;
     bool above = false;
     if (sequences < WAVE) {
@@ -358,7 +371,7 @@ __device__ inline void attn_bias_by_distance(const AttnArgs<E>& a, int head, flo
 struct AttnFar {
     float start;
     bool apart;
-    __device__ AttnFar(float bias, float c) : start(bias / c), apart(!(__builtin_fabsf(bias) < 1e30f * c) && bias != -INFINITY) {}
+    __device__ __forceinline__ AttnFar(float bias, float c) : start(bias / c), apart(!(__builtin_fabsf(bias) < 1e30f * c) && bias != -INFINITY) {}
 };
 // The scores, in units of log2, that a lane holds at distances d0 - (r % 4) - 8 (r / 4), times STEP (1: rows are keys, -1: queries)
 template <int STEP>
@@ -399,7 +412,7 @@ __device__ inline bool attn_finite(u32x4_t x) {
 // by the GROUP waves of a ring (tid among their threads), the tile being there: whether it holds such a value.  All waves of the block
 // come along.
 template <class E, int GROUP>
-__device__ inline bool attn_look_over(const char* tile, int bytes, int* said, int tid, int lane) {
+__device__ __forceinline__ bool attn_look_over(const char* tile, int bytes, int* said, int tid, int lane) {
     bool fine = true;
     for (int at = tid * 16; at < bytes; at += GROUP * 64 * 16) fine &= attn_finite<E>(*(const u32x4_t*)(tile + at));
     const bool any = __any(!fine);
@@ -411,7 +424,7 @@ __device__ inline bool attn_look_over(const char* tile, int bytes, int* said, in
     return __builtin_amdgcn_readfirstlane(bad) != 0;
 }
 template <class E, int DP, int TILES, class Sees>
-__device__ inline void attn_add_terms(const char* tile, const f32x16_t (&weight)[TILES], f32x16_t (&sums)[DP / 32], int lane, Sees sees) {
+__device__ __forceinline__ void attn_add_terms(const char* tile, const f32x16_t (&weight)[TILES], f32x16_t (&sums)[DP / 32], int lane, Sees sees) {
     using L = AttnTile<E, DP>;
     const int half = lane >> 5;
 #pragma nounroll
@@ -440,7 +453,7 @@ __device__ inline void attn_add_terms(const char* tile, const f32x16_t (&weight)
 }
 // sums[d] += weight^T tile, the summed index in the rows of both
 template <class E, int DP>
-__device__ inline void attn_add_product(uint32_t tile, const typename AttnTile<E, DP>::Lane& l, int row0, const f32x16_t& weight, f32x16_t (&sums)[DP / 32]) {
+__device__ __forceinline__ void attn_add_product(uint32_t tile, const typename AttnTile<E, DP>::Lane& l, int row0, const f32x16_t& weight, f32x16_t (&sums)[DP / 32]) {
     using T = AttnType<E>;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -458,7 +471,7 @@ __device__ inline void attn_add_product(uint32_t tile, const typename AttnTile<E
 template <int STEP>
 struct AttnWalk {
     int begin, clean, dirty, nclean, nfront, total;
-    __device__ AttnWalk(int begin_, int end, int from, int upto) : begin(begin_) {
+    __device__ __forceinline__ AttnWalk(int begin_, int end, int from, int upto) : begin(begin_) {
         clean = from > begin ? begin + (from - begin + STEP - 1) / STEP * STEP : begin;
         nclean = upto > clean ? (upto - clean) / STEP : 0;
         if (nclean == 0) clean = begin;
@@ -466,31 +479,43 @@ struct AttnWalk {
         nfront = (clean - begin) / STEP;
         total = nclean + nfront + (end > dirty ? (end - dirty + STEP - 1) / STEP : 0);
     }
-    __device__ int at(int n) const { return n < nclean ? clean + n * STEP : n < nclean + nfront ? begin + (n - nclean) * STEP : dirty + (n - nclean - nfront) * STEP; }
+    // (sums of selected values: a choice between members would keep the whole struct in memory)
+    __device__ __forceinline__ int at(int n) const {
+        return clean + n * STEP + (n >= nclean ? begin - dirty : 0) + (n >= nclean + nfront ? dirty - clean : 0);
+    }
 };
 
 // The tiles of a walk pass through a ring of `stages` (2 to 4) places in LDS: the place of a tile that is done with takes the next
 // one behind those on their way.  A wave has issued PER loads for each, which come back in order: it waits until only those of the
 // later tiles are out, then meets the others.
 struct AttnRing {
-    int stages, at = 0, to = 0, ahead = 0;         // ahead: fetched and not done with
+    int stages, at = 0, to = 0, ahead = 0, left = 0;         // ahead: fetched and not done with; left: not fetched
     __device__ explicit AttnRing(int stages_) : stages(stages_) {}
     template <class Fetch>
-    __device__ __forceinline__ void fill(Fetch&& fetch) {          // fetch(place): false when there is nothing left
-        while (ahead < stages && fetch(to)) {
-            ++ahead;
-            to = to + 1 == stages ? 0 : to + 1;
-        }
+    __device__ __forceinline__ void begin(int total, Fetch&& fetch) {          // fetch(place)
+        left = total;
+        while (ahead < stages && left > 0) put(fetch);
+    }
+    template <class Fetch>
+    __device__ __forceinline__ void put(Fetch&& fetch) {
+        fetch(to);
+        --left;
+        ++ahead;
+        to = to + 1 == stages ? 0 : to + 1;
+    }
+    template <class Fetch>
+    __device__ __forceinline__ void refill(Fetch&& fetch) {        // the place of the tile before
+        if (left > 0 && ahead < stages) put(fetch);
     }
     // the tile at `at` has come, and the one before it is done with by all waves
     template <int PER>
     __device__ __forceinline__ void arrived() const {
         static_assert(3 * PER < 64, "the counter has six bits");
         const int later = ahead - 1;
-        if (later <= 0) attn_wait<0>();
-        else if (later == 1) attn_wait<PER>();
+        if (later >= 3) attn_wait<3 * PER>();
         else if (later == 2) attn_wait<2 * PER>();
-        else attn_wait<3 * PER>();
+        else if (later == 1) attn_wait<PER>();
+        else attn_wait<0>();
         __syncthreads();
     }
     __device__ void done() {
@@ -504,11 +529,11 @@ template <class Walk, int KG>
 struct AttnRounds {
     const Walk& walk;
     int group, clean, total;
-    __device__ AttnRounds(const Walk& walk_, int group_)
+    __device__ __forceinline__ AttnRounds(const Walk& walk_, int group_)
         : walk(walk_), group(group_), clean((walk_.nclean + KG - 1) / KG), total(clean + (walk_.total - walk_.nclean + KG - 1) / KG) {}
-    __device__ int tile(int round) const { return round < clean ? round * KG + group : walk.nclean + (round - clean) * KG + group; }
-    __device__ int nearest(int round) const {
-        const int n = tile(round), last = (round < clean ? walk.nclean : walk.total) - 1;
+    __device__ __forceinline__ int tile(int round) const { return round * KG + group + (round >= clean ? walk.nclean - clean * KG : 0); }
+    __device__ __forceinline__ int nearest(int round) const {
+        const int n = tile(round), last = walk.nclean - 1 + (round >= clean ? walk.total - walk.nclean : 0);
         return n < last ? n : last;
     }
 };
@@ -516,7 +541,7 @@ template <int PER, class Rounds, class Fetch, class Step>
 __device__ __forceinline__ void attn_run_rounds(const Rounds& rounds, AttnRing& ring, Fetch&& fetch, Step&& step) {
     auto turn = [&](auto masked, int round) __attribute__((always_inline)) {
         ring.template arrived<PER>();
-        ring.fill(fetch);
+        ring.refill(fetch);
         step(masked, round, ring.at);
         ring.done();
     };
@@ -529,7 +554,7 @@ __device__ __forceinline__ void attn_run_rounds(const Rounds& rounds, AttnRing& 
 // every row sees.  Rows see keys [first, row], keys are seen by queries [key, last): both ends ascend from row to row.
 struct AttnSpan {
     int lo, hi, inner, top;
-    __device__ AttnSpan(bool there, int from, int upto) {         // what a lane's row sees
+    __device__ __forceinline__ AttnSpan(bool there, int from, int upto) {         // what a lane's row sees
         const uint32_t rows = (uint32_t)__ballot(there);           // (the halves of a wave say the same)
         if (rows == 0) { lo = inner = 0; hi = 0; top = 0x7fffffff; return; }
         const int a = __builtin_ctz(rows), b = 31 - __builtin_clz(rows);
@@ -539,7 +564,7 @@ struct AttnSpan {
         hi = __builtin_amdgcn_readlane(upto, b);
     }
     template <int WAVES>                                           // of the rows of WAVES waves
-    __device__ AttnSpan of_block(int* shared, int wave, int lane) const {
+    __device__ __forceinline__ AttnSpan of_block(int* shared, int wave, int lane) const {
         if (lane == 0) { shared[4 * wave] = hi > lo ? lo : 0x7fffffff; shared[4 * wave + 1] = hi; shared[4 * wave + 2] = inner; shared[4 * wave + 3] = top; }
         __syncthreads();
         AttnSpan all = *this;
@@ -637,9 +662,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
     const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
     if (all.hi <= all.lo) return;                   // no row of the block is in a sequence
-    AttnStage<E, DP, BN, RG> ks, vs;
-    ks.begin(a.k, a.dim, wave, lane);
-    vs.begin(a.v, a.dim, wave, lane);
+    const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
     const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
     const AttnRounds<AttnWalk<BN>, KG> rounds(walk, group);
     if (a.dim < DP) {
@@ -647,17 +670,26 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
         __syncthreads();
     }
     AttnRing ring(stages);
+    // the next round's tiles: while they are clean ones, a group's follow one another at a fixed distance
+    const int plain = ks.plainly(a.k, a.dim) && vs.plainly(a.v, a.dim) ? walk.nclean / KG : 0;
+    const int64_t to_next_k = (int64_t)(KG * BN) * a.k.token, to_next_v = (int64_t)(KG * BN) * a.v.token;
+    const E *next_k = a.k.p + (int64_t)kv * a.k.head + (int64_t)walk.at(group) * a.k.token, *next_v = a.v.p + (int64_t)kv * a.v.head + (int64_t)walk.at(group) * a.v.token;
     int next = 0;
     auto fetch = [&](int place) __attribute__((always_inline)) {
-        if (next == rounds.total) return false;
         char* const to = mine + place * 2 * BYTES;
-        const int j0 = walk.at(rounds.nearest(next));
-        const bool inside = next++ < rounds.clean;
-        ks.load(a.k, kv, j0, inside, all.hi, a.dim, to, wave, lane);
-        vs.load(a.v, kv, j0, inside, all.hi, a.dim, to + BYTES, wave, lane);
-        return true;
+        if (next < plain) {
+            ks.plain(a.k, next_k, attn_in_lds(to), wave);
+            vs.plain(a.v, next_v, attn_in_lds(to) + BYTES, wave);
+            next_k += to_next_k;
+            next_v += to_next_v;
+        } else {
+            const int j0 = walk.at(rounds.nearest(next));
+            ks.load(a.k, kv, j0, all.hi, a.dim, to, wave, lane);
+            vs.load(a.v, kv, j0, all.hi, a.dim, to + BYTES, wave, lane);
+        }
+        ++next;
     };
-    ring.fill(fetch);
+    ring.begin(rounds.total, fetch);
     typename T::Frag q[KS];
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
@@ -726,7 +758,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
                 l += s[b][r];
             }
         if (MASKED && terms) {
-            attn_add_terms<E, DP, JB>(vt, s, acc, lane, [&](int r) { return (uint32_t)(j0 + r - lower) <= reach; });
+            attn_add_terms<E, DP, JB>(vt, s, acc, lane, [&](int r) __attribute__((always_inline)) { return (uint32_t)(j0 + r - lower) <= reach; });
         } else {
 #pragma unroll
             for (int b = 0; b < JB; ++b) attn_add_product<E, DP>(attn_in_lds(vt), at, 32 * b, s[b], acc);
@@ -759,6 +791,11 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 // A block owns 128 queries like the forward kernel.  Writes dq (if wanted) and, for the kernel of the keys, lse and D_i: with a
 // bias the one that makes the row of dS sum to zero (formed from P and dP themselves; the rounding of o in do . o
 // would otherwise enter every pair of the far bucket with the same sign).
+// The sum, the rows of q and those of do take all registers of a wave of two on a SIMD at 128 elements a head: some fragments of do
+// are read from LDS (a register more than there are is read from memory, behind every tile on its way).  Three leave room for two
+// blocks on a CU and are enough: 8192 tokens, 16 heads: 209 us; two 274, four 335 (one block).  With a bias they are not (369 us), and
+// five with one block on a CU take 305 us.  (Two groups of waves have room for one next to the longest table of a bias.)
+template <class E, int DP, bool BIAS, int KG> constexpr int attn_fragments_out() { return sizeof(E) == 2 && DP > 96 ? !BIAS ? 3 : KG == 1 ? 5 : 1 : 0; }
 template <class E, int DP, bool BIAS, int KG>
 __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
@@ -770,7 +807,9 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     char* const mine = lds + group * stages * 2 * BYTES;         // the group's ring
     const typename L::Lane at(lane);
     int* const said = span + group * RG;
-    float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
+    constexpr int OUT = attn_fragments_out<E, DP, BIAS, KG>(), IN = KS - OUT;
+    char* const out = lds + KG * stages * 2 * BYTES + ((group * RG + wave) * OUT * 64 + lane) * 16;      // the lane's last OUT fragments of do
+    float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES + KG * RG * OUT * 1024);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -780,9 +819,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
     const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
     if (all.hi <= all.lo) return;
-    AttnStage<E, DP, BN, RG> ks, vs;
-    ks.begin(a.k, a.dim, wave, lane);
-    vs.begin(a.v, a.dim, wave, lane);
+    const AttnStage<E, DP, BN, RG, attn_fragments_out<E, DP, BIAS, KG>() == 0> ks(a.k, wave, lane), vs(a.v, wave, lane);
     const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
     const AttnRounds<AttnWalk<BN>, KG> rounds(walk, group);
     if (a.dim < DP) {
@@ -790,18 +827,27 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
         __syncthreads();
     }
     AttnRing ring(stages);
+    // the next round's tiles: while they are clean ones, a group's follow one another at a fixed distance
+    const int plain = ks.plainly(a.k, a.dim) && vs.plainly(a.v, a.dim) ? walk.nclean / KG : 0;
+    const int64_t to_next_k = (int64_t)(KG * BN) * a.k.token, to_next_v = (int64_t)(KG * BN) * a.v.token;
+    const E *next_k = a.k.p + (int64_t)kv * a.k.head + (int64_t)walk.at(group) * a.k.token, *next_v = a.v.p + (int64_t)kv * a.v.head + (int64_t)walk.at(group) * a.v.token;
     int next = 0;
     auto fetch = [&](int place) __attribute__((always_inline)) {
-        if (next == rounds.total) return false;
         char* const to = mine + place * 2 * BYTES;
-        const int j0 = walk.at(rounds.nearest(next));
-        const bool inside = next++ < rounds.clean;
-        ks.load(a.k, kv, j0, inside, all.hi, a.dim, to, wave, lane);
-        vs.load(a.v, kv, j0, inside, all.hi, a.dim, to + BYTES, wave, lane);
-        return true;
+        if (next < plain) {
+            ks.plain(a.k, next_k, attn_in_lds(to), wave);
+            vs.plain(a.v, next_v, attn_in_lds(to) + BYTES, wave);
+            next_k += to_next_k;
+            next_v += to_next_v;
+        } else {
+            const int j0 = walk.at(rounds.nearest(next));
+            ks.load(a.k, kv, j0, all.hi, a.dim, to, wave, lane);
+            vs.load(a.v, kv, j0, all.hi, a.dim, to + BYTES, wave, lane);
+        }
+        ++next;
     };
     const bool walks = a.gq || (BIAS && (a.gk || a.partial));       // else only D_i is wanted, if that
-    if (walks) ring.fill(fetch);
+    if (walks) ring.begin(rounds.total, fetch);
     typename T::Frag q[KS], go[KS];
     attn_own_rows<E, DP>(a.go, head, there ? row : 0, there, a.dim, lane, 1.0f, go);
     float delta = 0.0f, lse2 = INFINITY;
@@ -823,6 +869,10 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
         return;
     }
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
+    if constexpr (OUT > 0) {                       // (a wave's own: no barrier)
+#pragma unroll
+        for (int k = IN; k < KS; ++k) *(typename T::Frag*)(out + (k - IN) * 1024) = go[k];
+    }
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
     const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_log2);
     const int lower = there ? first : -1;
@@ -852,7 +902,12 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 #pragma unroll
             for (int k = 0; k < KS; ++k) s = T::mma(L::rows(attn_in_lds(kt), at, 32 * b, k), q[k], s);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(attn_in_lds(vt), at, 32 * b, k), go[k], dp);
+            for (int k = 0; k < KS; ++k) {
+                typename T::Frag g;
+                if constexpr (OUT > 0) { if (k >= IN) g = *(const typename T::Frag*)(out + (k - IN) * 1024); else g = go[k]; }
+                else g = go[k];
+                dp = T::mma(L::rows(attn_in_lds(vt), at, 32 * b, k), g, dp);
+            }
             const int j = j0 + 32 * b + 4 * half;
             if (BIAS && near) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance);
 #pragma unroll
@@ -864,7 +919,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
             }
             if (MASKED && terms) {
                 const f32x16_t w[1] = {s};
-                attn_add_terms<E, DP, 1>(kt + 32 * b * L::PITCH, w, acc, lane, [&](int r) { return (uint32_t)(j0 + 32 * b + r - lower) <= reach; });
+                attn_add_terms<E, DP, 1>(kt + 32 * b * L::PITCH, w, acc, lane, [&](int r) __attribute__((always_inline)) { return (uint32_t)(j0 + 32 * b + r - lower) <= reach; });
             } else {
                 attn_add_product<E, DP>(attn_in_lds(kt), at, 32 * b, s, acc);
             }
@@ -890,27 +945,26 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 }
 
 // ---- backward: gradients of the keys, the values and the bias table ----------------------------------------------------------
-// Two sums, keys and values of 32 rows of 128 elements take 192 registers of a wave, more than leaves room for a second wave on
-// its SIMD - and one wave alone cannot issue fast enough (4096 tokens, 32 heads of 128: 400 us): there the values stay in LDS.
-template <class E, int DP> constexpr bool attn_values_stay() { return sizeof(E) == 2 && DP > 64; }
-__host__ __device__ inline int attn_corner(int max_distance) { return 16 * 33 + max_distance + 63; }      // floats of a wave
 // A block owns 128 keys of one key head and walks the queries of the heads of its group from there on: the sums over
 // shared heads are made in registers, in a fixed order.  Where that makes too few blocks for the chip, the heads and then
 // the queries are shared out among several blocks, whose sums a second kernel adds up, in a fixed order too.
+//
+// Both sums, the keys and the values of 32 rows of 128 elements take 192 registers of a wave and leave no room for a second wave on
+// its SIMD above 64 elements a head (16 bits): one wave there is limited by what it can issue (8192 tokens, 16 heads of 128:
+// 413 us).  Two waves that share the work, one for each sum and both making P, take 406, and more for the bias; the
+// values in LDS, 475.
+__host__ __device__ inline int attn_corner(int max_distance) { return 16 * 33 + max_distance + 63; }      // floats of a wave
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
+__global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH, PER = 2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1;
+    constexpr int PLACE = 2 * BYTES + ATTN_WAVES * 8 * BM;       // queries, gradients of the output, and a copy of their statistics for each wave
     extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
-    constexpr int PLACE = 2 * BYTES + ATTN_WAVES * 8 * BM;       // queries, gradients of the output, and a copy of their statistics for each wave
-    constexpr bool STAY = attn_values_stay<E, DP>();             // the values of the block's keys are in LDS, too
-    char* const vtile = lds + stages * PLACE;
-    const uint32_t vrows = attn_in_lds(vtile + wave * 32 * L::PITCH);
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const typename L::Lane at(lane);
-    float* const by_distance = (float*)(vtile + (STAY ? ATTN_ROWS * L::PITCH : 0));   // (BIAS)
+    float* const by_distance = (float*)(lds + stages * PLACE);   // (BIAS)
     // (its gradient) half a tile of dS of this wave, and its sums of dS for every distance
     float* const corner = by_distance + a.max_distance + 1 + wave * attn_corner(a.max_distance), *const on_distance = corner + 16 * 33;
     const int kv_heads = a.heads / a.group, parts = a.head_parts * a.query_parts;
@@ -932,72 +986,81 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 ? 2 : 1) void attn_gra
                 for (int b = lane; b < a.buckets; b += WAVE) sums[(int64_t)g * a.partial_tiles * a.buckets + b] = 0.0f;
         if (parts == 1) return;
     }
-    AttnStage<E, DP, BM, ATTN_WAVES> qs, os;
-    qs.begin(a.q, a.dim, wave, lane);
-    os.begin(a.go, a.dim, wave, lane);
+    const AttnStage<E, DP, BM, ATTN_WAVES> qs(a.q, wave, lane), os(a.go, wave, lane);
     if (a.dim < DP) {
         for (int p = 0; p < stages; ++p) attn_clear(lds + p * PLACE, 2 * BYTES, tid, ATTN_THREADS);
-        if (STAY) attn_clear(vtile, ATTN_ROWS * L::PITCH, tid, ATTN_THREADS);
         __syncthreads();
     }
-    if constexpr (STAY) {                          // (waited for with the first tile, whose loads come later)
-        AttnStage<E, DP, ATTN_ROWS, ATTN_WAVES> vs;
-        vs.begin(a.v, a.dim, wave, lane);
-        vs.load(a.v, kv, tile * ATTN_ROWS, false, a.tokens, a.dim, vtile, wave, lane);
-    }
     AttnRing ring(stages);
+    const int plain = qs.plainly(a.q, a.dim) && os.plainly(a.go, a.dim) ? walk.nclean : 0;
+    const int64_t to_next_q = (int64_t)BM * a.q.token, to_next_o = (int64_t)BM * a.go.token;
+    const E *next_q, *next_o;
+    const float* next_s;
     int next_head = head0, next = from;
+    auto at_next = [&]() __attribute__((always_inline)) {
+        const int64_t i0 = walk.at(next);
+        next_q = a.q.p + (int64_t)next_head * a.q.head + i0 * a.q.token;
+        next_o = a.go.p + (int64_t)next_head * a.go.head + i0 * a.go.token;
+        next_s = a.stats + ((int64_t)next_head * a.tokens + i0) * 2;
+    };
+    at_next();
     auto fetch = [&](int place) __attribute__((always_inline)) {
-        if (next_head == head0 + heads || from == upto) return false;
         char* const to = lds + place * PLACE;
-        const int i0 = walk.at(next);
-        const bool inside = next < walk.nclean;
-        qs.load(a.q, next_head, i0, inside, all.hi, a.dim, to, wave, lane);
-        os.load(a.go, next_head, i0, inside, all.hi, a.dim, to + BYTES, wave, lane);
-        const int i = i0 + (lane >> 1), in = i < all.hi ? i : all.hi - 1;
-        attn_load_lds<4>(a.stats + ((int64_t)next_head * a.tokens + i0) * 2, (uint32_t)((in - i0) * 8 + (lane & 1) * 4), to + 2 * BYTES + wave * 8 * BM);
+        const uint32_t stat = attn_in_lds(to) + 2 * BYTES + wave * 8 * BM;
+        if (next < plain) {
+            qs.plain(a.q, next_q, attn_in_lds(to), wave);
+            os.plain(a.go, next_o, attn_in_lds(to) + BYTES, wave);
+            attn_load_lds<4>(next_s, attn_lane() * 4, stat);
+            next_q += to_next_q;
+            next_o += to_next_o;
+            next_s += 2 * BM;
+        } else {
+            const int i0 = walk.at(next);
+            qs.load(a.q, next_head, i0, all.hi, a.dim, to, wave, lane);
+            os.load(a.go, next_head, i0, all.hi, a.dim, to + BYTES, wave, lane);
+            const int i = i0 + (lane >> 1), in = i < all.hi ? i : all.hi - 1;
+            attn_load_lds<4>(a.stats + ((int64_t)next_head * a.tokens + i0) * 2, (uint32_t)((in - i0) * 8 + (lane & 1) * 4), stat);
+        }
         if (++next == upto) {
             next = from;
             ++next_head;
+            at_next();
         }
-        return true;
     };
-    ring.fill(fetch);
-    typename T::Frag k[KS], v[STAY ? 1 : KS];
-    attn_own_rows<E, DP>(a.k, kv, there ? key : 0, there, a.dim, lane, attn_sign(a.scale), k);
-    if constexpr (!STAY) attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
+    ring.begin((upto - from) * heads, fetch);
     const uint32_t reach = there ? (uint32_t)(last - key) : 0;       // query i sees the key if (unsigned)(i - key) < reach
     const float c = a.scale_log2;
+
+    typename T::Frag k[KS], v[KS];
+    attn_own_rows<E, DP>(a.k, kv, there ? key : 0, there, a.dim, lane, attn_sign(a.scale), k);
+    attn_own_rows<E, DP>(a.v, kv, there ? key : 0, there, a.dim, lane, 1.0f, v);
     f32x16_t gk[DB], gv[DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d) { gk[d] = f32x16_t{}; gv[d] = f32x16_t{}; }
-    float far_sum = 0.0f;                          // of the head at hand, from max_distance on
+    for (int d = 0; d < DB; ++d) {
+        gk[d] = f32x16_t{};
+        gv[d] = f32x16_t{};
+    }
+    float far_sum = 0.0f;                      // of the head at hand, from max_distance on
     AttnFar far(0.0f, 1.0f);
-    const auto is_near = [&](int i0) { return BIAS && (far.apart || i0 - (key0 + 31) < a.max_distance); };
-    const auto tile_of = [&](int place) { return lds + place * PLACE; };
-    // S and dP of a tile, rows in order
-    auto scores = [&](int n, int place, f32x16_t& s, f32x16_t& dp) __attribute__((always_inline)) {
-        s = attn_start(BIAS && !is_near(walk.at(n)) ? far.start : 0.0f);
-        dp = f32x16_t{};
-        const uint32_t qt = attn_in_lds(tile_of(place));
+    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_)::value;
+        char* const here = lds + place * PLACE;
+        const uint32_t qt = attn_in_lds(here), ot = qt + BYTES;
+        const float* const st = (const float*)(here + 2 * BYTES) + wave * 2 * BM;      // (lse2, D) of each row
+        const int i0 = walk.at(n), i = i0 + 4 * half;
+        bool terms = false;
+        if constexpr (MASKED) {
+            terms = attn_look_over<E, ATTN_WAVES>(here, 2 * BYTES, span, tid, lane);
+            if (i0 >= own.hi || i0 + BM <= own.lo) return;
+        }
+        const bool near = BIAS && (far.apart || i0 - (key0 + 31) < a.max_distance);
+        const float cc = near ? 1.0f : c;
+        f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
 #pragma unroll
         for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, at, 0, x), k[x], s);
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
-            if constexpr (STAY) dp = T::mma(L::rows(qt + BYTES, at, 0, x), L::rows(vrows, at, 0, x), dp);
-            else dp = T::mma(L::rows(qt + BYTES, at, 0, x), v[x], dp);
-        }
-    };
-    auto bias = [&](int n, f32x16_t& s) __attribute__((always_inline)) {
-        const int i0 = walk.at(n);
-        if (is_near(i0)) attn_add_bias<-1>(s, c, by_distance, i0 + 4 * half - key, a.max_distance);
-    };
-    // ... become P and dS
-    auto weights = [&](auto masked_, int n, int place, f32x16_t& s, f32x16_t& dp) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_)::value;
-        const float* const st = (const float*)(tile_of(place) + 2 * BYTES) + wave * 2 * BM;      // (lse2, D) of each row
-        const int i0 = walk.at(n), i = i0 + 4 * half;
-        const float cc = is_near(i0) ? 1.0f : c;
+        for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, at, 0, x), v[x], dp);
+        if (BIAS && near) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4_t st01 = *(const f32x4_t*)(st + 16 * g + 8 * half), st23 = *(const f32x4_t*)(st + 16 * g + 8 * half + 4);
@@ -1005,75 +1068,50 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 ? 2 : 1) void attn_gra
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
                 const float ls = e < 2 ? st01[2 * e] : st23[2 * e - 4], de = e < 2 ? st01[2 * e + 1] : st23[2 * e - 3];
-                float p = attn_exp2(__builtin_fmaf(s[r], cc, -ls));
-                float x = p * (dp[r] - de);
-                if (MASKED && (uint32_t)(i + e + 8 * g - key) >= reach) p = x = 0.0f;
-                s[r] = p;
-                dp[r] = x;
+                const bool hidden = MASKED && (uint32_t)(i + e + 8 * g - key) >= reach;
+                const float p = attn_exp2(__builtin_fmaf(s[r], cc, -ls));
+                s[r] = hidden ? 0.0f : p;
+                dp[r] = hidden ? 0.0f : p * (dp[r] - de);
             }
         }
-    };
-    auto by_bucket = [&](int n, const f32x16_t& dp) __attribute__((always_inline)) {
-        if (!BIAS || !sums) return;
-        const int i0 = walk.at(n);
-        if (i0 - (key0 + 31) >= a.max_distance) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) far_sum += dp[r];
-        } else {
-            // The tile of dS by diagonals - a distance has one value on each - 16 rows at a time: lane t adds up the
-            // diagonal of distance i0 - key0 - 31 + t, and adds it to that distance's sum.  Fixed order throughout.
-            float on = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = there ? dp[8 * h + r] : 0.0f;
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int col = 16 * h + r + 31 - lane;
-                    const float x = corner[r * 33 + (col & 31)];
-                    on += col >= 0 && col < 32 ? x : 0.0f;
-                }
-                __builtin_amdgcn_wave_barrier();
-            }
-            const int d = i0 - key0 - 31 + lane;
-            if (d >= 0 && lane < 63) on_distance[d] += on;
-        }
-    };
-    auto products = [&](int place, const f32x16_t& s, const f32x16_t& dp) __attribute__((always_inline)) {
-        attn_add_product<E, DP>(attn_in_lds(tile_of(place)) + BYTES, at, 0, s, gv);
-        attn_add_product<E, DP>(attn_in_lds(tile_of(place)), at, 0, dp, gk);
-    };
-    auto masked_step = [&](int n, int place) __attribute__((always_inline)) {
-        const char* const qt = tile_of(place);
-        const int i0 = walk.at(n);
-        const bool terms = attn_look_over<E, ATTN_WAVES>(qt, 2 * BYTES, span, tid, lane);
-        if (i0 >= own.hi || i0 + BM <= own.lo) return;
-        f32x16_t s, dp;
-        scores(n, place, s, dp);
-        bias(n, s);
-        weights(std::true_type{}, n, place, s, dp);
-        if (terms) {
+        if (MASKED && terms) {
+            const auto sees = [&](int r) __attribute__((always_inline)) { return (uint32_t)(i0 + r - key) < reach; };
             const f32x16_t pw[1] = {s}, xw[1] = {dp};
-            const auto sees = [&](int r) { return (uint32_t)(i0 + r - key) < reach; };
-            attn_add_terms<E, DP, 1>(qt + BYTES, pw, gv, lane, sees);
-            attn_add_terms<E, DP, 1>(qt, xw, gk, lane, sees);
+            attn_add_terms<E, DP, 1>(here + BYTES, pw, gv, lane, sees);
+            attn_add_terms<E, DP, 1>(here, xw, gk, lane, sees);
         } else {
-            products(place, s, dp);
+            attn_add_product<E, DP>(ot, at, 0, s, gv);
+            attn_add_product<E, DP>(qt, at, 0, dp, gk);
         }
-        by_bucket(n, dp);
-    };
-    auto clean_step = [&](int n, int place) __attribute__((always_inline)) {
-        f32x16_t s, dp;
-        scores(n, place, s, dp);
-        bias(n, s);
-        weights(std::false_type{}, n, place, s, dp);
-        products(place, s, dp);
-        by_bucket(n, dp);
+        if (BIAS && sums) {
+            if (i0 - (key0 + 31) >= a.max_distance) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) far_sum += dp[r];
+            } else {
+                // The tile of dS by diagonals - a distance has one value on each - 16 rows at a time: lane t adds up the
+                // diagonal of distance i0 - key0 - 31 + t, and adds it to that distance's sum.  Fixed order throughout.
+                float on = 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) corner[(4 * half + (r & 3) + 8 * (r >> 2)) * 33 + (lane & 31)] = there ? dp[8 * h + r] : 0.0f;
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int col = 16 * h + r + 31 - lane;
+                        const float x = corner[r * 33 + (col & 31)];
+                        on += col >= 0 && col < 32 ? x : 0.0f;
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                }
+                const int d = i0 - key0 - 31 + lane;
+                if (d >= 0 && lane < 63) on_distance[d] += on;
+            }
+        }
     };
     for (int g = 0; g < heads; ++g) {
         if (BIAS) {
-            __syncthreads();                        // the table of the head before is not read any more
+            __syncthreads();                    // the table of the head before is not read any more
             attn_bias_by_distance(a, head0 + g, by_distance, tid, ATTN_THREADS);
             far = AttnFar(attn_bias(a, head0 + g, a.buckets - 1), c);
             if (sums)
@@ -1082,18 +1120,18 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 ? 2 : 1) void attn_gra
         int n = from;
         for (; n < upto && n < walk.nclean; ++n) {
             ring.template arrived<PER>();
-            ring.fill(fetch);
-            clean_step(n, ring.at);
+            ring.refill(fetch);
+            step(std::false_type{}, n, ring.at);
             ring.done();
         }
         for (; n < upto; ++n) {
             ring.template arrived<PER>();
-            ring.fill(fetch);
-            masked_step(n, ring.at);
+            ring.refill(fetch);
+            step(std::true_type{}, n, ring.at);
             ring.done();
         }
         if (BIAS && sums && from < upto) {
-            far_sum = there ? far_sum : 0.0f;       // (a column without a key is masked in the tiles of the second loop only)
+            far_sum = there ? far_sum : 0.0f;   // (a column without a key is masked in the tiles of the second loop only)
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) far_sum += __shfl_xor(far_sum, d, WAVE);
             for (int b = lane; b < a.buckets; b += WAVE) {       // a bucket's distances, in order
@@ -1107,15 +1145,11 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 ? 2 : 1) void attn_gra
         }
     }
     if (!there) return;
-    const int64_t out = ((int64_t)key * kv_heads + kv) * a.dim;
-    if (parts > 1) {
-        const int64_t size = (int64_t)a.tokens * kv_heads * a.dim;
-        attn_write_row<float, DP>(a.part_k + part * size + out, gk, a.scale, a.dim, half, a.dim % 4 == 0);
-        attn_write_row<float, DP>(a.part_v + part * size + out, gv, 1.0f, a.dim, half, a.dim % 4 == 0);
-        return;
-    }
-    if (a.gk) attn_write_row<E, DP>(a.gk + out, gk, a.scale, a.dim, half, attn_whole(a.gk, a.dim));
-    if (a.gv) attn_write_row<E, DP>(a.gv + out, gv, 1.0f, a.dim, half, attn_whole(a.gv, a.dim));
+    const int64_t out = ((int64_t)key * kv_heads + kv) * a.dim, size = (int64_t)a.tokens * kv_heads * a.dim;
+    if (parts > 1) attn_write_row<float, DP>(a.part_k + part * size + out, gk, a.scale, a.dim, half, a.dim % 4 == 0);
+    else if (a.gk) attn_write_row<E, DP>(a.gk + out, gk, a.scale, a.dim, half, attn_whole(a.gk, a.dim));
+    if (parts > 1) attn_write_row<float, DP>(a.part_v + part * size + out, gv, 1.0f, a.dim, half, a.dim % 4 == 0);
+    else if (a.gv) attn_write_row<E, DP>(a.gv + out, gv, 1.0f, a.dim, half, attn_whole(a.gv, a.dim));
 }
 
 // dk and dv from their parts, in order; rows that no sequence holds are left as they are
@@ -1257,15 +1291,15 @@ inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
         bool two = false;
         if constexpr (!(sizeof(E) == 4 && DP > 64)) {
             two = attn_two_groups<E, DP>(a, tiles);
-            if (two) attn_row_launch<2>(attn_grad_query_kernel<E, DP, BIAS, 2>, a, tiles, place, bias, asked_q[1], "attention_backward (queries)");
+            if (two) attn_row_launch<2>(attn_grad_query_kernel<E, DP, BIAS, 2>, a, tiles, place, bias + 2 * attn_fragments_out<E, DP, BIAS, 2>() * ATTN_WAVES * 1024, asked_q[1], "attention_backward (queries)");
         }
-        if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias, asked_q[0], "attention_backward (queries)");
+        if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias + attn_fragments_out<E, DP, BIAS, 1>() * ATTN_WAVES * 1024, asked_q[0], "attention_backward (queries)");
     }
     if (a.gk || a.gv || grad_table) {
-        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = (attn_values_stay<E, DP>() ? attn_tile_bytes<E, DP>(ATTN_ROWS) : 0) + bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
+        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
         const int parts = a.head_parts * a.query_parts;
         const unsigned blocks = (unsigned)(tiles * kv * parts);
-        const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && blocks > 256 ? 2 : 1);
+        const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && DP <= 64 && blocks > 256 ? 2 : 1);
         auto* kernel = attn_grad_key_kernel<E, DP, BIAS>;
         if (!attn_lds((const void*)kernel, stages * place + rest, asked_k)) return;
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_THREADS), stages * place + rest, stream(), a, tiles, stages);
