@@ -95,6 +95,25 @@ mxt_tensor mxt_module_weight(mxt_module m);
 mxt_tensor mxt_module_bias(mxt_module m);        /* NULL if the module has none */
 void mxt_module_release(mxt_module m);
 mxt_tensor mxt_mse_loss(mxt_tensor pred, mxt_tensor target);
+/* Attention over packed sequences and the clipped policy loss (no counterpart in the reference; formulas, masks and
+ * roundings: hip_attention_* and hip_policy_loss_* in maidenx_hip.h), f32 and bf16, with gradients.
+ *   indices        : a list of whole numbers on the device: the token offsets of attention, the targets of policy_loss.  A
+ *                    backward pass holds on to the lists it needs; steps of mxt_run_steps use lists made before.
+ *   attention      : query [tokens, heads, dim], key and value [tokens, kv_heads, dim] of any strides, or [tokens, heads * dim]
+ *                    as Linear writes them (heads and kv_heads say how many; 0: from a 3-d shape); bias NULL or
+ *                    [buckets, heads].  The result has the query's shape; tokens that no sequence holds get zeros, also in the
+ *                    gradients.  query, key and value that require gradients must not share a buffer (backward visits a buffer once).
+ *   policy_loss    : logits [rows, vocabulary], the other tensors f32 [rows] without gradients; the loss is one f32 element.
+ *                    logp (may be NULL) receives a new handle: the log-probability of every target.
+ * Each call waits for its kernels to report an offset or a target out of range (not while steps are recorded). */
+typedef void* mxt_indices;
+mxt_indices mxt_indices_new(const int32_t* values, size_t count);
+void mxt_indices_release(mxt_indices indices);
+mxt_tensor mxt_attention(mxt_tensor query, mxt_tensor key, mxt_tensor value, mxt_indices offsets, mxt_tensor bias,
+                         size_t max_distance, size_t heads, size_t kv_heads, float scale);
+mxt_tensor mxt_policy_loss(mxt_tensor logits, mxt_indices target, mxt_tensor old_logp, mxt_tensor ref_logp,
+                           mxt_tensor advantage, mxt_tensor weight, float clip_low, float clip_high, float kl_weight,
+                           mxt_tensor* logp);
 int mxt_sgd_step(mxt_module m, float lr);
 int mxt_sgd_zero_grad(mxt_module m);
 /* optimizers/adam.rs:16-99 with f64 hyper-parameters; the moments live in the optimizer object, one pair per

@@ -62,6 +62,11 @@ struct HipBackend {
         static constexpr auto matmul = &hip_matmul_##S;                                                                  \
         static constexpr auto matmul_backward = &hip_matmul_backward_##S;                                                \
         static constexpr auto adam_step = &hip_adam_step_##S;                                                            \
+        static constexpr auto attention = &hip_attention_##S;                                                            \
+        static constexpr auto attention_backward = &hip_attention_backward_##S;                                          \
+        static constexpr auto policy_loss = &hip_policy_loss_##S##_i32;                                                  \
+        static constexpr auto policy_loss_backward = &hip_policy_loss_backward_##S##_i32;                                \
+        static constexpr auto policy_loss_step = &hip_policy_loss_step_##S##_i32;                                        \
         /* host-side steps of the reference, done on the device */                                                       \
         static void fill(size_t n, E* p, E v) { if (n) hip_fill_##S(n, p, v); }                                          \
         static void cast_from_bool(size_t n, const uint8_t* in, E* out) { if (n) hip_cast_bool_##S(n, in, out); }        \

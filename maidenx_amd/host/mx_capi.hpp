@@ -52,6 +52,10 @@ inline T& ref(mxt_tensor t) {
     if (!t) throw mxt::Error(mxt::ErrKind::InvalidArgument, "null tensor handle");
     return *(T*)t;
 }
+inline mxt::Indices<B>& list(mxt_indices l) {
+    if (!l) throw mxt::Error(mxt::ErrKind::InvalidArgument, "null indices handle");
+    return *(mxt::Indices<B>*)l;
+}
 inline mxt::Shape to_shape(const size_t* s, size_t n) { return mxt::Shape(s, s + n); }
 inline bool is(const char* a, const char* b) { return std::strcmp(a, b) == 0; }
 [[noreturn]] inline void unknown(const char* family, const char* op) {
@@ -243,6 +247,29 @@ mxt_tensor mxt_module_bias(mxt_module m) {
 void mxt_module_release(mxt_module m) { delete (Module*)m; }
 mxt_tensor mxt_mse_loss(mxt_tensor pred, mxt_tensor target) {
     return guard_t([&] { return mxt::mse_loss<B>(ref(pred), ref(target)); });
+}
+mxt_indices mxt_indices_new(const int32_t* values, size_t count) {
+    mxt::Indices<B>* made = nullptr;
+    const int rc = guard_i([&] {
+        if (count && !values) throw mxt::Error(mxt::ErrKind::InvalidArgument, "null values");
+        made = new mxt::Indices<B>(values, count);
+    });
+    return rc ? nullptr : made;
+}
+void mxt_indices_release(mxt_indices indices) { delete (mxt::Indices<B>*)indices; }
+mxt_tensor mxt_attention(mxt_tensor query, mxt_tensor key, mxt_tensor value, mxt_indices offsets, mxt_tensor bias, size_t max_distance,
+                         size_t heads, size_t kv_heads, float scale) {
+    return guard_t([&] { return mxt::attention<B>(ref(query), ref(key), ref(value), list(offsets), bias ? &ref(bias) : nullptr, max_distance, heads, kv_heads, scale); });
+}
+mxt_tensor mxt_policy_loss(mxt_tensor logits, mxt_indices target, mxt_tensor old_logp, mxt_tensor ref_logp, mxt_tensor advantage, mxt_tensor weight,
+                           float clip_low, float clip_high, float kl_weight, mxt_tensor* logp) {
+    return guard_t([&] {
+        T each;
+        T loss = mxt::policy_loss<B>(ref(logits), list(target), ref(old_logp), ref_logp ? &ref(ref_logp) : nullptr, ref(advantage), ref(weight), clip_low, clip_high,
+                                     kl_weight, logp ? &each : nullptr);
+        if (logp) *logp = new T(each);
+        return loss;
+    });
 }
 int mxt_sgd_step(mxt_module m, float lr) { return guard_i([&] { mxt::SGD<B>(lr).step(((Module*)m)->parameters()); }); }
 int mxt_sgd_zero_grad(mxt_module m) { return guard_i([&] { mxt::SGD<B>(0.0f).zero_grad(((Module*)m)->parameters()); }); }

@@ -1424,6 +1424,170 @@ Tensor<B> mse_loss(const Tensor<B>& pred, const Tensor<B>& target) {            
     return squared.sum_all().div_scalar((float)squared.size());
 }
 
+// ---- attention and the policy loss: no counterpart in the reference ------------------------------------
+// A list of whole numbers on the device (token offsets, target indices), with the host's copy, which is what can be checked
+// before a call.  Not a tensor: nothing is computed on it and nothing flows back through it.
+template <class B>
+struct Indices {
+    std::vector<int32_t> values;
+    std::shared_ptr<Storage<B>> buf;
+    Indices(const int32_t* v, size_t n) : values(v, v + n), buf(std::make_shared<Storage<B>>(n, DType::F32)) {      // (four bytes each)
+        if (n) B::h2d(buf->ptr, values.data(), n * sizeof(int32_t));
+    }
+    const int32_t* p() const { return (const int32_t*)buf->ptr; }
+};
+
+// Causal attention over packed sequences with heads that share keys and a bias by bucketed distance (hip_attention_*).  query
+// [tokens, heads, dim], key and value [tokens, kv_heads, dim], or the heads side by side in one axis, as Linear writes them; the
+// result has the query's shape.  Tokens that no sequence holds give zeros.
+template <class B>
+Tensor<B> attention(const Tensor<B>& query, const Tensor<B>& key, const Tensor<B>& value, const Indices<B>& offsets, const Tensor<B>* bias,
+                    size_t max_distance, size_t heads, size_t kv_heads, float scale) {
+    using T = Tensor<B>;
+    const size_t tokens = query.ndim() ? query.shape()[0] : 0;
+    struct View { size_t heads, dim, strides[3]; };
+    auto view = [&](const T& t, size_t given, const char* what) {
+        const bool split = t.ndim() == 3;
+        if ((!split && t.ndim() != 2) || t.shape()[0] != tokens)
+            throw Error(ErrKind::InvalidShape, std::string("attention: ") + what + " must be [tokens, heads, dim] or [tokens, heads * dim], not " + shape_str(t.shape()));
+        if (split ? given && given != t.shape()[1] : !given || t.shape()[1] % given)
+            throw Error(ErrKind::InvalidShape, std::string("attention: ") + what + " " + shape_str(t.shape()) + " does not hold " + std::to_string(given) + " heads");
+        const size_t h = split ? t.shape()[1] : given, d = split ? t.shape()[2] : t.shape()[1] / given;
+        const size_t elem = t.strides()[t.ndim() - 1];
+        return View{h, d, {t.strides()[0], split ? t.strides()[1] : d * elem, elem}};
+    };
+    const View q = view(query, heads, "query"), k = view(key, kv_heads, "key"), v = view(value, kv_heads, "value");
+    if (q.heads == 0 || k.heads == 0 || q.heads % k.heads || v.heads != k.heads || k.dim != q.dim || v.dim != q.dim || q.dim == 0 || q.dim > 128)
+        throw Error(ErrKind::ShapeMismatch, "attention: " + shape_str(query.shape()) + ", " + shape_str(key.shape()) + " and " + shape_str(value.shape()) +
+                                                ": heads in whole groups and 1 .. 128 elements each");
+    if (!is_float(query.dtype) || key.dtype != query.dtype || value.dtype != query.dtype || (bias && bias->dtype != query.dtype))
+        throw Error(ErrKind::UnsupportedDType, "attention: query, key, value and bias must have one float type");
+    size_t buckets = 0;
+    if (bias) {
+        buckets = bias->ndim() == 2 ? bias->shape()[0] : 0;
+        if (buckets < 2 || buckets > 256 || bias->shape()[1] != q.heads) throw Error(ErrKind::ShapeMismatch, "attention: bias must be [2 .. 256 buckets, heads]");
+        if (max_distance <= buckets / 2 || max_distance > 4096) throw Error(ErrKind::InvalidArgument, "attention: max_distance lies above buckets / 2 and up to 4096");
+    }
+    if (offsets.values.empty()) throw Error(ErrKind::InvalidArgument, "attention: offsets hold one entry more than there are sequences");
+    for (size_t i = 0; i < offsets.values.size(); ++i)
+        if (offsets.values[i] < (i ? offsets.values[i - 1] : 0) || (size_t)offsets.values[i] > tokens)
+            throw Error(ErrKind::InvalidArgument, "attention: offsets must ascend from 0 or more to the number of tokens or less");
+    // the backward walk visits a buffer once: gradients of two operands in one buffer would not both arrive
+    const T* const operands[3] = {&query, &key, &value};
+    for (int i = 0; i < 3; ++i)
+        for (int j = 0; j < i; ++j)
+            if (operands[i]->requires_grad && operands[j]->requires_grad && operands[i]->buf == operands[j]->buf)
+                throw Error(ErrKind::InvalidOperation, "attention: query, key and value that require gradients must not share a buffer");
+    const bool covered = offsets.values.front() == 0 && (size_t)offsets.values.back() == tokens;      // (else rows are left out)
+    auto room = [covered](const Shape& shape, DType dt) { return covered ? T::empty(shape, dt) : T::zeros(shape, dt); };
+    std::vector<size_t> md = {tokens, q.heads, k.heads, q.dim, offsets.values.size() - 1, buckets, bias ? max_distance : 0};
+    for (const View* x : {&q, &k, &v}) md.insert(md.end(), x->strides, x->strides + 3);
+    for (const T* t : operands) md.push_back(t->offset());
+    const T table = bias ? bias->detach().contiguous() : T();
+    T out = room(query.shape(), query.dtype), lse = T::empty({q.heads, tokens}, DType::F32);
+    by_dtype(query.dtype, "attention", [&](auto tag) {
+        using E = typename decltype(tag)::type;
+        B::template K<E>::attention(md.data(), offsets.p(), query.template p<E>(), key.template p<E>(), value.template p<E>(),
+                                    bias ? table.template p<E>() + table.offset() : nullptr, scale, out.template p<E>(), lse.template p<float>());
+    });
+    ++backend_calls();
+    B::check();
+    if (query.requires_grad || key.requires_grad || value.requires_grad || (bias && bias->requires_grad)) {
+        out.with_grad();
+        std::vector<T> inputs = {query, key, value};
+        if (bias) inputs.push_back(*bias);
+        const T saved = T::share_buffer(out);
+        out.set_node("attention", inputs, [md, offsets, table, saved, lse, scale, room](const std::vector<T>& in, const T& go_in) {
+            const T go = go_in.to_dtype(saved.dtype).contiguous();
+            std::vector<T> g(in.size());
+            bool any = false;
+            for (size_t i = 0; i < in.size(); ++i)
+                if (T::wanted(in, i)) {
+                    g[i] = i < 3 ? room(in[i].shape(), saved.dtype) : T::empty(in[i].shape(), saved.dtype);
+                    g[i].sums_from_zero = true;      // (taken over as it is; a zero in it may have either sign)
+                    any = true;
+                }
+            if (any) {
+                by_dtype(saved.dtype, "attention", [&](auto tag) {
+                    using E = typename decltype(tag)::type;
+                    auto to = [&](size_t i) { return i < g.size() && g[i].buf ? g[i].template p<E>() : (E*)nullptr; };
+                    B::template K<E>::attention_backward(md.data(), offsets.p(), in[0].template p<E>(), in[1].template p<E>(), in[2].template p<E>(),
+                                                         table.buf ? table.template p<E>() + table.offset() : nullptr, scale, saved.template p<E>(),
+                                                         lse.template p<float>(), go.template p<E>() + go.offset(), to(0), to(1), to(2), to(3));
+                });
+                ++backend_calls();
+                B::check();
+            }
+            return g;
+        });
+    }
+    return out;
+}
+
+// The clipped policy loss with a KL term (hip_policy_loss_*): logits [rows, vocabulary], one target, old and reference log-probability,
+// advantage and weight for each row.  Where logits require a gradient, loss and gradient are made together, in one pass over the logits:
+// backward() from the loss hands that gradient over, any other seed (or a second call) makes it anew.
+// logp (may be null) receives the log-probability of every target.
+template <class B>
+Tensor<B> policy_loss(const Tensor<B>& logits, const Indices<B>& target, const Tensor<B>& old_logp, const Tensor<B>* ref_logp, const Tensor<B>& advantage,
+                      const Tensor<B>& weight, float clip_low, float clip_high, float kl_weight, Tensor<B>* logp_out) {
+    using T = Tensor<B>;
+    if (logits.ndim() != 2 || logits.shape()[1] == 0) throw Error(ErrKind::InvalidShape, "policy_loss: logits must be [rows, vocabulary]");
+    const size_t rows = logits.shape()[0], vocab = logits.shape()[1];
+    if (!is_float(logits.dtype)) throw Error(ErrKind::UnsupportedDType, "policy_loss: needs float logits");
+    if (target.values.size() != rows) throw Error(ErrKind::ShapeMismatch, "policy_loss: one target for each row");
+    if (!(clip_low >= 0.0f) || !(clip_high >= 0.0f)) throw Error(ErrKind::InvalidArgument, "policy_loss: clip_low and clip_high must not be negative");
+    if (!ref_logp && kl_weight != 0.0f) throw Error(ErrKind::InvalidArgument, "policy_loss: a KL term needs ref_logp");
+    auto row_list = [&](const T& t, const char* what) {
+        if (t.shape() != Shape{rows}) throw Error(ErrKind::ShapeMismatch, std::string("policy_loss: ") + what + " must have one element for each row");
+        if (t.dtype != DType::F32) throw Error(ErrKind::UnsupportedDType, std::string("policy_loss: ") + what + " must be f32");
+        if (t.requires_grad) throw Error(ErrKind::InvalidOperation, std::string("policy_loss: ") + what + " has no gradient (detach it)");
+        return t.contiguous();
+    };
+    const T old = row_list(old_logp, "old_logp"), ref = ref_logp ? row_list(*ref_logp, "ref_logp") : T(), adv = row_list(advantage, "advantage"), w = row_list(weight, "weight");
+    auto at = [](const T& t) { return t.buf ? t.template p<float>() + t.offset() : (const float*)nullptr; };
+    const std::vector<size_t> md = {rows, vocab, logits.strides()[0], logits.strides()[1], logits.offset()};
+    T loss = T::empty(Shape{}, DType::F32), logp = T::empty({rows}, DType::F32), lse = T::empty({rows}, DType::F32);
+    auto ready = std::make_shared<T>();
+    by_dtype(logits.dtype, "policy_loss", [&](auto tag) {
+        using E = typename decltype(tag)::type;
+        if (logits.requires_grad) {
+            *ready = T::empty(logits.shape(), logits.dtype);
+            B::template K<E>::policy_loss_step(md.data(), target.p(), logits.template p<E>(), at(old), at(ref), at(adv), at(w), clip_low, clip_high, kl_weight, nullptr,
+                                               loss.template p<float>(), logp.template p<float>(), lse.template p<float>(), ready->template p<E>());
+        } else {
+            B::template K<E>::policy_loss(md.data(), target.p(), logits.template p<E>(), at(old), at(ref), at(adv), at(w), clip_low, clip_high, kl_weight,
+                                          loss.template p<float>(), logp.template p<float>(), lse.template p<float>());
+        }
+    });
+    ++backend_calls();
+    B::check();
+    if (logp_out) *logp_out = logp;
+    if (logits.requires_grad) {
+        loss.with_grad();
+        loss.set_node("policy_loss", {logits}, [=](const std::vector<T>& in, const T& go_in) {
+            T g;
+            if (go_in.unit_seed && ready->buf) {
+                std::swap(g, *ready);
+            } else {
+                const T go = go_in.unit_seed ? go_in : go_in.to_dtype(DType::F32).contiguous();
+                g = T::empty(in[0].shape(), in[0].dtype);
+                by_dtype(in[0].dtype, "policy_loss", [&](auto tag) {
+                    using E = typename decltype(tag)::type;
+                    B::template K<E>::policy_loss_backward(md.data(), target.p(), in[0].template p<E>(), at(old), at(ref), at(adv), at(w), clip_low, clip_high, kl_weight,
+                                                           logp.template p<float>(), lse.template p<float>(), at(go), g.template p<E>());
+                });
+                ++backend_calls();
+                B::check();
+            }
+            g.sums_from_zero = true;      // (taken over as it is; a zero in it may have either sign)
+            return std::vector<T>{g};
+        });
+        loss.node->takes_unit_seed = true;
+    }
+    return loss;
+}
+
 template <class B>
 struct SGD {                                                                        // nn/optimizers/sgd.rs:6-37
     float lr;

@@ -6,7 +6,7 @@
     y = x.mul(x).sum_all(); y.backward(); x.grad().numpy()
 
 Method names follow crates/maidenx_tensor (add, sub, mul, div, matmul, sum, sum_to_shape, transpose,
-reshape, ...) and crates/maidenx_nn (Linear, Conv2d, MSELoss, SGD).  Errors of the reference's `Result`
+reshape, ...) and crates/maidenx_nn (Linear, Conv2d, MSELoss, SGD); attention and policy_loss have no counterpart there.  Errors of the reference's `Result`
 become `MxError` with the variant name in `.kind`.
 """
 import ctypes as C
@@ -44,7 +44,8 @@ def _bind(lib):
         "mxt_unary_scalar": ([C.c_char_p, P, F], P), "mxt_reduce": ([C.c_char_p, P, I, I], P), "mxt_shape_op": ([C.c_char_p, P, P, SZ], P),
         "mxt_linear_new": ([P, P], P), "mxt_linear_new_seeded": ([SZ, SZ, I, C.c_uint64], P),
         "mxt_conv2d_new": ([P, P, SZ, SZ, SZ, SZ, SZ, SZ], P), "mxt_module_forward": ([P, P], P), "mxt_module_weight": ([P], P),
-        "mxt_module_bias": ([P], P), "mxt_module_release": ([P], None), "mxt_mse_loss": ([P, P], P), "mxt_sgd_step": ([P, F], I),
+        "mxt_module_bias": ([P], P), "mxt_module_release": ([P], None), "mxt_mse_loss": ([P, P], P), "mxt_indices_new": ([P, SZ], P), "mxt_indices_release": ([P], None),
+        "mxt_attention": ([P, P, P, P, P, SZ, SZ, SZ, F], P), "mxt_policy_loss": ([P, P, P, P, P, P, F, F, F, P], P), "mxt_sgd_step": ([P, F], I),
         "mxt_sgd_zero_grad": ([P], I), "mxt_train": ([P, P, P, F, SZ, P], I), "mxt_set_graph_replay": ([I], None),
         "mxt_last_train_replayed": ([], SZ), "mxt_run_steps": ([P, P, SZ], I), "mxt_set_conv_skip_unread_grad_cols": ([I], None), "mxt_set_autograd_shortcuts": ([I], None), "mxt_set_fused_nn_kernels": ([I], None), "mxt_set_sum_all_in_one_pass": ([I], None), "mxt_set_conv_gathered_products": ([I], None),
         "mxt_adam_new": ([C.c_double] * 4, P), "mxt_adam_release": ([P], None), "mxt_adam_set_fused": ([P, I], None), "mxt_adam_step": ([P, P], I),
@@ -124,6 +125,32 @@ class Host:
 
     def mse_loss(self, pred, target):
         return self._t(self.lib.mxt_mse_loss(pred.h, target.h))
+
+    def indices(self, values):
+        """Whole numbers on the device: the token offsets of attention(), the targets of policy_loss()."""
+        a = np.asarray(values)
+        if a.ndim != 1 or (a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31)):
+            raise MxError("InvalidArgument", "indices: a list of 32-bit whole numbers")
+        return Indices(self, np.ascontiguousarray(a, dtype=np.int32))
+
+    def attention(self, query, key, value, offsets, bias=None, max_distance=0, heads=0, kv_heads=0, scale=None):
+        """Causal attention over packed sequences: sequence s is the tokens [offsets[s], offsets[s + 1]).  query [tokens, heads, dim],
+        key and value [tokens, kv_heads, dim], or [tokens, heads * dim] with `heads` and `kv_heads` given; bias: a table
+        [buckets, heads] by bucketed distance, the last bucket from max_distance on.  scale: 1 / sqrt(dim) by default."""
+        if scale is None:
+            dim = query.shape[-1] // (heads if len(query.shape) == 2 and heads else 1)
+            scale = dim ** -0.5 if dim else 1.0
+        return self._t(self.lib.mxt_attention(query.h, key.h, value.h, offsets.h, bias.h if bias is not None else None, max_distance,
+                                              heads, kv_heads, scale))
+
+    def policy_loss(self, logits, target, old_logp, advantage, weight, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_weight=0.0,
+                    return_logp=False):
+        """sum of weight * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight * KL estimate) over the rows of `logits`, where
+        r = exp(logp - old_logp); rows of weight zero are left out.  With return_logp also the log-probabilities of the targets."""
+        logp = C.c_void_p()
+        loss = self._t(self.lib.mxt_policy_loss(logits.h, target.h, old_logp.h, ref_logp.h if ref_logp is not None else None, advantage.h,
+                                                weight.h, clip_low, clip_high, kl_weight, C.byref(logp) if return_logp else None))
+        return (loss, Tensor(self, logp.value)) if return_logp else loss
 
     def train(self, module, x, y, lr, epochs, record_losses=False):
         """examples/device/cpu.rs:32-38, `epochs` times in native code."""
@@ -311,6 +338,20 @@ class Tensor:
     def transpose(self, d0, d1): return self._shp(b"transpose", (d0, d1))
     def squeeze(self, d): return self._shp(b"squeeze", (d,))
     def unsqueeze(self, d): return self._shp(b"unsqueeze", (d,))
+
+
+class Indices:
+    def __init__(self, host, values):
+        self.m = host
+        self.h = host.lib.mxt_indices_new(values.ctypes.data, values.size)
+        if not self.h:
+            host._raise()
+
+    def __del__(self):
+        try:
+            self.m.lib.mxt_indices_release(self.h)
+        except Exception:
+            pass
 
 
 class Module:

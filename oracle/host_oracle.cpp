@@ -30,7 +30,12 @@ extern "C" {
     void oracle_mean_##S(size_t, size_t, size_t, const size_t*, const E*, E*);                                      \
     void oracle_sum_to_shape_##S(size_t, size_t, const size_t*, const E*, E*);                                      \
     void oracle_matmul_##S(size_t, const size_t*, const E*, const E*, E*);                                          \
-    void oracle_matmul_backward_##S(size_t, size_t, const size_t*, const E*, const E*, const E*, E*, E*);
+    void oracle_matmul_backward_##S(size_t, size_t, const size_t*, const E*, const E*, const E*, E*, E*);           \
+    void oracle_attention_##S(const size_t*, const int32_t*, const E*, const E*, const E*, const E*, float, E*, float*); \
+    void oracle_attention_backward_##S(const size_t*, const int32_t*, const E*, const E*, const E*, const E*, float, const E*, const float*, const E*, E*, E*, E*, E*); \
+    void oracle_policy_loss_##S##_i32(const size_t*, const int32_t*, const E*, const float*, const float*, const float*, const float*, float, float, float, float*, float*, float*); \
+    void oracle_policy_loss_backward_##S##_i32(const size_t*, const int32_t*, const E*, const float*, const float*, const float*, const float*, float, float, float, const float*, const float*, const float*, E*); \
+    void oracle_policy_loss_step_##S##_i32(const size_t*, const int32_t*, const E*, const float*, const float*, const float*, const float*, float, float, float, const float*, float*, float*, float*, E*);
 ORC_DECL(float, f32)
 ORC_DECL(uint16_t, bf16)     // the oracle's bf16 is a struct of one uint16_t: the same bits at this boundary
 void oracle_conv2d_im2col_f32(size_t, const size_t*, const float*, float*);
@@ -78,6 +83,11 @@ template <> inline uint16_t orc_one<uint16_t>() { return 0x3F80; }
         static constexpr auto sum_to_shape = &oracle_sum_to_shape_##S;                                                   \
         static constexpr auto matmul = &oracle_matmul_##S;                                                               \
         static constexpr auto matmul_backward = &oracle_matmul_backward_##S;                                             \
+        static constexpr auto attention = &oracle_attention_##S;                                                         \
+        static constexpr auto attention_backward = &oracle_attention_backward_##S;                                       \
+        static constexpr auto policy_loss = &oracle_policy_loss_##S##_i32;                                               \
+        static constexpr auto policy_loss_backward = &oracle_policy_loss_backward_##S##_i32;                             \
+        static constexpr auto policy_loss_step = &oracle_policy_loss_step_##S##_i32;                                     \
         /* The reference does these on the host as well. */                                                             \
         static void fill(size_t n, E* p, E v) { for (size_t i = 0; i < n; ++i) p[i] = v; }                               \
         static void cast_from_bool(size_t n, const uint8_t* in, E* out) { for (size_t i = 0; i < n; ++i) out[i] = in[i] ? orc_one<E>() : E(0); } \
