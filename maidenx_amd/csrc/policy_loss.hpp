@@ -145,20 +145,28 @@ __device__ inline PolicySum policy_join_block(PolicySum s, PolicySum* shared) {
     return s;
 }
 
+// lp = x_target - lse.  What follows subtracts it from numbers near to it and sums terms that cancel: the subtraction of the two
+// is made in f64, and the logarithm of the sum gets the digits that f32 drops from a product of its own with what it stands for.
+__device__ inline double policy_logp(float x, PolicySum s, float log_sum) {
+    const float base = s.base == -INFINITY ? 0.0f : s.base;
+    const float missing = __builtin_isinf(log_sum) ? 0.0f : __builtin_fmaf(s.sum, __builtin_amdgcn_exp2f(-log_sum), -1.0f) * POLICY_LOG2E;
+    return ((double)x * (double)POLICY_LOG2E - (double)base - (double)log_sum - (double)missing) * 0.6931471805599453;
+}
+
 // ---- a row's term of the loss and its gradient with respect to lp -----------------------------------------------------------
 struct PolicyToken {
     float term, g;
 };
 template <class E, class I>
-__device__ inline PolicyToken policy_token(const PolicyArgs<E, I>& a, int row, float logp) {
+__device__ inline PolicyToken policy_token(const PolicyArgs<E, I>& a, int row, double logp) {
     const float w = a.weight[row], adv = a.advantage[row];
-    const float ratio = expf(logp - a.old_logp[row]);
+    const float ratio = expf((float)(logp - (double)a.old_logp[row]));
     const float clipped = fminf(fmaxf(ratio, a.least), a.most) * adv, plain = ratio * adv;
     PolicyToken t;
     t.term = -(plain <= clipped || plain != plain ? plain : clipped);
     t.g = plain <= clipped ? -plain : plain != plain ? plain : 0.0f;
     if (a.beta != 0.0f) {
-        const float away = a.ref_logp[row] - logp, grown = expm1f(away);
+        const float away = (float)((double)a.ref_logp[row] - logp), grown = expm1f(away);
         t.term += a.beta * (grown - away);
         t.g -= a.beta * grown;
     }
@@ -236,9 +244,9 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E,
         const float base = s.base == -INFINITY ? 0.0f : s.base, log_sum = __builtin_amdgcn_logf(s.sum);
         lse2 = base + log_sum;
         if (tid == 0 || STEP) {
-            const float logp = (__builtin_fmaf(T::get(x[(int64_t)target * a.elem]), POLICY_LOG2E, -base) - log_sum) * POLICY_LN2;
+            const double logp = policy_logp(T::get(x[(int64_t)target * a.elem]), s, log_sum);
             const PolicyToken t = policy_token(a, row, logp);
-            if (tid == 0) policy_write(a, row, logp, lse2 * POLICY_LN2, t.term);
+            if (tid == 0) policy_write(a, row, (float)logp, lse2 * POLICY_LN2, t.term);
             scale = STEP ? t.g * (a.grad_loss ? a.grad_loss[0] : 1.0f) : 0.0f;
         }
     } else if (tid == 0) {
@@ -313,8 +321,9 @@ __global__ __launch_bounds__(POLICY_SUM_THREADS) void policy_join_kernel(const P
             PolicySum s = policy_join_wave(lane < nparts ? parts[(int64_t)row * nparts + lane] : PolicySum{-INFINITY, 0.0f});
             const float base = s.base == -INFINITY ? 0.0f : s.base, log_sum = __builtin_amdgcn_logf(s.sum);
             lse = (base + log_sum) * POLICY_LN2;
-            logp = (__builtin_fmaf(PolicyType<E>::get(a.logits[(int64_t)row * a.row + (int64_t)target * a.elem]), POLICY_LOG2E, -base) - log_sum) * POLICY_LN2;
-            term = policy_token(a, row, logp).term;
+            const double lp = policy_logp(PolicyType<E>::get(a.logits[(int64_t)row * a.row + (int64_t)target * a.elem]), s, log_sum);
+            logp = (float)lp;
+            term = policy_token(a, row, lp).term;
         }
         if (lane == 0) {
             a.logp[row] = logp;
