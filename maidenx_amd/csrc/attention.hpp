@@ -226,8 +226,8 @@ __device__ __forceinline__ void attn_load_lds(const void* base, uint32_t off, ui
     else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" :: "s"(place), "v"(off), "s"(from) : "memory");
 }
 
-// GROUP waves move the tiles of their own ring; `wave` is a wave's number among them.  KEEP: a lane's offset stays in a register.
-template <class E, int DP, int ROWS, int GROUP, bool KEEP = true>
+// GROUP waves move the tiles of their own ring; `wave` is a wave's number among them.
+template <class E, int DP, int ROWS, int GROUP>
 struct AttnStage {
     using L = AttnTile<E, DP>;
     static constexpr int CALLS = ROWS * L::PITCH / 1024;       // wave instructions for a tile
@@ -247,14 +247,11 @@ struct AttnStage {
     __device__ static bool plainly(const AttnView<E>& view, int dim) { return view.vec && dim == DP && CALLS % GROUP == 0; }
     uint32_t kept;
     __device__ __forceinline__ AttnStage(const AttnView<E>& view, int wave, int lane) : kept(offset(view, 0, wave, lane)) {}
-    // (Without KEEP the offset is made anew each time: where registers are short it is the first thing that the compiler puts in
-    // memory, and a load from there waits for every tile on its way.)
     __device__ __forceinline__ void plain(const AttnView<E>& view, const E* base, uint32_t tile, int wave) const {
         const int lane = attn_lane();
-        const uint32_t first = KEEP ? kept : offset(view, 0, wave, lane);
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            attn_load_lds<16>(ALIKE ? base + u * STRIDE * view.token : base, ALIKE ? first : offset(view, u, wave, lane), tile + (u * GROUP + wave) * 1024);
+            attn_load_lds<16>(ALIKE ? base + u * STRIDE * view.token : base, ALIKE ? kept : offset(view, u, wave, lane), tile + (u * GROUP + wave) * 1024);
     }
     // any tile that begins at a token before hi
     __device__ static __forceinline__ void load(const AttnView<E>& view, int head, int token0, int hi, int dim, char* tile, int wave, int lane) {
@@ -368,6 +365,11 @@ __device__ inline void attn_bias_by_distance(const AttnArgs<E>& a, int head, flo
 }
 // Every distance from max_distance on has one bias: a tile of such pairs starts its product there (in units of the product),
 // and costs nothing.  Where that cannot be represented - a bias near the type's limits - the tile goes the way of a near one.
+// how many of n tiles, a step apart, lie at `room` or before it, the first lying at 0
+__device__ __forceinline__ int attn_tiles_beyond(int room, int step, int n) {
+    const int fit = room < 0 ? 0 : room / step + 1;
+    return fit < n ? fit : n;
+}
 struct AttnFar {
     float start;
     bool apart;
@@ -537,17 +539,21 @@ struct AttnRounds {
         return n < last ? n : last;
     }
 };
+// Kinds of tiles, each in a loop of its own.  (Clean ones that lie beyond max_distance for every row of the block, with one bias for all
+// pairs, are a kind where that pays: in the kernel of the keys up to 64 elements a head, 280 -> 262 us.  The others lose by it.)
+enum { ATTN_FAR, ATTN_CLEAN, ATTN_MASKED };
+template <int KIND> using AttnKind = std::integral_constant<int, KIND>;
 template <int PER, class Rounds, class Fetch, class Step>
 __device__ __forceinline__ void attn_run_rounds(const Rounds& rounds, AttnRing& ring, Fetch&& fetch, Step&& step) {
-    auto turn = [&](auto masked, int round) __attribute__((always_inline)) {
+    auto turn = [&](auto kind, int round) __attribute__((always_inline)) {
         ring.template arrived<PER>();
         ring.refill(fetch);
-        step(masked, round, ring.at);
+        step(kind, round, ring.at);
         ring.done();
     };
     int round = 0;
-    for (; round < rounds.clean; ++round) turn(std::false_type{}, round);
-    for (; round < rounds.total; ++round) turn(std::true_type{}, round);
+    for (; round < rounds.clean; ++round) turn(AttnKind<ATTN_CLEAN>{}, round);
+    for (; round < rounds.total; ++round) turn(AttnKind<ATTN_MASKED>{}, round);
 }
 
 // What a wave has to know of its 32 rows, and a block of all its rows: the other axis from begin to end; [inner, top) is what
@@ -702,8 +708,8 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
     float m = -INFINITY, l = 0.0f;
-    auto step = [&](auto masked_, int round, int place) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_)::value;
+    auto step = [&](auto kind_, int round, int place) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(kind_)::value == ATTN_MASKED;
         const char* const kt = mine + place * 2 * BYTES;
         const char* const vt = kt + BYTES;
         const int n = rounds.tile(round), j0 = walk.at(n);
@@ -791,25 +797,22 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 // A block owns 128 queries like the forward kernel.  Writes dq (if wanted) and, for the kernel of the keys, lse and D_i: with a
 // bias the one that makes the row of dS sum to zero (formed from P and dP themselves; the rounding of o in do . o
 // would otherwise enter every pair of the far bucket with the same sign).
-// The sum, the rows of q and those of do take all registers of a wave of two on a SIMD at 128 elements a head: some fragments of do
-// are read from LDS (a register more than there are is read from memory, behind every tile on its way).  Three leave room for two
-// blocks on a CU and are enough: 8192 tokens, 16 heads: 209 us; two 274, four 335 (one block).  With a bias they are not (369 us), and
-// five with one block on a CU take 305 us.  (Two groups of waves have room for one next to the longest table of a bias.)
-template <class E, int DP, bool BIAS, int KG> constexpr int attn_fragments_out() { return sizeof(E) == 2 && DP > 96 ? !BIAS ? 3 : KG == 1 ? 5 : 1 : 0; }
+// The sum, the rows of q and those of do take 128 registers at 128 elements a head.  With 64 keys to a tile the rest does not suffice (a
+// register more than there are is read from memory, behind every tile on its way): 8192 tokens, 16 heads with a bias 313 us, with 32
+// keys 212.
+template <class E, int DP> constexpr int attn_grad_keys() { return sizeof(E) == 2 && DP > 96 ? 32 : attn_keys<E>(); }
 template <class E, int DP, bool BIAS, int KG>
 __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int RG = ATTN_ROWS / 32, BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
+    constexpr int RG = ATTN_ROWS / 32, BN = attn_grad_keys<E, DP>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[4 * RG * KG];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, group = __builtin_amdgcn_readfirstlane(tid / (64 * RG)), wave = __builtin_amdgcn_readfirstlane(tid / 64 % RG);
     char* const mine = lds + group * stages * 2 * BYTES;         // the group's ring
     const typename L::Lane at(lane);
     int* const said = span + group * RG;
-    constexpr int OUT = attn_fragments_out<E, DP, BIAS, KG>(), IN = KS - OUT;
-    char* const out = lds + KG * stages * 2 * BYTES + ((group * RG + wave) * OUT * 64 + lane) * 16;      // the lane's last OUT fragments of do
-    float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES + KG * RG * OUT * 1024);
+    float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
     attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
@@ -819,7 +822,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
     const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
     if (all.hi <= all.lo) return;
-    const AttnStage<E, DP, BN, RG, attn_fragments_out<E, DP, BIAS, KG>() == 0> ks(a.k, wave, lane), vs(a.v, wave, lane);
+    const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
     const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
     const AttnRounds<AttnWalk<BN>, KG> rounds(walk, group);
     if (a.dim < DP) {
@@ -869,10 +872,6 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
         return;
     }
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
-    if constexpr (OUT > 0) {                       // (a wave's own: no barrier)
-#pragma unroll
-        for (int k = IN; k < KS; ++k) *(typename T::Frag*)(out + (k - IN) * 1024) = go[k];
-    }
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
     const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_log2);
     const int lower = there ? first : -1;
@@ -882,8 +881,8 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
     float rest = 0.0f;
-    auto step = [&](auto masked_, int round, int place) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_)::value;
+    auto step = [&](auto kind_, int round, int place) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(kind_)::value == ATTN_MASKED;
         const char* const kt = mine + place * 2 * BYTES;
         const char* const vt = kt + BYTES;
         const int n = rounds.tile(round), j0 = walk.at(n);
@@ -902,12 +901,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 #pragma unroll
             for (int k = 0; k < KS; ++k) s = T::mma(L::rows(attn_in_lds(kt), at, 32 * b, k), q[k], s);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                typename T::Frag g;
-                if constexpr (OUT > 0) { if (k >= IN) g = *(const typename T::Frag*)(out + (k - IN) * 1024); else g = go[k]; }
-                else g = go[k];
-                dp = T::mma(L::rows(attn_in_lds(vt), at, 32 * b, k), g, dp);
-            }
+            for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(attn_in_lds(vt), at, 32 * b, k), go[k], dp);
             const int j = j0 + 32 * b + 4 * half;
             if (BIAS && near) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance);
 #pragma unroll
@@ -1042,8 +1036,8 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     }
     float far_sum = 0.0f;                      // of the head at hand, from max_distance on
     AttnFar far(0.0f, 1.0f);
-    auto step = [&](auto masked_, int n, int place) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_)::value;
+    auto step = [&](auto kind_, int n, int place) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(kind_)::value == ATTN_MASKED, NEAR = BIAS && decltype(kind_)::value != ATTN_FAR;
         char* const here = lds + place * PLACE;
         const uint32_t qt = attn_in_lds(here), ot = qt + BYTES;
         const float* const st = (const float*)(here + 2 * BYTES) + wave * 2 * BM;      // (lse2, D) of each row
@@ -1053,14 +1047,14 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             terms = attn_look_over<E, ATTN_WAVES>(here, 2 * BYTES, span, tid, lane);
             if (i0 >= own.hi || i0 + BM <= own.lo) return;
         }
-        const bool near = BIAS && (far.apart || i0 - (key0 + 31) < a.max_distance);
+        const bool near = NEAR && (far.apart || i0 - (key0 + 31) < a.max_distance);
         const float cc = near ? 1.0f : c;
         f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
 #pragma unroll
         for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, at, 0, x), k[x], s);
 #pragma unroll
         for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, at, 0, x), v[x], dp);
-        if (BIAS && near) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance);
+        if (NEAR && near) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4_t st01 = *(const f32x4_t*)(st + 16 * g + 8 * half), st23 = *(const f32x4_t*)(st + 16 * g + 8 * half + 4);
@@ -1084,7 +1078,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             attn_add_product<E, DP>(qt, at, 0, dp, gk);
         }
         if (BIAS && sums) {
-            if (i0 - (key0 + 31) >= a.max_distance) {
+            if (!NEAR || i0 - (key0 + 31) >= a.max_distance) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) far_sum += dp[r];
             } else {
@@ -1117,19 +1111,22 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             if (sums)
                 for (int n = lane; n < a.max_distance + 63; n += WAVE) on_distance[n] = 0.0f;
         }
+        auto turn = [&](auto kind, int n) __attribute__((always_inline)) {
+            ring.template arrived<PER>();
+            ring.refill(fetch);
+            step(kind, n, ring.at);
+            ring.done();
+        };
+        const int clean = upto < walk.nclean ? upto : walk.nclean;
         int n = from;
-        for (; n < upto && n < walk.nclean; ++n) {
-            ring.template arrived<PER>();
-            ring.refill(fetch);
-            step(std::false_type{}, n, ring.at);
-            ring.done();
+        if constexpr (BIAS && DP <= 64) {           // (queries walk away from the keys: near tiles come first)
+            const int beyond = far.apart ? clean : walk.nclean - attn_tiles_beyond(walk.dirty - BM - (tile * ATTN_ROWS + ATTN_ROWS - 1 + a.max_distance), BM, walk.nclean);
+            for (; n < clean && n < beyond; ++n) turn(AttnKind<ATTN_CLEAN>{}, n);
+            for (; n < clean; ++n) turn(AttnKind<ATTN_FAR>{}, n);
+        } else {
+            for (; n < clean; ++n) turn(AttnKind<ATTN_CLEAN>{}, n);
         }
-        for (; n < upto; ++n) {
-            ring.template arrived<PER>();
-            ring.refill(fetch);
-            step(std::true_type{}, n, ring.at);
-            ring.done();
-        }
+        for (; n < upto; ++n) turn(AttnKind<ATTN_MASKED>{}, n);
         if (BIAS && sums && from < upto) {
             far_sum = there ? far_sum : 0.0f;   // (a column without a key is masked in the tiles of the second loop only)
 #pragma unroll
@@ -1287,13 +1284,13 @@ inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
     const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS, kv = a.heads / a.group;
     const size_t bias = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
     {
-        const size_t place = 2 * attn_tile_bytes<E, DP>(attn_keys<E>());
+        const size_t place = 2 * attn_tile_bytes<E, DP>(attn_grad_keys<E, DP>());
         bool two = false;
         if constexpr (!(sizeof(E) == 4 && DP > 64)) {
             two = attn_two_groups<E, DP>(a, tiles);
-            if (two) attn_row_launch<2>(attn_grad_query_kernel<E, DP, BIAS, 2>, a, tiles, place, bias + 2 * attn_fragments_out<E, DP, BIAS, 2>() * ATTN_WAVES * 1024, asked_q[1], "attention_backward (queries)");
+            if (two) attn_row_launch<2>(attn_grad_query_kernel<E, DP, BIAS, 2>, a, tiles, place, bias, asked_q[1], "attention_backward (queries)");
         }
-        if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias + attn_fragments_out<E, DP, BIAS, 1>() * ATTN_WAVES * 1024, asked_q[0], "attention_backward (queries)");
+        if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias, asked_q[0], "attention_backward (queries)");
     }
     if (a.gk || a.gv || grad_table) {
         const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
