@@ -243,8 +243,9 @@ struct AttnStage {
     __device__ static uint32_t offset(const AttnView<E>& view, int u, int wave, int lane) {
         return ((uint32_t)row_of(u, wave, lane) * (uint32_t)view.token + piece_of(u, wave, lane) * L::T::CHUNK) * (uint32_t)sizeof(E);
     }
-    // whether every lane brings a piece of every tile that lies within the walk: then a tile's loads are plain() ones
-    __device__ static bool plainly(const AttnView<E>& view, int dim) { return view.vec && dim == DP && CALLS % GROUP == 0; }
+    // whether every lane brings a piece of every tile that lies within the walk: then a tile's loads are plain() ones.  (Rows of 96
+    // elements have a pitch of 128: a lane that has no piece of the row must not reach for one.)
+    __device__ static bool plainly(const AttnView<E>& view, int dim) { return view.vec && dim == DP && L::DATA == L::PIECES && CALLS % GROUP == 0; }
     uint32_t kept;
     __device__ __forceinline__ AttnStage(const AttnView<E>& view, int wave, int lane) : kept(offset(view, 0, wave, lane)) {}
     __device__ __forceinline__ void plain(const AttnView<E>& view, const E* base, uint32_t tile, int wave) const {
@@ -272,7 +273,7 @@ struct AttnStage {
         }
     }
 };
-// pieces that no load brings (dim below DP) have to be zeros: once, for all tiles that lie there later
+// pieces that no load brings (dim below the pitch) have to be zeros: once, for all tiles that lie there later
 __device__ inline void attn_clear(char* tiles, int bytes, int tid, int threads) {
     for (int at = tid * 16; at < bytes; at += threads * 16) *(u32x4_t*)(tiles + at) = u32x4_t{0, 0, 0, 0};
 }
@@ -671,7 +672,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
     const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
     const AttnRounds<AttnWalk<BN>, KG> rounds(walk, group);
-    if (a.dim < DP) {
+    if (a.dim * (int)sizeof(E) < L::PITCH) {
         attn_clear(lds, KG * stages * 2 * BYTES, tid, 64 * RG * KG);
         __syncthreads();
     }
@@ -825,7 +826,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
     const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
     const AttnRounds<AttnWalk<BN>, KG> rounds(walk, group);
-    if (a.dim < DP) {
+    if (a.dim * (int)sizeof(E) < L::PITCH) {
         attn_clear(lds, KG * stages * 2 * BYTES, tid, 64 * RG * KG);
         __syncthreads();
     }
@@ -981,7 +982,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         if (parts == 1) return;
     }
     const AttnStage<E, DP, BM, ATTN_WAVES> qs(a.q, wave, lane), os(a.go, wave, lane);
-    if (a.dim < DP) {
+    if (a.dim * (int)sizeof(E) < L::PITCH) {
         for (int p = 0; p < stages; ++p) attn_clear(lds + p * PLACE, 2 * BYTES, tid, ATTN_THREADS);
         __syncthreads();
     }
