@@ -293,3 +293,11 @@ def test_gradients_are_the_differences(hip):
             down = value()
             flat[i] = kept
             assert abs((up - down) * 2.0 ** 5 - grad.reshape(-1)[i]) < 3e-3
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_the_longest_table(hip, dt, dim):
+    """256 buckets up to a distance of 4096: the most shared memory that a call asks for, with few blocks and with many."""
+    Attention(dt, [300, 45], 2, 1, dim, buckets=256, distance=4096, seed=dim).check(hip)
+    Attention(dt, [150] * 4, 70, 35, dim, buckets=256, distance=4096, seed=dim + 1).check(hip)
