@@ -300,43 +300,45 @@ __device__ inline void attn_own_rows(const AttnView<E>& view, int head, int toke
 // ---- sequences -----------------------------------------------------------------------------------------------------------
 // First token of the sequence of `row` and the first token behind it; false if no sequence holds the row.  Offsets that
 // do not ascend give some bounds with first <= row < last <= tokens: never an access outside the tensors.
-__device__ __forceinline__ bool attn_sequence(const int32_t* offsets, int sequences, int tokens, int row, int lane, int& first, int& last) {
+// CHECK: one wave of the first block looks the offsets over; the host reports what it finds with the next status.
+template <bool CHECK, class E>
+__device__ __forceinline__ bool attn_sequence(const AttnArgs<E>& a, int row, int lane, int& first, int& last) {
+    const int32_t* const offsets = a.offsets;
+    const int sequences = a.sequences, tokens = a.tokens;
+    const bool looks = CHECK && blockIdx.x == 0 && threadIdx.x < WAVE;
     int lo = -1, hi = tokens;
     bool above = false;
     if (sequences < WAVE) {
         const int mine = lane <= sequences ? offsets[lane] : -1;
+        if (looks) {
+            const int next = __shfl_down(mine, 1, WAVE);
+            if (lane <= sequences && (mine < 0 || mine > tokens || (lane < sequences && next < mine))) *a.flag = 1;
+        }
         for (int e = 0; e <= sequences; ++e) {
             const int off = __builtin_amdgcn_readlane(mine, e);
             if (off <= row) { if (off > lo) lo = off; }
             else { above = true; if (off < hi) hi = off; }
         }
     } else {
-        int a = 0, b = sequences + 1;              // offsets[0 .. a) <= row < offsets[b ..)
-        while (a < b) {
-            const int m = (a + b) >> 1;
-            if (offsets[m] <= row) a = m + 1;
+        if (looks)
+            for (int e = lane; e <= sequences; e += WAVE) {
+                const int off = offsets[e];
+                if (off < 0 || off > tokens || (e < sequences && offsets[e + 1] < off)) *a.flag = 1;
+            }
+        int upto = 0, b = sequences + 1;           // offsets[0 .. upto) <= row < offsets[b ..)
+        while (upto < b) {
+            const int m = (upto + b) >> 1;
+            if (offsets[m] <= row) upto = m + 1;
             else b = m;
         }
-        if (a > 0) lo = offsets[a - 1];
-        if (a <= sequences) { above = true; hi = offsets[a]; }
+        if (upto > 0) lo = offsets[upto - 1];
+        if (upto <= sequences) { above = true; hi = offsets[upto]; }
         if (hi <= row) hi = row + 1;
     }
     first = lo < 0 ? 0 : lo > row ? row : lo;
     last = hi > tokens ? tokens : hi;
     return row < tokens && lo >= 0 && above;
 }
-// One wave of the first block looks the offsets over; the host reports what it finds with the next status.
-template <class E>
-__device__ inline void attn_check_offsets(const AttnArgs<E>& a) {
-    if (blockIdx.x != 0 || threadIdx.x >= WAVE) return;
-    bool bad = false;
-    for (int e = threadIdx.x; e <= a.sequences; e += WAVE) {
-        const int off = a.offsets[e];
-        if (off < 0 || off > a.tokens || (e < a.sequences && a.offsets[e + 1] < off)) bad = true;
-    }
-    if (bad) *a.flag = 1;
-}
-
 // tile of rows and head of a block.  The blocks of a tile follow one another (the longest first); with a multiple of eight
 // heads, neighbouring heads - which share their keys - are eight blocks apart: on one XCD, behind one L2.
 __device__ inline void attn_place(int block, int tiles, int heads, bool last_first, int& tile, int& head) {
@@ -660,13 +662,12 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     const typename L::Lane at(lane);
     int* const said = span + group * RG;
     float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
-    attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
     const int kv = head / a.group;
     const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
     int first, last;
-    const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
+    const bool there = attn_sequence<true>(a, row, lane, first, last);
     const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
     if (all.hi <= all.lo) return;                   // no row of the block is in a sequence
     const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
@@ -814,13 +815,12 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     const typename L::Lane at(lane);
     int* const said = span + group * RG;
     float* const by_distance = (float*)(lds + KG * stages * 2 * BYTES);
-    attn_check_offsets(a);
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
     const int kv = head / a.group;
     const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
     int first, last;
-    const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, row, lane, first, last);
+    const bool there = attn_sequence<true>(a, row, lane, first, last);
     const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
     if (all.hi <= all.lo) return;
     const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
@@ -969,7 +969,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     kv /= parts;
     const int key0 = tile * ATTN_ROWS + wave * 32, key = key0 + (lane & 31);
     int first, last;
-    const bool there = attn_sequence(a.offsets, a.sequences, a.tokens, key, lane, first, last);
+    const bool there = attn_sequence<false>(a, key, lane, first, last);
     const AttnSpan own(there, key, last), all = own.of_block<ATTN_WAVES>(span, wave, lane);      // queries
     const int head0 = kv * a.group + part / a.query_parts * a.group / a.head_parts, heads = a.group / a.head_parts;
     float* const sums = BIAS && a.partial ? a.partial + ((int64_t)head0 * a.partial_tiles + (query_part * tiles + tile) * ATTN_WAVES + wave) * a.buckets : nullptr;
