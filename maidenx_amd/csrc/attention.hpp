@@ -644,17 +644,20 @@ __device__ inline bool attn_whole(const E* out, int dim) { return dim % 4 == 0 &
 __device__ inline float attn_sign(float scale) { return scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f; }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------
-template <class E> constexpr int attn_keys() { return sizeof(E) == 4 ? 32 : 64; }     // keys of a tile: 64 KB of LDS for two tiles of keys and values either way
+// KG groups of waves share a walk; four of them own 64 rows (two waves each), not 128.  Keys of a tile: 64 KB of LDS for two tiles of keys
+// and values of a group, 32 KB where four groups have rings.
+template <int KG> constexpr int attn_row_waves() { return KG == 4 ? 2 : ATTN_ROWS / 32; }
+template <class E, int DP, int KG> constexpr int attn_keys() { return sizeof(E) == 4 || (KG == 4 && DP > 64) ? 32 : 64; }
 template <class E, int DP>
 constexpr size_t attn_tile_bytes(int rows) { return (size_t)rows * AttnTile<E, DP>::PITCH; }
 // the running maximum may be this much (a factor of 2^8) behind before the sums are rescaled
 constexpr float ATTN_BEHIND = 8.0f;
 
 template <class E, int DP, bool BIAS, int KG>
-__global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles, int stages) {
+__global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_forward_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int RG = ATTN_ROWS / 32, BN = attn_keys<E>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
+    constexpr int RG = attn_row_waves<KG>(), BN = attn_keys<E, DP, KG>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[4 * RG * KG];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, group = __builtin_amdgcn_readfirstlane(tid / (64 * RG)), wave = __builtin_amdgcn_readfirstlane(tid / 64 % RG);
@@ -665,7 +668,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
     const int kv = head / a.group;
-    const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
+    const int row0 = tile * (32 * RG) + wave * 32, row = row0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence<true>(a, row, lane, first, last);
     const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
@@ -802,12 +805,12 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
 // The sum, the rows of q and those of do take 128 registers at 128 elements a head.  With 64 keys to a tile the rest does not suffice (a
 // register more than there are is read from memory, behind every tile on its way): 8192 tokens, 16 heads with a bias 313 us, with 32
 // keys 212.
-template <class E, int DP> constexpr int attn_grad_keys() { return sizeof(E) == 2 && DP > 96 ? 32 : attn_keys<E>(); }
+template <class E, int DP, int KG> constexpr int attn_grad_keys() { return sizeof(E) == 2 && DP > 96 ? 32 : attn_keys<E, DP, KG>(); }
 template <class E, int DP, bool BIAS, int KG>
-__global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
+__global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
-    constexpr int RG = ATTN_ROWS / 32, BN = attn_grad_keys<E, DP>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
+    constexpr int RG = attn_row_waves<KG>(), BN = attn_grad_keys<E, DP, KG>(), JB = BN / 32, DB = DP / 32, KS = DP / 16, BYTES = BN * L::PITCH;
     extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[4 * RG * KG];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, group = __builtin_amdgcn_readfirstlane(tid / (64 * RG)), wave = __builtin_amdgcn_readfirstlane(tid / 64 % RG);
@@ -818,7 +821,7 @@ __global__ __launch_bounds__(ATTN_ROWS * 2 * KG, sizeof(E) == 4 && DP > 64 ? 1 :
     int tile, head;
     attn_place(blockIdx.x, tiles, a.heads, true, tile, head);
     const int kv = head / a.group;
-    const int row0 = tile * ATTN_ROWS + wave * 32, row = row0 + (lane & 31);
+    const int row0 = tile * (32 * RG) + wave * 32, row = row0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence<true>(a, row, lane, first, last);
     const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
@@ -1256,43 +1259,60 @@ inline int attn_stages(size_t place, size_t rest, int rings, int blocks) {
     return n >= 4 ? 4 : n >= 3 ? 3 : n >= 2 || blocks == 1 ? 2 : attn_stages(place, rest, rings, 1);
 }
 template <int KG, class Kernel, class E>
-inline void attn_row_launch(Kernel* kernel, const AttnArgs<E>& a, int tiles, size_t place, size_t rest, uint64_t& asked, const char* what) {
+inline void attn_row_launch(Kernel* kernel, const AttnArgs<E>& a, size_t place, uint64_t& asked, const char* what) {
+    const int rows = 32 * attn_row_waves<KG>(), tiles = (a.tokens + rows - 1) / rows;
     const unsigned blocks = (unsigned)(tiles * a.heads);
+    const size_t rest = a.table ? ((size_t)a.max_distance + 1) * 4 : 0;
     const int stages = attn_stages(place, rest, KG, KG > 1 || blocks <= 256 ? 1 : 2);
     const size_t lds = KG * stages * place + rest;
     if (!attn_lds((const void*)kernel, lds, asked)) return;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ATTN_ROWS * 2 * KG), lds, stream(), a, tiles, stages);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * attn_row_waves<KG>() * KG), lds, stream(), a, tiles, stages);
     MXH_LAUNCH_CHECK(what);
 }
 // Up to two blocks for every CU, the time is that of the longest walks: two groups of waves share each (one block of 512
 // threads to a CU).  Beyond, they are ahead no more: 4096 tokens in one sequence, 16 heads of 128 (512 blocks): 93 against 110 us
-// forward, 32 heads: 185 against 161 us.  f32 heads above 64 take too many registers for it.
+// forward, 32 heads: 185 against 161 us.  With less than three blocks for four CUs, four groups share the walks of half as many
+// rows: f32, 1024 tokens, 8 heads of 64 with a bias (64 blocks) 47 -> 31 us forward, 65 -> 41 us dq, f16, 1802 tokens, 12 heads of 80 (180
+// blocks) 34 -> 29 and 40 -> 33 us; with 256 blocks they lose: bf16, 2000 tokens, 16 heads of 64: 32 -> 40 us.
+// f32 heads above 64 take too many registers for either.
 template <class E, int DP>
-inline bool attn_two_groups(const AttnArgs<E>& a, int tiles) { return !(sizeof(E) == 4 && DP > 64) && (int64_t)tiles * a.heads <= 512; }
+inline int attn_groups(const AttnArgs<E>& a) {
+    const int64_t blocks = (int64_t)((a.tokens + ATTN_ROWS - 1) / ATTN_ROWS) * a.heads;
+    return (sizeof(E) == 4 && DP > 64) || blocks > 512 ? 1 : blocks > 192 ? 2 : 4;
+}
 
+template <class E, int DP, bool BIAS, int KG>
+inline void attn_forward_groups(const AttnArgs<E>& a) {
+    static uint64_t asked = 0;
+    attn_row_launch<KG>(attn_forward_kernel<E, DP, BIAS, KG>, a, 2 * attn_tile_bytes<E, DP>(attn_keys<E, DP, KG>()), asked, "attention");
+}
+template <class E, int DP, bool BIAS, int KG>
+inline void attn_query_groups(const AttnArgs<E>& a) {
+    static uint64_t asked = 0;
+    attn_row_launch<KG>(attn_grad_query_kernel<E, DP, BIAS, KG>, a, 2 * attn_tile_bytes<E, DP>(attn_grad_keys<E, DP, KG>()), asked, "attention_backward (queries)");
+}
 template <class E, int DP, bool BIAS>
 inline void attn_forward_launch(const AttnArgs<E>& a) {
-    static uint64_t asked[2] = {0, 0};
-    const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS;
-    const size_t place = 2 * attn_tile_bytes<E, DP>(attn_keys<E>()), rest = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
-    if constexpr (!(sizeof(E) == 4 && DP > 64))
-        if (attn_two_groups<E, DP>(a, tiles)) return attn_row_launch<2>(attn_forward_kernel<E, DP, BIAS, 2>, a, tiles, place, rest, asked[1], "attention");
-    attn_row_launch<1>(attn_forward_kernel<E, DP, BIAS, 1>, a, tiles, place, rest, asked[0], "attention");
+    if constexpr (!(sizeof(E) == 4 && DP > 64)) {
+        if (attn_groups<E, DP>(a) == 4) return attn_forward_groups<E, DP, BIAS, 4>(a);
+        if (attn_groups<E, DP>(a) == 2) return attn_forward_groups<E, DP, BIAS, 2>(a);
+    }
+    attn_forward_groups<E, DP, BIAS, 1>(a);
+}
+template <class E, int DP, bool BIAS>
+inline void attn_query_launch(const AttnArgs<E>& a) {
+    if constexpr (!(sizeof(E) == 4 && DP > 64)) {
+        if (attn_groups<E, DP>(a) == 4) return attn_query_groups<E, DP, BIAS, 4>(a);
+        if (attn_groups<E, DP>(a) == 2) return attn_query_groups<E, DP, BIAS, 2>(a);
+    }
+    attn_query_groups<E, DP, BIAS, 1>(a);
 }
 template <class E, int DP, bool BIAS>
 inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
-    static uint64_t asked_q[2] = {0, 0}, asked_k = 0;
+    static uint64_t asked_k = 0;
     const int tiles = (a.tokens + ATTN_ROWS - 1) / ATTN_ROWS, kv = a.heads / a.group;
     const size_t bias = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
-    {
-        const size_t place = 2 * attn_tile_bytes<E, DP>(attn_grad_keys<E, DP>());
-        bool two = false;
-        if constexpr (!(sizeof(E) == 4 && DP > 64)) {
-            two = attn_two_groups<E, DP>(a, tiles);
-            if (two) attn_row_launch<2>(attn_grad_query_kernel<E, DP, BIAS, 2>, a, tiles, place, bias, asked_q[1], "attention_backward (queries)");
-        }
-        if (!two) attn_row_launch<1>(attn_grad_query_kernel<E, DP, BIAS, 1>, a, tiles, place, bias, asked_q[0], "attention_backward (queries)");
-    }
+    attn_query_launch<E, DP, BIAS>(a);
     if (a.gk || a.gv || grad_table) {
         const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
         const int parts = a.head_parts * a.query_parts;

@@ -301,3 +301,12 @@ def test_the_longest_table(hip, dt, dim):
     """256 buckets up to a distance of 4096: the most shared memory that a call asks for, with few blocks and with many."""
     Attention(dt, [300, 45], 2, 1, dim, buckets=256, distance=4096, seed=dim).check(hip)
     Attention(dt, [150] * 4, 70, 35, dim, buckets=256, distance=4096, seed=dim + 1).check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("buckets", [0, 16])
+def test_walks_of_every_number_of_groups(hip, dt, dim, buckets):
+    """Blocks for about a quarter of the CUs, for all of them, and for more than two each: the walks are shared differently."""
+    for heads in (4, 40, 90):
+        Attention(dt, [650, 3, 140], heads, heads // 2, dim, buckets=buckets, distance=100 if buckets else 0, seed=dim + heads).check(hip)
