@@ -193,6 +193,8 @@ __device__ inline void policy_write(const PolicyArgs<E, I>& a, int row, float lo
 // ---- one block a row -------------------------------------------------------------------------------------------------------
 // K pieces of a thread stay in registers between the sums and the gradient; K = 0: rows that do not fit, or whose elements are not
 // neighbours, are read again (from the caches, as a block's row is what its CU read last).
+// Loss and gradient, bf16: 2048 rows of 32000 (six in ten count) 45 us = 4.7 TB/s, 8192 rows of 50001 381 us = 4.1 TB/s, where a large copy
+// reaches 4.7; loss alone, f32, 3000 rows of 32000 (seven in ten) 46 us = 5.8 TB/s.
 template <class E, class I, int THREADS, int K, bool STEP>
 __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E, I> a) {
     using T = PolicyType<E>;
@@ -288,6 +290,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E,
 }
 
 // ---- a few long rows: several blocks a row -----------------------------------------------------------------------------------
+// f16, 16 rows of 128000: 5 us, and 3 us to join them.
 constexpr int POLICY_PART_THREADS = 256;
 constexpr int POLICY_MAX_PARTS = 64;
 template <class E, class I>
