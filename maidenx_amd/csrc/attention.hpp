@@ -26,6 +26,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "attention_walk.hpp"
 #include "mxh.hpp"
 
 namespace mxh {
@@ -203,7 +204,7 @@ __device__ inline u32x4_t attn_piece(const E* row, int d, int dim, int64_t elem,
 // ROWS tokens of one operand, from memory to a tile in LDS.  Rows are whole 16-byte pieces in the usual case: they go
 // straight to LDS (a wave's instruction fills 1 KB in a row; which piece of which row a lane fetches undoes the swizzle), with no
 // register in between, and are waited for a tile later.  The compiler does not know of these loads, so that it does not wait for
-// them before every read of LDS: AttnRing::arrived() does, in front of the barrier that hands a tile over.  Anything else
+// them before every read of LDS: attn_arrived() does, in front of the barrier that hands a tile over.  Anything else
 // (other strides, heads that are not whole pieces) goes through registers, element by element.
 // A token behind the last one that counts is replaced by that one: the mask hides what it brings.
 template <int N>
@@ -230,14 +231,13 @@ __device__ __forceinline__ void attn_load_lds(const void* base, uint32_t off, ui
 template <class E, int DP, int ROWS, int GROUP>
 struct AttnStage {
     using L = AttnTile<E, DP>;
-    static constexpr int CALLS = ROWS * L::PITCH / 1024;       // wave instructions for a tile
-    static constexpr int N = (CALLS + GROUP - 1) / GROUP;      // of a wave: that many, or (a small tile) none
-    static_assert(CALLS % GROUP == 0 || CALLS < GROUP, "what a wave waits for is counted");
+    using Share = AttnShare<ROWS, L::PITCH, GROUP>;
+    static constexpr int N = Share::N;                         // wave instructions of a wave for a tile
     // A wave's instructions bring rows that are STRIDE apart: where the swizzle is the same for them, one offset serves all, and
     // the rest is in the base.
     static constexpr int STRIDE = GROUP * 64 / L::PIECES;
     static constexpr bool ALIKE = STRIDE % 16 == 0;
-    __device__ static int row_of(int u, int wave, int lane) { return ((u * GROUP + wave) * 64 + lane) / L::PIECES; }
+    __device__ static int row_of(int u, int wave, int lane) { return Share::row_of(u, wave, lane); }
     __device__ static int piece_of(int u, int wave, int lane) { return (lane % L::PIECES) ^ L::swizzle(row_of(u, wave, lane)); }
     // bytes from the tile's first token to the lane's piece
     __device__ static uint32_t offset(const AttnView<E>& view, int u, int wave, int lane) {
@@ -245,14 +245,14 @@ struct AttnStage {
     }
     // whether every lane brings a piece of every tile that lies within the walk: then a tile's loads are plain() ones.  (Rows of 96
     // elements have a pitch of 128: a lane that has no piece of the row must not reach for one.)
-    __device__ static bool plainly(const AttnView<E>& view, int dim) { return view.vec && dim == DP && L::DATA == L::PIECES && CALLS % GROUP == 0; }
+    __device__ static bool plainly(const AttnView<E>& view, int dim) { return view.vec && dim == DP && L::DATA == L::PIECES; }
     uint32_t kept;
     __device__ __forceinline__ AttnStage(const AttnView<E>& view, int wave, int lane) : kept(offset(view, 0, wave, lane)) {}
     __device__ __forceinline__ void plain(const AttnView<E>& view, const E* base, uint32_t tile, int wave) const {
         const int lane = attn_lane();
 #pragma unroll
         for (int u = 0; u < N; ++u)
-            attn_load_lds<16>(ALIKE ? base + u * STRIDE * view.token : base, ALIKE ? kept : offset(view, u, wave, lane), tile + (u * GROUP + wave) * 1024);
+            attn_load_lds<16>(ALIKE ? base + u * STRIDE * view.token : base, ALIKE ? kept : offset(view, u, wave, lane), tile + Share::call_of(u, wave) * 1024);
     }
     // any tile that begins at a token before hi
     __device__ static __forceinline__ void load(const AttnView<E>& view, int head, int token0, int hi, int dim, char* tile, int wave, int lane) {
@@ -262,7 +262,7 @@ struct AttnStage {
             for (int u = 0; u < N; ++u) {
                 const int row = row_of(u, wave, lane), piece = piece_of(u, wave, lane), in = token0 + row < hi ? row : hi - 1 - token0;
                 const uint32_t from = (uint32_t)(in * (int)view.token + piece * L::T::CHUNK) * (uint32_t)sizeof(E);
-                if (piece * L::T::CHUNK < dim && row < ROWS) attn_load_lds<16>(base, from, attn_in_lds(tile) + (u * GROUP + wave) * 1024);
+                if (piece * L::T::CHUNK < dim) attn_load_lds<16>(base, from, attn_in_lds(tile) + Share::call_of(u, wave) * 1024);
             }
         } else {
 #pragma nounroll
@@ -270,6 +270,7 @@ struct AttnStage {
                 const int row = slot / L::PIECES, piece = (slot % L::PIECES) ^ L::swizzle(row), in = token0 + row < hi ? row : hi - 1 - token0;
                 *(u32x4_t*)(tile + slot * 16) = attn_piece<E>(base + (int64_t)in * view.token, piece * L::T::CHUNK, dim, view.elem, 0);
             }
+            attn_wait<0>();        // fewer loads than are counted for a tile: so none of those before stays on its way
         }
     }
 };
@@ -490,44 +491,17 @@ struct AttnWalk {
     }
 };
 
-// The tiles of a walk pass through a ring of `stages` (2 to 4) places in LDS: the place of a tile that is done with takes the next
-// one behind those on their way.  A wave has issued PER loads for each, which come back in order: it waits until only those of the
-// later tiles are out, then meets the others.
-struct AttnRing {
-    int stages, at = 0, to = 0, ahead = 0, left = 0;         // ahead: fetched and not done with; left: not fetched
-    __device__ explicit AttnRing(int stages_) : stages(stages_) {}
-    template <class Fetch>
-    __device__ __forceinline__ void begin(int total, Fetch&& fetch) {          // fetch(place)
-        left = total;
-        while (ahead < stages && left > 0) put(fetch);
-    }
-    template <class Fetch>
-    __device__ __forceinline__ void put(Fetch&& fetch) {
-        fetch(to);
-        --left;
-        ++ahead;
-        to = to + 1 == stages ? 0 : to + 1;
-    }
-    template <class Fetch>
-    __device__ __forceinline__ void refill(Fetch&& fetch) {        // the place of the tile before
-        if (left > 0 && ahead < stages) put(fetch);
-    }
-    // the tile at `at` has come, and the one before it is done with by all waves
-    template <int PER>
-    __device__ __forceinline__ void arrived() const {
-        static_assert(3 * PER < 64, "the counter has six bits");
-        const int later = ahead - 1;
-        if (later >= 3) attn_wait<3 * PER>();
-        else if (later == 2) attn_wait<2 * PER>();
-        else if (later == 1) attn_wait<PER>();
-        else attn_wait<0>();
-        __syncthreads();
-    }
-    __device__ void done() {
-        --ahead;
-        at = at + 1 == stages ? 0 : at + 1;
-    }
-};
+// the tile at the ring's place has come, and the one before it is done with by all waves
+template <int PER>
+__device__ __forceinline__ void attn_arrived(const AttnRing& ring) {
+    static_assert(3 * PER < 64, "the counter has six bits");
+    const int later = ring.later();
+    if (later >= 3) attn_wait<3 * PER>();
+    else if (later == 2) attn_wait<2 * PER>();
+    else if (later == 1) attn_wait<PER>();
+    else attn_wait<0>();
+    __syncthreads();
+}
 // A walk in rounds: in each, KG groups of waves take a tile of their own (every KG-th), all clean or none.  A group that is left without one in the
 // last round fetches one that it does not need: every wave counts the same loads.
 template <class Walk, int KG>
@@ -549,7 +523,7 @@ template <int KIND> using AttnKind = std::integral_constant<int, KIND>;
 template <int PER, class Rounds, class Fetch, class Step>
 __device__ __forceinline__ void attn_run_rounds(const Rounds& rounds, AttnRing& ring, Fetch&& fetch, Step&& step) {
     auto turn = [&](auto kind, int round) __attribute__((always_inline)) {
-        ring.template arrived<PER>();
+        attn_arrived<PER>(ring);
         ring.refill(fetch);
         step(kind, round, ring.at);
         ring.done();
@@ -1120,7 +1094,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
                 for (int n = lane; n < a.max_distance + 63; n += WAVE) on_distance[n] = 0.0f;
         }
         auto turn = [&](auto kind, int n) __attribute__((always_inline)) {
-            ring.template arrived<PER>();
+            attn_arrived<PER>(ring);
             ring.refill(fetch);
             step(kind, n, ring.at);
             ring.done();

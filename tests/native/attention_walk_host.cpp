@@ -1,0 +1,90 @@
+// The whole-number part of the attention kernels (maidenx_amd/csrc/attention_walk.hpp) on the host: which wave brings what of a
+// tile, and whether a tile has come when the ring says so.
+#include <cstring>
+#include <deque>
+#include <vector>
+
+#include "../../maidenx_amd/csrc/attention_walk.hpp"
+
+using namespace mxh;
+
+namespace {
+
+// what a wave has issued and not waited for, in order: the number of the tile
+struct Wave {
+    std::deque<int> out;
+    void wait(int left) { while ((int)out.size() > left) out.pop_front(); }
+};
+
+template <int ROWS, int PITCH, int GROUP>
+struct Walked {
+    using Share = AttnShare<ROWS, PITCH, GROUP>;
+    // every 16-byte place of the tile is filled, from the row that lies there, and every wave issues N instructions with a lane that
+    // has something to bring (the first piece of a row is always there); what goes wrong, counted
+    static int shares() {
+        std::vector<int> filled(Share::CALLS, 0);
+        int wrong = 0;
+        for (int wave = 0; wave < GROUP; ++wave)
+            for (int u = 0; u < Share::N; ++u) {
+                const int call = Share::call_of(u, wave);
+                if (call < 0 || call >= Share::CALLS) { ++wrong; continue; }
+                ++filled[call];
+                for (int lane = 0; lane < 64; ++lane) {
+                    const int row = Share::row_of(u, wave, lane);
+                    wrong += row < 0 || row >= ROWS || row != (call * 64 + lane) * 16 / PITCH;
+                }
+            }
+        for (int n : filled) wrong += n == 0;
+        return wrong;
+    }
+    // `total` tiles of two operands through a ring; an operand that is not direct goes through registers, after which nothing is
+    // out; `own` loads of every wave besides.  How often a wave goes on while a load of its tile is still out.
+    static int waits(int stages, int total, bool direct_a, bool direct_b, int own) {
+        const int per = 2 * Share::N + own;
+        std::vector<Wave> waves(GROUP);
+        AttnRing ring(stages);
+        int next = 0, early = 0;
+        std::vector<int> in_place(stages, -1);
+        auto fetch = [&](int place) {
+            for (int w = 0; w < GROUP; ++w) {
+                for (bool direct : {direct_a, direct_b}) {
+                    for (int u = 0; direct && u < Share::N; ++u)
+                        if (Share::row_of(u, w, 0) < ROWS) waves[w].out.push_back(next);
+                    if (!direct) waves[w].wait(0);
+                }
+                for (int x = 0; x < own; ++x) waves[w].out.push_back(next);
+            }
+            in_place[place] = next++;
+        };
+        ring.begin(total, fetch);
+        for (int tile = 0; tile < total; ++tile) {
+            const int later = ring.later();
+            for (Wave& w : waves) {
+                w.wait((later < 3 ? later : 3) * per);
+                for (int t : w.out) early += t <= tile;
+            }
+            early += in_place[ring.at] != tile;
+            ring.refill(fetch);
+            ring.done();
+        }
+        return early + ring.left;
+    }
+};
+
+template <class F>
+int each(F&& f) {
+    int wrong = 0;
+    wrong += f(Walked<32, 64, 4>{}) + f(Walked<32, 128, 4>{}) + f(Walked<32, 256, 4>{}) + f(Walked<32, 512, 4>{});
+    wrong += f(Walked<64, 64, 4>{}) + f(Walked<64, 128, 4>{}) + f(Walked<64, 256, 4>{});
+    wrong += f(Walked<32, 128, 2>{}) + f(Walked<32, 256, 2>{}) + f(Walked<64, 64, 2>{}) + f(Walked<64, 128, 2>{});
+    return wrong;
+}
+
+}  // namespace
+
+extern "C" {
+int walk_shares() { return each([](auto w) { return w.shares(); }); }
+int walk_waits(int stages, int total, int direct_a, int direct_b, int own) {
+    return each([&](auto w) { return w.waits(stages, total, direct_a != 0, direct_b != 0, own); });
+}
+}

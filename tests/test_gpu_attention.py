@@ -310,3 +310,18 @@ def test_walks_of_every_number_of_groups(hip, dt, dim, buckets):
     """Blocks for about a quarter of the CUs, for all of them, and for more than two each: the walks are shared differently."""
     for heads in (4, 40, 90):
         Attention(dt, [650, 3, 140], heads, heads // 2, dim, buckets=buckets, distance=100 if buckets else 0, seed=dim + heads).check(hip)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [16, 32])
+@pytest.mark.parametrize("layout", ["packed", "odd"])
+@pytest.mark.parametrize("heads,kv,buckets", [(4, 2, 0), (4, 2, 16), (96, 48, 16)])
+def test_small_heads_wait_for_their_rows(hip, dt, dim, layout, heads, kv, buckets):
+    """Tiles of 64-byte rows are fewer loads than a block has waves.  Walks of many tiles, with few blocks and with many: the keys' and
+    values' gradients against 64 bits, and the same bits from call to call."""
+    a = Attention(dt, [900, 130], heads, kv, dim, buckets=buckets, distance=100 if buckets else 0, layout=layout, seed=dim + heads)
+    a.check(hip)
+    out, lse = a.forward(hip)
+    first = [g.tobytes() for g in a.backward(hip, out, lse) if g is not None]
+    for _ in range(4):
+        assert [g.tobytes() for g in a.backward(hip, out, lse) if g is not None] == first
