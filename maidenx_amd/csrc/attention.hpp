@@ -317,8 +317,7 @@ __device__ __forceinline__ bool attn_sequence(const AttnArgs<E>& a, int row, int
         }
         for (int e = 0; e <= sequences; ++e) {
             const int off = __builtin_amdgcn_readlane(mine, e);
-            if (off <= row) { if (off > lo) lo = off; }
-            else { above = true; if (off < hi) hi = off; }
+            attn_take_offset(off, row, lo, hi, above);
         }
     } else {
         if (looks)
@@ -326,19 +325,9 @@ __device__ __forceinline__ bool attn_sequence(const AttnArgs<E>& a, int row, int
                 const int off = offsets[e];
                 if (off < 0 || off > tokens || (e < sequences && offsets[e + 1] < off)) *a.flag = 1;
             }
-        int upto = 0, b = sequences + 1;           // offsets[0 .. upto) <= row < offsets[b ..)
-        while (upto < b) {
-            const int m = (upto + b) >> 1;
-            if (offsets[m] <= row) upto = m + 1;
-            else b = m;
-        }
-        if (upto > 0) lo = offsets[upto - 1];
-        if (upto <= sequences) { above = true; hi = offsets[upto]; }
-        if (hi <= row) hi = row + 1;
+        attn_search(offsets, sequences, row, lo, hi, above);
     }
-    first = lo < 0 ? 0 : lo > row ? row : lo;
-    last = hi > tokens ? tokens : hi;
-    return row < tokens && lo >= 0 && above;
+    return attn_bounds(row, tokens, lo, hi, above, first, last);
 }
 // tile of rows and head of a block.  The blocks of a tile follow one another (the longest first); with a multiple of eight
 // heads, neighbouring heads - which share their keys - are eight blocks apart: on one XCD, behind one L2.
@@ -472,25 +461,6 @@ __device__ __forceinline__ void attn_add_product(uint32_t tile, const typename A
     }
 }
 
-// The tiles of a block's walk over [begin, end): first those that every row of the block sees whole, [clean, dirty) in steps of
-// STEP, then the rest, in front of them and behind.
-template <int STEP>
-struct AttnWalk {
-    int begin, clean, dirty, nclean, nfront, total;
-    __device__ __forceinline__ AttnWalk(int begin_, int end, int from, int upto) : begin(begin_) {
-        clean = from > begin ? begin + (from - begin + STEP - 1) / STEP * STEP : begin;
-        nclean = upto > clean ? (upto - clean) / STEP : 0;
-        if (nclean == 0) clean = begin;
-        dirty = clean + nclean * STEP;
-        nfront = (clean - begin) / STEP;
-        total = nclean + nfront + (end > dirty ? (end - dirty + STEP - 1) / STEP : 0);
-    }
-    // (sums of selected values: a choice between members would keep the whole struct in memory)
-    __device__ __forceinline__ int at(int n) const {
-        return clean + n * STEP + (n >= nclean ? begin - dirty : 0) + (n >= nclean + nfront ? dirty - clean : 0);
-    }
-};
-
 // the tile at the ring's place has come, and the one before it is done with by all waves
 template <int PER>
 __device__ __forceinline__ void attn_arrived(const AttnRing& ring) {
@@ -502,20 +472,6 @@ __device__ __forceinline__ void attn_arrived(const AttnRing& ring) {
     else attn_wait<0>();
     __syncthreads();
 }
-// A walk in rounds: in each, KG groups of waves take a tile of their own (every KG-th), all clean or none.  A group that is left without one in the
-// last round fetches one that it does not need: every wave counts the same loads.
-template <class Walk, int KG>
-struct AttnRounds {
-    const Walk& walk;
-    int group, clean, total;
-    __device__ __forceinline__ AttnRounds(const Walk& walk_, int group_)
-        : walk(walk_), group(group_), clean((walk_.nclean + KG - 1) / KG), total(clean + (walk_.total - walk_.nclean + KG - 1) / KG) {}
-    __device__ __forceinline__ int tile(int round) const { return round * KG + group + (round >= clean ? walk.nclean - clean * KG : 0); }
-    __device__ __forceinline__ int nearest(int round) const {
-        const int n = tile(round), last = walk.nclean - 1 + (round >= clean ? walk.total - walk.nclean : 0);
-        return n < last ? n : last;
-    }
-};
 // Kinds of tiles, each in a loop of its own.  (Clean ones that lie beyond max_distance for every row of the block, with one bias for all
 // pairs, are a kind where that pays: in the kernel of the keys up to 64 elements a head, 280 -> 262 us.  The others lose by it.)
 enum { ATTN_FAR, ATTN_CLEAN, ATTN_MASKED };
@@ -533,40 +489,28 @@ __device__ __forceinline__ void attn_run_rounds(const Rounds& rounds, AttnRing& 
     for (; round < rounds.total; ++round) turn(AttnKind<ATTN_MASKED>{}, round);
 }
 
-// What a wave has to know of its 32 rows, and a block of all its rows: the other axis from begin to end; [inner, top) is what
-// every row sees.  Rows see keys [first, row], keys are seen by queries [key, last): both ends ascend from row to row.
-struct AttnSpan {
-    int lo, hi, inner, top;
-    __device__ __forceinline__ AttnSpan(bool there, int from, int upto) {         // what a lane's row sees
-        const uint32_t rows = (uint32_t)__ballot(there);           // (the halves of a wave say the same)
-        if (rows == 0) { lo = inner = 0; hi = 0; top = 0x7fffffff; return; }
-        const int a = __builtin_ctz(rows), b = 31 - __builtin_clz(rows);
-        lo = __builtin_amdgcn_readlane(from, a);
-        inner = __builtin_amdgcn_readlane(from, b);
-        top = __builtin_amdgcn_readlane(upto, a);
-        hi = __builtin_amdgcn_readlane(upto, b);
-    }
-    template <int WAVES>                                           // of the rows of WAVES waves
-    __device__ __forceinline__ AttnSpan of_block(int* shared, int wave, int lane) const {
-        if (lane == 0) { shared[4 * wave] = hi > lo ? lo : 0x7fffffff; shared[4 * wave + 1] = hi; shared[4 * wave + 2] = inner; shared[4 * wave + 3] = top; }
-        __syncthreads();
-        AttnSpan all = *this;
-        all.lo = 0x7fffffff;
-        all.hi = 0;
+// the span of a wave's 32 rows: a lane's row sees [from, upto)
+__device__ __forceinline__ AttnSpan attn_span(bool there, int from, int upto) {
+    const uint32_t rows = (uint32_t)__ballot(there);           // (the halves of a wave say the same)
+    if (rows == 0) return AttnSpan();
+    const int a = __builtin_ctz(rows), b = 31 - __builtin_clz(rows);
+    return AttnSpan(__builtin_amdgcn_readlane(from, a), __builtin_amdgcn_readlane(upto, a), __builtin_amdgcn_readlane(from, b), __builtin_amdgcn_readlane(upto, b));
+}
+// of the rows of WAVES waves
+template <int WAVES>
+__device__ __forceinline__ AttnSpan attn_span_of_block(const AttnSpan& own, int* shared, int wave, int lane) {
+    if (lane == 0) own.put(shared + 4 * wave);
+    __syncthreads();
+    AttnSpan all;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            all.lo = shared[4 * w] < all.lo ? shared[4 * w] : all.lo;
-            all.hi = shared[4 * w + 1] > all.hi ? shared[4 * w + 1] : all.hi;
-            all.inner = shared[4 * w + 2] > all.inner ? shared[4 * w + 2] : all.inner;
-            all.top = shared[4 * w + 3] < all.top ? shared[4 * w + 3] : all.top;
-        }
-        all.lo = __builtin_amdgcn_readfirstlane(all.lo);
-        all.hi = __builtin_amdgcn_readfirstlane(all.hi);
-        all.inner = __builtin_amdgcn_readfirstlane(all.inner);
-        all.top = __builtin_amdgcn_readfirstlane(all.top);
-        return all;
-    }
-};
+    for (int w = 0; w < WAVES; ++w) all.join(shared + 4 * w);
+    all.close();
+    all.lo = __builtin_amdgcn_readfirstlane(all.lo);
+    all.hi = __builtin_amdgcn_readfirstlane(all.hi);
+    all.inner = __builtin_amdgcn_readfirstlane(all.inner);
+    all.top = __builtin_amdgcn_readfirstlane(all.top);
+    return all;
+}
 
 // Sums of another group of waves for the same rows, through LDS: `count` registers of a wave, four at a time.
 template <int DB>
@@ -648,7 +592,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     const int row0 = tile * (32 * RG) + wave * 32, row = row0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence<true>(a, row, lane, first, last);
-    const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
+    const AttnSpan own = attn_span(there, first, row + 1), all = attn_span_of_block<RG>(own, span, wave, lane);      // keys
     if (all.hi <= all.lo) return;                   // no row of the block is in a sequence
     const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
     const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
@@ -802,7 +746,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     const int row0 = tile * (32 * RG) + wave * 32, row = row0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence<true>(a, row, lane, first, last);
-    const AttnSpan own(there, first, row + 1), all = own.of_block<RG>(span, wave, lane);      // keys
+    const AttnSpan own = attn_span(there, first, row + 1), all = attn_span_of_block<RG>(own, span, wave, lane);      // keys
     if (all.hi <= all.lo) return;
     const AttnStage<E, DP, BN, RG> ks(a.k, wave, lane), vs(a.v, wave, lane);
     const AttnWalk<BN> walk(all.lo, all.hi, all.inner, all.top);
@@ -951,7 +895,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     const int key0 = tile * ATTN_ROWS + wave * 32, key = key0 + (lane & 31);
     int first, last;
     const bool there = attn_sequence<false>(a, key, lane, first, last);
-    const AttnSpan own(there, key, last), all = own.of_block<ATTN_WAVES>(span, wave, lane);      // queries
+    const AttnSpan own = attn_span(there, key, last), all = attn_span_of_block<ATTN_WAVES>(own, span, wave, lane);      // queries
     const int head0 = kv * a.group + part / a.query_parts * a.group / a.head_parts, heads = a.group / a.head_parts;
     float* const sums = BIAS && a.partial ? a.partial + ((int64_t)head0 * a.partial_tiles + (query_part * tiles + tile) * ATTN_WAVES + wave) * a.buckets : nullptr;
     const AttnWalk<BM> walk(all.lo, all.hi > all.lo ? all.hi : all.lo, all.inner, all.top);

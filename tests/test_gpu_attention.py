@@ -325,3 +325,16 @@ def test_small_heads_wait_for_their_rows(hip, dt, dim, layout, heads, kv, bucket
     first = [g.tobytes() for g in a.backward(hip, out, lse) if g is not None]
     for _ in range(4):
         assert [g.tobytes() for g in a.backward(hip, out, lse) if g is not None] == first
+
+
+@pytest.mark.parametrize("dt,dim", [("f32", 80), ("bf16", 24), ("f16", 96), ("bf16", 64)])
+def test_bad_offsets_of_many_sequences_are_reported(hip, dt, dim):
+    """Among 64 sequences and more a row's sequence is found by halves: where offsets do not ascend, an early row may see further than
+    a late one.  Every access stays within the tokens (the walk's own test goes through them all), and the call is reported."""
+    a = Attention(dt, [1500], 2, 1, dim, buckets=8, distance=16, seed=32)
+    out, lse = a.forward(hip)
+    a.offsets = np.array([0] + [1500] * 31 + [20] + [30] * 32, dtype=np.int32)
+    with pytest.raises(L.HipError, match="offsets of attention"):
+        a.forward(hip)
+    with pytest.raises(L.HipError, match="offsets of attention"):
+        a.backward(hip, out, lse)
