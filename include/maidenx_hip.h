@@ -672,6 +672,7 @@ void hip_softmax_f64(size_t num_els, size_t num_dims, size_t dim, const size_t* 
  *   ln(max_distance / E))), exactly.  -inf takes a pair out; a row whose pairs are all out has an output of zeros and
  *   lse = -inf, and gives no gradient.  Any finite bias is a bias.
  * scale: any value, zero and negative ones included.  dim: 1 .. 128.
+ * Without tokens or sequences there is nothing to do but to zero grad_bias; with tokens = 0 the tensors' addresses may be NULL.
  * output [tokens, heads, dim] and lse [heads, tokens] (f32) are contiguous.  Rows of tokens that no sequence holds are
  *   not written, here and in the gradients.  Outputs must not overlap inputs.
  * Scores, statistics and sums are f32; P (and dS in the backward pass) are rounded to the tensors' type where they enter a
@@ -699,6 +700,7 @@ MX_DECL_ATTENTION(mx_f16, f16)
  * metadata = rows, vocabulary | strides of the row and the element axis of the logits | their offset.  target: device indices
  *   [rows]; one outside [0, vocabulary) in a row that counts leaves the row out and is reported by hip_get_last_status() like an
  *   index out of range.  old_logp, ref_logp (NULL if kl_weight is 0), advantage, weight: f32 [rows].  clip_low, clip_high >= 0.
+ * Without rows the loss is zero, and the addresses of everything else may be NULL.
  * loss [1], logp [rows] (lp), lse [rows]: f32.  grad_logits [rows, vocabulary]: contiguous, of the logits' type.
  *   hip_policy_loss_..           the loss
  *   hip_policy_loss_backward_..  grad_logits = grad_loss[0] * (d loss / d x) from logp and lse of the forward call; grad_loss NULL: 1

@@ -1131,7 +1131,8 @@ inline bool attn_view(AttnView<E>& v, const void* base, const size_t* strides, s
 // metadata: tokens, heads, kv_heads, dim, sequences, buckets, max_distance | q, k, v strides | q, k, v offsets
 template <class E>
 inline bool attn_arguments(AttnArgs<E>& a, const size_t* md, const int32_t* offsets, const E* q, const E* k, const E* v, const E* table, float scale) {
-    if (!md || !offsets || !q || !k || !v) { set_status(ERR_INVALID, "attention: null argument"); return false; }
+    const bool some = !md || md[0] != 0;        // (tensors of no tokens have no address)
+    if (!md || !offsets || (some && (!q || !k || !v))) { set_status(ERR_INVALID, "attention: null argument"); return false; }
     const size_t tokens = md[0], heads = md[1], kv = md[2], dim = md[3], sequences = md[4];
     if (heads == 0 || kv == 0 || dim == 0 || heads % kv != 0) { set_status(ERR_INVALID, "attention: heads must be a multiple of kv_heads, and dim positive"); return false; }
     if (dim > (size_t)ATTN_MAX_DIM) { set_status(ERR_UNSUPPORTED, "attention: head dimension above 128"); return false; }
@@ -1159,6 +1160,7 @@ inline bool attn_arguments(AttnArgs<E>& a, const size_t* md, const int32_t* offs
         a.max_distance = (int32_t)distance;
         if (!attn_borders((int)buckets, (int)distance, a.borders)) return false;
     }
+    if (tokens == 0 || sequences == 0) return true;
     a.flag = index_flag();
     return a.flag != nullptr;
 }
@@ -1271,7 +1273,7 @@ inline void attn_by_dim(const AttnArgs<E>& a, F&& f) {
 template <class E>
 inline void attention_entry(const size_t* md, const int32_t* offsets, const E* q, const E* k, const E* v, const E* table, float scale, E* out, float* lse) {
     AttnArgs<E> a;
-    if (!out || !lse) { set_status(ERR_INVALID, "attention: null output"); return; }
+    if ((!out || !lse) && !(md && md[0] == 0)) { set_status(ERR_INVALID, "attention: null output"); return; }
     if (!attn_arguments(a, md, offsets, q, k, v, table, scale)) return;
     if (a.tokens == 0 || a.sequences == 0) return;
     a.out = out;
@@ -1286,7 +1288,7 @@ template <class E>
 inline void attention_backward_entry(const size_t* md, const int32_t* offsets, const E* q, const E* k, const E* v, const E* table, float scale, const E* out,
                                      const float* lse, const E* grad_out, E* gq, E* gk, E* gv, E* grad_table) {
     AttnArgs<E> a;
-    if (!out || !lse || !grad_out) { set_status(ERR_INVALID, "attention_backward: null argument"); return; }
+    if ((!out || !lse || !grad_out) && !(md && md[0] == 0)) { set_status(ERR_INVALID, "attention_backward: null argument"); return; }
     if (grad_table && !table) { set_status(ERR_INVALID, "attention_backward: the gradient of a bias that was not given"); return; }
     if (!attn_arguments(a, md, offsets, q, k, v, table, scale)) return;
     if (!gq && !gk && !gv && !grad_table) return;
@@ -1297,8 +1299,12 @@ inline void attention_backward_entry(const size_t* md, const int32_t* offsets, c
     a.gq = gq;
     a.gk = gk;
     a.gv = gv;
-    const bool empty = a.tokens == 0 || a.sequences == 0;
-    if (empty && !grad_table) return;
+    if (a.tokens == 0 || a.sequences == 0) {        // no pair: the table's gradient is zero
+        if (!grad_table) return;
+        hipLaunchKernelGGL(attn_grad_table_kernel<E>, dim3((unsigned)a.buckets, (unsigned)a.heads), dim3(ATTN_THREADS), 0, stream(), (const float*)nullptr, 0, a.buckets, a.heads, grad_table);
+        MXH_LAUNCH_CHECK("attention_backward (bias)");
+        return;
+    }
     // parts of the kernel of the keys: until there are two blocks for every CU, first the heads of a group, then the queries
     // (eight tiles of them at least)
     const size_t tiles = cdiv((size_t)a.tokens, (size_t)ATTN_ROWS), kv = (size_t)(a.heads / a.group);
@@ -1307,18 +1313,13 @@ inline void attention_backward_entry(const size_t* md, const int32_t* offsets, c
     while (tiles * kv * a.head_parts * a.query_parts < 512 && (size_t)a.tokens / 32 / a.query_parts >= 16) a.query_parts *= 2;
     const int parts = a.head_parts * a.query_parts;
     const size_t stats = ((size_t)a.heads * a.tokens * 2 + 63) / 64 * 64, sums = parts > 1 ? ((size_t)a.tokens * kv * a.dim + 63) / 64 * 64 * parts : 0;
-    a.partial_tiles = empty ? 0 : (int)(ATTN_WAVES * tiles) * a.query_parts;
+    a.partial_tiles = (int)(ATTN_WAVES * tiles) * a.query_parts;
     const size_t partials = grad_table ? (size_t)a.heads * a.partial_tiles * a.buckets : 0;
     a.stats = (float*)scratch((stats + 2 * sums + partials) * sizeof(float));
     if (!a.stats) return;
     a.part_k = a.stats + stats;
     a.part_v = a.part_k + sums;
     a.partial = grad_table ? a.part_v + sums : nullptr;
-    if (empty) {
-        hipLaunchKernelGGL(attn_grad_table_kernel<E>, dim3((unsigned)a.buckets, (unsigned)a.heads), dim3(ATTN_THREADS), 0, stream(), a.partial, 0, a.buckets, a.heads, grad_table);
-        MXH_LAUNCH_CHECK("attention_backward (bias)");
-        return;
-    }
     attn_by_dim(a, [&](auto dp) {
         if (table) attn_backward_launch<E, decltype(dp)::value, true>(a, grad_table);
         else attn_backward_launch<E, decltype(dp)::value, false>(a, grad_table);

@@ -374,8 +374,9 @@ void policy_sum(const float* terms, int n, float* loss);
 template <class E, class I>
 inline bool policy_arguments(PolicyArgs<E, I>& a, const size_t* md, const I* target, const E* logits, const float* old_logp, const float* ref_logp,
                              const float* advantage, const float* weight, float low, float high, float beta) {
-    if (!md || !target || !logits || !old_logp || !advantage || !weight) { set_status(ERR_INVALID, "policy_loss: null argument"); return false; }
-    if (!ref_logp && beta != 0.0f) { set_status(ERR_INVALID, "policy_loss: the KL term needs ref_logp"); return false; }
+    const bool some = !md || md[0] != 0;        // (tensors of no rows have no address)
+    if (!md || (some && (!target || !logits || !old_logp || !advantage || !weight))) { set_status(ERR_INVALID, "policy_loss: null argument"); return false; }
+    if (some && !ref_logp && beta != 0.0f) { set_status(ERR_INVALID, "policy_loss: the KL term needs ref_logp"); return false; }
     if (!(low >= 0.0f) || !(high >= 0.0f)) { set_status(ERR_INVALID, "policy_loss: the clip range is not negative"); return false; }
     if (md[1] == 0) { set_status(ERR_INVALID, "policy_loss: an empty vocabulary"); return false; }
     if (md[0] >= (1ull << 31) - 1024 || md[1] >= (1ull << 31) - 1024) { set_status(ERR_TOO_LARGE, "policy_loss: too many rows or logits"); return false; }
@@ -393,6 +394,7 @@ inline bool policy_arguments(PolicyArgs<E, I>& a, const size_t* md, const I* tar
     a.beta = beta;
     a.rows = (int32_t)md[0];
     a.vocab = (int32_t)md[1];
+    if (a.rows == 0) return true;
     a.flag = index_flag();
     return a.flag != nullptr;
 }
@@ -426,7 +428,8 @@ template <class E, class I>
 inline void policy_entry(const size_t* md, const I* target, const E* logits, const float* old_logp, const float* ref_logp, const float* advantage,
                          const float* weight, float low, float high, float beta, const float* grad_loss, float* loss, float* logp, float* lse, E* grad, bool step) {
     PolicyArgs<E, I> a;
-    if (!loss || !logp || !lse || (step && !grad)) { set_status(ERR_INVALID, "policy_loss: null output"); return; }
+    const bool some = !md || md[0] != 0;
+    if (!loss || (some && (!logp || !lse || (step && !grad)))) { set_status(ERR_INVALID, "policy_loss: null output"); return; }
     if (!policy_arguments(a, md, target, logits, old_logp, ref_logp, advantage, weight, low, high, beta)) return;
     a.grad_loss = grad_loss;
     a.loss = loss;
@@ -463,7 +466,7 @@ template <class E, class I>
 inline void policy_backward_entry(const size_t* md, const I* target, const E* logits, const float* old_logp, const float* ref_logp, const float* advantage,
                                   const float* weight, float low, float high, float beta, const float* logp, const float* lse, const float* grad_loss, E* grad) {
     PolicyArgs<E, I> a;
-    if (!logp || !lse || !grad) { set_status(ERR_INVALID, "policy_loss_backward: null argument"); return; }
+    if ((!logp || !lse || !grad) && !(md && md[0] == 0)) { set_status(ERR_INVALID, "policy_loss_backward: null argument"); return; }
     if (!policy_arguments(a, md, target, logits, old_logp, ref_logp, advantage, weight, low, high, beta)) return;
     if (a.rows == 0) return;
     a.grad_loss = grad_loss;

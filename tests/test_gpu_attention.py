@@ -338,3 +338,35 @@ def test_bad_offsets_of_many_sequences_are_reported(hip, dt, dim):
         a.forward(hip)
     with pytest.raises(L.HipError, match="offsets of attention"):
         a.backward(hip, out, lse)
+
+
+FIRST_CALL = """
+import sys
+sys.path[:0] = {paths!r}
+import numpy as np
+import maidenx_amd.lib as L
+from language import meta_attention
+md = meta_attention(0, 2, 1, 8, {sequences}, 4, 8, [16, 8, 1], [8, 8, 1], [8, 8, 1])
+offsets = L.DeviceBuffer.from_numpy(np.zeros({sequences} + 1, np.int32))
+table = L.DeviceBuffer.from_numpy(np.ones(8, np.{np}))
+grad = L.DeviceBuffer.from_numpy(np.ones(8, np.{np}))
+L.call("attention_{dt}", md, offsets, None, None, None, table, 1.0, None, None)
+L.synchronize()
+L.call("attention_backward_{dt}", md, offsets, None, None, None, table, 1.0, None, None, None, None, None, None, grad)
+L.synchronize()
+assert (grad.to_numpy(np.{np}) == 0).all()
+print("zeros")
+"""
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("sequences", [0, 3])
+def test_no_tokens(dt, sequences):
+    """The first calls of a process, when the library has no workspace yet: no tokens, tensors without an address, and a table whose
+    gradient is zero."""
+    import subprocess
+    import sys
+    from helpers import ROOT
+    code = FIRST_CALL.format(paths=[ROOT, ROOT + "/tests"], sequences=sequences, dt=dt, np="float32" if dt == "f32" else "uint16")
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0 and "zeros" in p.stdout, p.stderr[-2000:]

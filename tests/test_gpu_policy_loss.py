@@ -179,3 +179,13 @@ def test_gradient_is_the_differences(hip):
                 sides.append(float(p.forward(hip)[0][0]))
             p.x[r, v] = kept
             assert abs((sides[0] - sides[1]) * 2.0 ** 6 - grad[r, v]) < 2e-3
+
+
+@pytest.mark.parametrize("suffix", ["f32_i64", "bf16_i32", "f16_i64"])
+def test_no_rows_and_no_addresses(hip, suffix):
+    """Tensors of no rows may have no address; the loss is zero, a separate backward call has nothing to write."""
+    md, none = u64(0, 5, 5, 1, 0), [Null()] * 6
+    for name, rest in (("policy_loss_", []), ("policy_loss_step_", [Null()])):
+        loss = hip.call(name + suffix, md, *none, 0.2, 0.2, 0.1, *rest, Out(1, "f32"), Null(), Null(), *([Null()] if rest else []))[0]
+        assert loss[0] == 0
+    hip.call("policy_loss_backward_" + suffix, md, *none, 0.2, 0.2, 0.1, Null(), Null(), Null(), Null())
