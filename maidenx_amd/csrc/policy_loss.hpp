@@ -106,28 +106,34 @@ __device__ inline void policy_store(E* row, int vocab, int lead, int piece, bool
     }
 }
 
-// running (base, sum) of a row in units of log2: the sum of exp2(x log2(e) - base)
+// running (base, sum) of a row: the sum of exp(x - base).  The difference is taken before it is brought to units of log2: logits near
+// the type's limits have no such units.
 struct PolicySum {
     float base, sum;
 };
+// An instruction less for each logit: exp(x - base) as 2^(x log2(e) - base log2(e)), where base is small enough for its product's rounding
+// to be nothing beside the tensors' own (16 bits; 256 log2(e) 2^-24 = 2^-15).  bf16, 8192 rows of 50001: 329 us with
+// the choice, 395 where every logit is subtracted from; 2048 rows of 32000 are the same, 50.
+template <class E>
+__device__ inline bool policy_near(float base) { return sizeof(E) == 2 && __builtin_fabsf(base) <= 256.0f; }
+__device__ inline float policy_exp(float x) { return __builtin_amdgcn_exp2f(x * POLICY_LOG2E); }
 __device__ inline PolicySum policy_join(PolicySum a, PolicySum b) {
     const float base = fmaxf(a.base, b.base);
     if (base == -INFINITY) return {base, a.sum + b.sum};     // (nothing yet: sums are zero, or NaN)
-    return {base, a.sum * __builtin_amdgcn_exp2f(a.base - base) + b.sum * __builtin_amdgcn_exp2f(b.base - base)};
+    return {base, a.sum * policy_exp(a.base - base) + b.sum * policy_exp(b.base - base)};
 }
 template <int N>
 __device__ inline void policy_take(PolicySum& s, const float (&x)[N]) {
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
-    top *= POLICY_LOG2E;
     if (top > s.base) {
-        s.sum *= __builtin_amdgcn_exp2f(s.base - top);
+        s.sum *= policy_exp(s.base - top);
         s.base = top;
     }
     const float base = s.base == -INFINITY ? 0.0f : s.base;
 #pragma unroll
-    for (int e = 0; e < N; ++e) s.sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], POLICY_LOG2E, -base));
+    for (int e = 0; e < N; ++e) s.sum += policy_exp(x[e] - base);
 }
 __device__ inline PolicySum policy_join_wave(PolicySum s) {
 #pragma unroll
@@ -150,7 +156,7 @@ __device__ inline PolicySum policy_join_block(PolicySum s, PolicySum* shared) {
 __device__ inline double policy_logp(float x, PolicySum s, float log_sum) {
     const float base = s.base == -INFINITY ? 0.0f : s.base;
     const float missing = __builtin_isinf(log_sum) ? 0.0f : __builtin_fmaf(s.sum, __builtin_amdgcn_exp2f(-log_sum), -1.0f) * POLICY_LOG2E;
-    return ((double)x * (double)POLICY_LOG2E - (double)base - (double)log_sum - (double)missing) * 0.6931471805599453;
+    return (double)x - (double)base - ((double)log_sum + (double)missing) * 0.6931471805599453;
 }
 
 // ---- a row's term of the loss and its gradient with respect to lp -----------------------------------------------------------
@@ -193,8 +199,8 @@ __device__ inline void policy_write(const PolicyArgs<E, I>& a, int row, float lo
 // ---- one block a row -------------------------------------------------------------------------------------------------------
 // K pieces of a thread stay in registers between the sums and the gradient; K = 0: rows that do not fit, or whose elements are not
 // neighbours, are read again (from the caches, as a block's row is what its CU read last).
-// Loss and gradient, bf16: 2048 rows of 32000 (six in ten count) 45 us = 4.7 TB/s, 8192 rows of 50001 381 us = 4.1 TB/s, where a large copy
-// reaches 4.7; loss alone, f32, 3000 rows of 32000 (seven in ten) 46 us = 5.8 TB/s.
+// Loss and gradient, bf16: 2048 rows of 32000 (six in ten count) 50 us a call = 4.2 TB/s, 8192 rows of 50001 329 us = 4.7 TB/s, where a large
+// copy reaches 4.7; loss alone, f32, 3000 rows of 32000 (seven in ten) 50 us a call = 5.3 TB/s.
 template <class E, class I, int THREADS, int K, bool STEP>
 __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E, I> a) {
     using T = PolicyType<E>;
@@ -206,7 +212,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E,
     const int lead = K || a.elem == 1 ? policy_lead(x) : 0, pieces = (lead + a.vocab + N - 1) / N;
     E* const y = STEP ? a.grad + (int64_t)row * a.vocab : nullptr;
     const bool aligned = STEP && policy_lead(y) == lead && (K || a.elem == 1);
-    float scale = 0.0f, lse2 = 0.0f;
+    float scale = 0.0f, base = 0.0f, log_sum = 0.0f;
     policy_piece held[K ? K : 1];
     if (target >= 0) {
         PolicySum s{-INFINITY, 0.0f};
@@ -224,16 +230,25 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E,
                     for (int e = 0; e < N; ++e) top = fmaxf(top, T::get(z[e]));
                 }
             }
-            s.base = top * POLICY_LOG2E;
-            const float base = s.base == -INFINITY ? 0.0f : s.base;
+            s.base = top;
+            const float from = s.base == -INFINITY ? 0.0f : s.base;
+            auto add = [&](auto exponential) {
 #pragma unroll
-            for (int u = 0; u < K; ++u) {
-                if (tid + u * THREADS < pieces) {
-                    E z[N];
-                    __builtin_memcpy(z, &held[u], 16);
+                for (int u = 0; u < K; ++u) {
+                    if (tid + u * THREADS < pieces) {
+                        E z[N];
+                        __builtin_memcpy(z, &held[u], 16);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) s.sum += __builtin_amdgcn_exp2f(__builtin_fmaf(T::get(z[e]), POLICY_LOG2E, -base));
+                        for (int e = 0; e < N; ++e) s.sum += exponential(T::get(z[e]));
+                    }
                 }
+            };
+            if (policy_near<E>(from)) {
+                const float from2 = from * POLICY_LOG2E;
+                add([&](float z) { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, POLICY_LOG2E, -from2)); });
+                s.sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(from, POLICY_LOG2E, -from2));      // what the product's rounding left in every term
+            } else {
+                add([&](float z) { return policy_exp(z - from); });
             }
         } else {
             for (int p = tid; p < pieces; p += THREADS) {
@@ -243,12 +258,12 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E,
             }
         }
         s = policy_join_block<THREADS>(s, shared);
-        const float base = s.base == -INFINITY ? 0.0f : s.base, log_sum = __builtin_amdgcn_logf(s.sum);
-        lse2 = base + log_sum;
+        base = s.base == -INFINITY ? 0.0f : s.base;
+        log_sum = __builtin_amdgcn_logf(s.sum);
         if (tid == 0 || STEP) {
             const double logp = policy_logp(T::get(x[(int64_t)target * a.elem]), s, log_sum);
             const PolicyToken t = policy_token(a, row, logp);
-            if (tid == 0) policy_write(a, row, (float)logp, lse2 * POLICY_LN2, t.term);
+            if (tid == 0) policy_write(a, row, (float)logp, __builtin_fmaf(log_sum, POLICY_LN2, base), t.term);
             scale = STEP ? t.g * (a.grad_loss ? a.grad_loss[0] : 1.0f) : 0.0f;
         }
     } else if (tid == 0) {
@@ -261,31 +276,39 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E,
             for (int p = tid; p < out_pieces; p += THREADS) policy_store(y, a.vocab, out_lead, p, true, zero);
             return;
         }
-        auto finish = [&](float (&z)[N], int p) {
+        const float lse2 = __builtin_fmaf(base, POLICY_LOG2E, log_sum);
+        auto finish = [&](auto near, float (&z)[N], int p) {
             const int v0 = p * N - lead;
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e] = scale * ((v0 + e == target ? 1.0f : 0.0f) - __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], POLICY_LOG2E, -lse2)));
+            for (int e = 0; e < N; ++e) {
+                const float share = near ? __builtin_fmaf(z[e], POLICY_LOG2E, -lse2) : __builtin_fmaf(z[e] - base, POLICY_LOG2E, -log_sum);
+                z[e] = scale * ((v0 + e == target ? 1.0f : 0.0f) - __builtin_amdgcn_exp2f(share));
+            }
             policy_store(y, a.vocab, lead, p, aligned, z);
         };
-        if constexpr (K > 0) {
+        auto all = [&](auto near) {
+            if constexpr (K > 0) {
 #pragma unroll
-            for (int u = 0; u < K; ++u) {
-                if (tid + u * THREADS < pieces) {
-                    E h[N];
+                for (int u = 0; u < K; ++u) {
+                    if (tid + u * THREADS < pieces) {
+                        E h[N];
+                        float z[N];
+                        __builtin_memcpy(h, &held[u], 16);
+#pragma unroll
+                        for (int e = 0; e < N; ++e) z[e] = T::get(h[e]);
+                        finish(near, z, tid + u * THREADS);
+                    }
+                }
+            } else {
+                for (int p = tid; p < pieces; p += THREADS) {
                     float z[N];
-                    __builtin_memcpy(h, &held[u], 16);
-#pragma unroll
-                    for (int e = 0; e < N; ++e) z[e] = T::get(h[e]);
-                    finish(z, tid + u * THREADS);
+                    policy_load(x, a.elem, a.vocab, lead, p, a.elem == 1, z);
+                    finish(near, z, p);
                 }
             }
-        } else {
-            for (int p = tid; p < pieces; p += THREADS) {
-                float z[N];
-                policy_load(x, a.elem, a.vocab, lead, p, a.elem == 1, z);
-                finish(z, p);
-            }
-        }
+        };
+        if (policy_near<E>(base)) all(std::true_type{});
+        else all(std::false_type{});
     }
 }
 
@@ -323,7 +346,7 @@ __global__ __launch_bounds__(POLICY_SUM_THREADS) void policy_join_kernel(const P
         if (target >= 0) {
             PolicySum s = policy_join_wave(lane < nparts ? parts[(int64_t)row * nparts + lane] : PolicySum{-INFINITY, 0.0f});
             const float base = s.base == -INFINITY ? 0.0f : s.base, log_sum = __builtin_amdgcn_logf(s.sum);
-            lse = (base + log_sum) * POLICY_LN2;
+            lse = __builtin_fmaf(log_sum, POLICY_LN2, base);
             const double lp = policy_logp(PolicyType<E>::get(a.logits[(int64_t)row * a.row + (int64_t)target * a.elem]), s, log_sum);
             logp = (float)lp;
             term = policy_token(a, row, lp).term;
@@ -354,14 +377,17 @@ __global__ __launch_bounds__(POLICY_PART_THREADS) void policy_grad_kernel(const 
     const bool aligned = a.elem == 1 && policy_lead(x) == lead;
     const int from = blockIdx.x * per, upto = from + per < pieces ? from + per : pieces;
     const float scale = target >= 0 ? policy_token(a, row, a.logp[row]).g * (a.grad_loss ? a.grad_loss[0] : 1.0f) : 0.0f;
-    const float lse2 = a.lse[row] * POLICY_LOG2E;
+    // x - lse = (x - x_target) + lp: whichever of lse and lp is the smaller has lost less to its rounding
+    const float lse = a.lse[row], lp = a.logp[row];
+    const bool by_target = target >= 0 && __builtin_fabsf(lp) <= __builtin_fabsf(lse);
+    const float base = by_target ? PolicyType<E>::get(x[(int64_t)target * a.elem]) : lse, rest = by_target ? lp * POLICY_LOG2E : 0.0f;
     for (int p = from + threadIdx.x; p < upto; p += POLICY_PART_THREADS) {
         float z[N] = {};
         if (scale != 0.0f) {
             policy_load(x, a.elem, a.vocab, lead, p, aligned, z);
             const int v0 = p * N - lead;
 #pragma unroll
-            for (int e = 0; e < N; ++e) z[e] = scale * ((v0 + e == target ? 1.0f : 0.0f) - __builtin_amdgcn_exp2f(__builtin_fmaf(z[e], POLICY_LOG2E, -lse2)));
+            for (int e = 0; e < N; ++e) z[e] = scale * ((v0 + e == target ? 1.0f : 0.0f) - __builtin_amdgcn_exp2f(__builtin_fmaf(z[e] - base, POLICY_LOG2E, rest)));
         }
         policy_store(y, a.vocab, lead, p, true, z);
     }

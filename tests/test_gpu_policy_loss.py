@@ -189,3 +189,37 @@ def test_no_rows_and_no_addresses(hip, suffix):
         loss = hip.call(name + suffix, md, *none, 0.2, 0.2, 0.1, *rest, Out(1, "f32"), Null(), Null(), *([Null()] if rest else []))[0]
         assert loss[0] == 0
     hip.call("policy_loss_backward_" + suffix, md, *none, 0.2, 0.2, 0.1, Null(), Null(), Null(), Null())
+
+
+TOP = {"f32": float(np.finfo(np.float32).max), "bf16": 3.3895313892515355e38, "f16": 65504.0}
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("rows,vocab", [(30, 7), (30, 200), (3, 9000), (260, 33001), (258, 70000)])
+@pytest.mark.parametrize("what", ["lowest", "highest", "both", "one"])
+def test_logits_at_the_limits(hip, dt, rows, vocab, what):
+    """Rows of nothing but the type's lowest value or its highest, with the lowest in between, or with a single highest one.  What is
+    left of x - max is 0 or beyond any exponent: the bounds are those of the same rows with 0 and -200 in their place (whose
+    exponentials are zero in f32); lse is the row's largest logit more, to a rounding of its own."""
+    p, q = Policy(dt, rows, vocab, seed=14, share=1.0, spread=0.0), Policy(dt, rows, vocab, seed=14, share=1.0, spread=0.0)
+    r, top = np.random.default_rng(14), TOP[dt]
+    low = np.zeros((rows, vocab), bool)
+    if what == "both":
+        low = r.random((rows, vocab)) < 0.5
+    if what == "one":
+        low[:] = True
+    low[np.arange(rows), p.target] = False
+    q.x = np.where(low, -200.0, 0.0)
+    p.x = np.where(low, -top, -top if what == "lowest" else top)
+    lp = -q.log_sum(q.x)
+    p.old = q.old = (lp - 0.1).astype(np.float32)
+    p.ref = q.ref = (lp + 0.1).astype(np.float32)
+    want, bound = q.exact()
+    bound["lse"] = bound["lse"] + np.abs(p.x).max() * 2.0 ** -23
+    want["lse"] = want["lse"] + p.x.max(1)
+    loss, logp, lse = p.forward(hip)
+    for name, got in (("loss", loss), ("logp", logp), ("lse", lse)):
+        p.close(got, want[name], bound[name], "forward " + name)
+    p.close(p.backward(hip, logp, lse), want["grad"], bound["grad"], "backward")
+    for name, got in zip(("loss", "logp", "lse", "grad"), p.step(hip)):
+        p.close(got, want[name], bound[name], "step " + name)
