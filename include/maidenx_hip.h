@@ -670,7 +670,8 @@ void hip_softmax_f64(size_t num_els, size_t num_dims, size_t dim, const size_t* 
  * bias: NULL, or a learned table [buckets, heads], contiguous (buckets 2 .. 256, buckets / 2 < max_distance <= 4096): with
  *   E = buckets / 2, distance n has bucket n below E, else min(buckets - 1, E + floor((buckets - E) * ln(n / E) /
  *   ln(max_distance / E))), exactly.  -inf takes a pair out; a row whose pairs are all out has an output of zeros and
- *   lse = -inf, and gives no gradient.  Any finite bias is a bias.
+ *   lse = -inf, and gives no gradient.  Any finite bias is a bias, the type's lowest value too: where it drowns q . k, a row
+ *   with nothing else in view spreads evenly over its keys, forward and backward.
  * scale: any value, zero and negative ones included.  dim: 1 .. 128.
  * Without tokens or sequences there is nothing to do but to zero grad_bias; with tokens = 0 the tensors' addresses may be NULL.
  * output [tokens, heads, dim] and lse [heads, tokens] (f32) are contiguous.  Rows of tokens that no sequence holds are

@@ -37,11 +37,11 @@ constexpr int ATTN_MAX_DISTANCE = 4096;
 constexpr int ATTN_THREADS = 256, ATTN_WAVES = ATTN_THREADS / WAVE;
 constexpr int ATTN_ROWS = 128;              // rows (of queries, or of keys in the backward pass for keys) that a block owns: 32 a wave
 constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
-constexpr float ATTN_FLT_MAX = 3.402823466e+38f;
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef float f32x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -63,10 +63,11 @@ struct AttnArgs {
     const E* table;            // [buckets, heads], null: no bias
     int32_t tokens, heads, group, dim, sequences;
     int32_t buckets, exact_to, max_distance;
-    float scale, scale_log2;   // scale_log2 = |scale| * log2(e); the sign goes into an operand
+    float scale, scale_abs, scale_log2;   // scale_log2 = |scale| * log2(e); the sign goes into an operand
     E *out, *gq, *gk, *gv;
     float *lse, *partial;
     float* stats;              // [heads, tokens]: (lse in units of log2, D)
+    float* near_stats;         // with a bias, [heads, tokens]: (lse, log2 of what the row of P sums to with that lse)
     float *part_k, *part_v;    // with more than one part: [parts][tokens, kv_heads, dim] sums in f32
     int32_t head_parts, query_parts, partial_tiles;
     int* flag;
@@ -345,19 +346,17 @@ __device__ inline int attn_bucket(const AttnArgs<E>& a, int distance) {
     for (int m = 0; m < a.buckets - a.exact_to - 1; ++m) b += distance >= (int)a.borders[m];
     return b;
 }
-// in units of log2; a finite bias stays finite: the type's lowest value is a value like any other, only -inf takes a pair out
 template <class E>
-__device__ inline float attn_bias(const AttnArgs<E>& a, int head, int bucket) {
-    const float b = AttnType<E>::get(a.table[(int64_t)bucket * a.heads + head]), x = b * ATTN_LOG2E;
-    return __builtin_isinf(b) ? b : x > ATTN_FLT_MAX ? ATTN_FLT_MAX : x < -ATTN_FLT_MAX ? -ATTN_FLT_MAX : x;
-}
+__device__ inline float attn_bias(const AttnArgs<E>& a, int head, int bucket) { return AttnType<E>::get(a.table[(int64_t)bucket * a.heads + head]); }
 // by_distance[n], n = 0 .. max_distance: the bias of a head, the last for every distance from max_distance on
 template <class E>
 __device__ inline void attn_bias_by_distance(const AttnArgs<E>& a, int head, float* by_distance, int tid, int threads) {
     for (int n = tid; n <= a.max_distance; n += threads) by_distance[n] = attn_bias(a, head, attn_bucket(a, n));
 }
 // Every distance from max_distance on has one bias: a tile of such pairs starts its product there (in units of the product),
-// and costs nothing.  Where that cannot be represented - a bias near the type's limits - the tile goes the way of a near one.
+// and costs nothing.  A bias is any finite number, the type's lowest value among them, and rows may hold nothing else: there q . k is
+// lost beside it, and what decides is that equal scores stay equal.  So a large one goes the way of a near tile, where scores
+// are formed as they are defined, and the maximum and lse with them: only their differences are brought to units of log2.
 // how many of n tiles, a step apart, lie at `room` or before it, the first lying at 0
 __device__ __forceinline__ int attn_tiles_beyond(int room, int step, int n) {
     const int fit = room < 0 ? 0 : room / step + 1;
@@ -366,16 +365,17 @@ __device__ __forceinline__ int attn_tiles_beyond(int room, int step, int n) {
 struct AttnFar {
     float start;
     bool apart;
-    __device__ __forceinline__ AttnFar(float bias, float c) : start(bias / c), apart(!(__builtin_fabsf(bias) < 1e30f * c) && bias != -INFINITY) {}
+    __device__ __forceinline__ AttnFar(float bias, float scale)
+        : start(bias / scale), apart(!(__builtin_fabsf(bias) < 1024.0f && __builtin_fabsf(bias) < 1e30f * scale) && bias != -INFINITY) {}
 };
-// The scores, in units of log2, that a lane holds at distances d0 - (r % 4) - 8 (r / 4), times STEP (1: rows are keys, -1: queries)
+// The scores that a lane holds at distances d0 - (r % 4) - 8 (r / 4), times STEP (1: rows are keys, -1: queries)
 template <int STEP>
-__device__ inline void attn_add_bias(f32x16_t& s, float c, const float* by_distance, int d0, int max_distance) {
+__device__ inline void attn_add_bias(f32x16_t& s, float scale, const float* by_distance, int d0, int max_distance) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         int n = d0 - STEP * ((r & 3) + 8 * (r >> 2));
         n = n < 0 ? 0 : n > max_distance ? max_distance : n;
-        s[r] = __builtin_fmaf(s[r], c, by_distance[n]);
+        s[r] = __builtin_fmaf(s[r], scale, by_distance[n]);
     }
 }
 __device__ inline f32x16_t attn_start(float x) {
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     typename T::Frag q[KS];
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
-    const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_log2);
+    const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_abs);
 
     const int lower = there ? first : -1;           // key j is seen if (unsigned)(j - lower) <= reach
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
@@ -633,6 +633,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     f32x16_t acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
+    constexpr float UNIT = BIAS ? ATTN_LOG2E : 1.0f;          // of the maximum: as scores are with a bias, else of log2
     float m = -INFINITY, l = 0.0f;
     auto step = [&](auto kind_, int round, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(kind_)::value == ATTN_MASKED;
@@ -657,9 +658,8 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
         const int j = j0 + 4 * half;                // key of row 0 of the lane's results
         if (BIAS && near) {
 #pragma unroll
-            for (int b = 0; b < JB; ++b) attn_add_bias<1>(s[b], c, by_distance, row - j - 32 * b, a.max_distance);
+            for (int b = 0; b < JB; ++b) attn_add_bias<1>(s[b], a.scale_abs, by_distance, row - j - 32 * b, a.max_distance);
         }
-        const float cc = BIAS && near ? 1.0f : c;   // what is left to multiply the scores by
         if constexpr (MASKED) {
 #pragma unroll
             for (int b = 0; b < JB; ++b)
@@ -673,20 +673,32 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
 #pragma unroll
             for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
         best = fmaxf(best, attn_other_half(best));
-        best *= cc;
-        if (__any(best > m + ATTN_BEHIND)) {
-            const float next = fmaxf(m, best), fix = next == -INFINITY ? 1.0f : attn_exp2(m - next);
+        best *= BIAS ? near ? 1.0f : a.scale_abs : c;
+        if (__any(best > m + ATTN_BEHIND / UNIT)) {
+            const float next = fmaxf(m, best), fix = next == -INFINITY ? 1.0f : attn_exp2((m - next) * UNIT);
             l *= fix;
 #pragma unroll
             for (int d = 0; d < DB; ++d) acc[d] *= fix;
             m = next;
         }
         const float base = m == -INFINITY ? 0.0f : m;
+        if (BIAS && near) {
+#pragma unroll
+            for (int b = 0; b < JB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = (s[b][r] - base) * ATTN_LOG2E;
+        } else {
+            const float base2 = base * UNIT;
+#pragma unroll
+            for (int b = 0; b < JB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = __builtin_fmaf(s[b][r], c, -base2);
+        }
 #pragma unroll
         for (int b = 0; b < JB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[b][r] = attn_exp2(__builtin_fmaf(s[b][r], cc, -base));
+                s[b][r] = attn_exp2(s[b][r]);
                 l += s[b][r];
             }
         if (MASKED && terms) {
@@ -706,7 +718,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
         for (int g = 1; g < KG; ++g) {
             const float* const from = left + ((g - 1) * RG + wave) * attn_left<DB>();
             const float m2 = from[DB * 1024 + lane], l2 = from[DB * 1024 + 64 + lane], next = fmaxf(m, m2);
-            const float by = next == -INFINITY ? 1.0f : attn_exp2(m - next), by2 = next == -INFINITY ? 1.0f : attn_exp2(m2 - next);
+            const float by = next == -INFINITY ? 1.0f : attn_exp2((m - next) * UNIT), by2 = next == -INFINITY ? 1.0f : attn_exp2((m2 - next) * UNIT);
             attn_take<DB>(from, acc, by, by2, lane);
             l = __builtin_fmaf(l2, by2, l * by);
             m = next;
@@ -715,7 +727,8 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     l += attn_other_half(l);
     if (!there) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;       // nothing but -inf: an output of zeros
-    if (half == 0) a.lse[(int64_t)head * a.tokens + row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * ATTN_LN2;
+    const float log_l = __builtin_amdgcn_logf(l);
+    if (half == 0) a.lse[(int64_t)head * a.tokens + row] = l == 0.0f ? -INFINITY : BIAS ? __builtin_fmaf(log_l, ATTN_LN2, m) : (m + log_l) * ATTN_LN2;
     attn_write_row<E, DP>(a.out + ((int64_t)row * a.heads + head) * a.dim, acc, inv, a.dim, half, attn_whole(a.out, a.dim));
 }
 
@@ -727,6 +740,39 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
 // The sum, the rows of q and those of do take 128 registers at 128 elements a head.  With 64 keys to a tile the rest does not suffice (a
 // register more than there are is read from memory, behind every tile on its way): 8192 tokens, 16 heads with a bias 313 us, with 32
 // keys 212.
+//
+// With a bias, scores and lse may be so large that lse has lost the logarithm of the sum to its rounding (masks by large negative numbers:
+// the row of P would sum to the number of its keys).  Beyond ATTN_ROUGH - 2^8 2^-24 = 2^-16 - a wave forms that sum first, keys straight
+// from memory: seldom, and slowly.
+constexpr float ATTN_ROUGH = 256.0f;
+template <class E, int DP>
+__device__ inline float attn_row_sum(const AttnArgs<E>& a, int head, int kv, int row, int lane, const AttnSpan& own, int lower, uint32_t reach, float lse,
+                                     const typename AttnType<E>::Frag (&q)[DP / 16]) {
+    float z = 0.0f;
+#pragma nounroll
+    for (int j0 = own.lo; j0 < own.hi; j0 += 32) {
+        const int j = j0 + (lane & 31) < own.hi ? j0 + (lane & 31) : j0;
+        const E* const from = a.k.p + (int64_t)kv * a.k.head + (int64_t)j * a.k.token;
+        f32x16_t s = {};
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+            u32x4_t part[sizeof(E) / 2];
+            for (int c = 0; c < (int)sizeof(E) / 2; ++c) part[c] = attn_piece<E>(from, 16 * x + 8 * (lane >> 5) + c * AttnType<E>::CHUNK, a.dim, a.k.elem, a.k.vec);
+            s = AttnType<E>::mma(__builtin_bit_cast(typename AttnType<E>::Frag, part), q[x], s);
+            __builtin_amdgcn_sched_barrier(0);       // a few registers at a time
+        }
+        float mine[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mine[r] = s[r];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int key = j0 + 4 * (lane >> 5) + (r & 3) + 8 * (r >> 2);
+            if ((uint32_t)(key - lower) <= reach) z += attn_exp2((__builtin_fmaf(mine[r], a.scale_abs, attn_bias(a, head, attn_bucket(a, row - key))) - lse) * ATTN_LOG2E);
+        }
+    }
+    z += attn_other_half(z);
+    return z > 0.0f ? z : 1.0f;      // (nothing in view, or NaN)
+}
 template <class E, int DP, int KG> constexpr int attn_grad_keys() { return sizeof(E) == 2 && DP > 96 ? 32 : attn_keys<E, DP, KG>(); }
 template <class E, int DP, bool BIAS, int KG>
 __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && DP > 64 ? 1 : 2) void attn_grad_query_kernel(const AttnArgs<E> a, int tiles, int stages) {
@@ -779,7 +825,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     if (walks) ring.begin(rounds.total, fetch);
     typename T::Frag q[KS], go[KS];
     attn_own_rows<E, DP>(a.go, head, there ? row : 0, there, a.dim, lane, 1.0f, go);
-    float delta = 0.0f, lse2 = INFINITY;
+    float delta = 0.0f, lse = INFINITY;
     {
         attn_own_rows<E, DP>(a.o, head, there ? row : 0, there, a.dim, lane, 1.0f, q);
 #pragma unroll
@@ -789,20 +835,29 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
         delta += attn_other_half(delta);
     }
     if (there) {
-        const float x = a.lse[(int64_t)head * a.tokens + row];
-        lse2 = x == -INFINITY ? INFINITY : x * ATTN_LOG2E;       // a row of nothing but -inf: P is zero
+        lse = a.lse[(int64_t)head * a.tokens + row];
+        if (lse == -INFINITY) lse = INFINITY;                    // a row of nothing but -inf: P is zero
     }
     float* const stat = a.stats + ((int64_t)head * a.tokens + row) * 2;
     if (!walks) {
-        if (there && half == 0 && group == 0) { stat[0] = lse2; stat[1] = delta; }
+        if (there && half == 0 && group == 0) { stat[0] = lse * ATTN_LOG2E; stat[1] = delta; }      // (never with a bias: the gradient of the values alone wants no D)
         return;
     }
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
     if (BIAS) attn_bias_by_distance(a, head, by_distance, tid, 64 * RG * KG);
-    const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_log2);
+    const AttnFar far(BIAS ? attn_bias(a, head, a.buckets - 1) : 0.0f, a.scale_abs);
     const int lower = there ? first : -1;
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
     const float c = a.scale_log2;
+    const int64_t to_near = BIAS ? a.near_stats - a.stats : 0;
+    if constexpr (BIAS) {                 // (kept in memory over the walk, where registers are scarce; both halves and all groups write the same)
+        float z = 1.0f;
+        if (__any(__builtin_fabsf(lse) > ATTN_ROUGH && lse != INFINITY)) z = attn_row_sum<E, DP>(a, head, kv, row, lane, own, lower, reach, lse, q);
+        if (there) {
+            stat[to_near] = lse;
+            stat[to_near + 1] = __builtin_amdgcn_logf(z);
+        }
+    }
     f32x16_t acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
@@ -820,7 +875,6 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
             if (idle || j0 >= own.hi || j0 + BN <= own.lo) return;
         }
         const bool near = BIAS && (far.apart || row0 - (j0 + BN - 1) < a.max_distance);
-        const float cc = BIAS && near ? 1.0f : c;
 #pragma unroll
         for (int b = 0; b < JB; ++b) {
             f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
@@ -829,10 +883,18 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
 #pragma unroll
             for (int k = 0; k < KS; ++k) dp = T::mma(L::rows(attn_in_lds(vt), at, 32 * b, k), go[k], dp);
             const int j = j0 + 32 * b + 4 * half;
-            if (BIAS && near) attn_add_bias<1>(s, c, by_distance, row - j, a.max_distance);
+            if (BIAS && near) {
+                attn_add_bias<1>(s, a.scale_abs, by_distance, row - j, a.max_distance);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = (s[r] - lse) * ATTN_LOG2E;
+            } else {
+                const float lse2 = lse * ATTN_LOG2E;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, -lse2);
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[r] = attn_exp2(__builtin_fmaf(s[r], cc, -lse2));
+                s[r] = attn_exp2(s[r]);
                 s[r] *= dp[r] - delta;
                 if (MASKED && (uint32_t)(j + (r & 3) + 8 * (r >> 2) - lower) > reach) s[r] = 0.0f;
                 if (BIAS) rest += s[r];
@@ -860,8 +922,9 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     }
     if (BIAS) rest += attn_other_half(rest);
     if (!there) return;
-    if (half == 0) { stat[0] = lse2; stat[1] = BIAS ? delta + rest : delta; }
-    if (a.gq) attn_write_row<E, DP>(a.gq + ((int64_t)row * a.heads + head) * a.dim, acc, a.scale, a.dim, half, attn_whole(a.gq, a.dim));
+    const float log_z = BIAS ? *(const volatile float*)(stat + to_near + 1) : 0.0f, inv = BIAS ? attn_exp2(-log_z) : 1.0f;
+    if (half == 0) { stat[0] = __builtin_fmaf(lse, ATTN_LOG2E, log_z); stat[1] = BIAS ? __builtin_fmaf(rest, inv, delta) : delta; }
+    if (a.gq) attn_write_row<E, DP>(a.gq + ((int64_t)row * a.heads + head) * a.dim, acc, a.scale * inv, a.dim, half, attn_whole(a.gq, a.dim));
 }
 
 // ---- backward: gradients of the keys, the values and the bias table ----------------------------------------------------------
@@ -874,12 +937,15 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
 // 413 us = 535 TFLOP/s; of 64, with two waves, 218 us = 508).  Two waves that share the work, one for each sum and both making P, take
 // 406, and more for the bias; the values in LDS, 475.
 __host__ __device__ inline int attn_corner(int max_distance) { return 16 * 33 + max_distance + 63; }      // floats of a wave
+// Statistics of the 32 rows of a tile: 256 bytes for (lse2, D), 256 for (lse, log2 of the row's sum), which a bias wants.  Every wave
+// brings one of the two, 4 bytes a lane: that some bring the same keeps the count of loads alike.
+constexpr int ATTN_STATS = 512;
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH, PER = 2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1;
-    constexpr int PLACE = 2 * BYTES + ATTN_WAVES * 8 * BM;       // queries, gradients of the output, and a copy of their statistics for each wave
+    constexpr int PLACE = 2 * BYTES + ATTN_STATS;                // queries, gradients of the output, and their statistics
     extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -915,18 +981,18 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     const int plain = qs.plainly(a.q, a.dim) && os.plainly(a.go, a.dim) ? walk.nclean : 0;
     const int64_t to_next_q = (int64_t)BM * a.q.token, to_next_o = (int64_t)BM * a.go.token;
     const E *next_q, *next_o;
-    const float* next_s;
+    const float *const stats = BIAS && (wave & 1) ? a.near_stats : a.stats, *next_s;
     int next_head = head0, next = from;
     auto at_next = [&]() __attribute__((always_inline)) {
         const int64_t i0 = walk.at(next);
         next_q = a.q.p + (int64_t)next_head * a.q.head + i0 * a.q.token;
         next_o = a.go.p + (int64_t)next_head * a.go.head + i0 * a.go.token;
-        next_s = a.stats + ((int64_t)next_head * a.tokens + i0) * 2;
+        next_s = stats + ((int64_t)next_head * a.tokens + i0) * 2;
     };
     at_next();
     auto fetch = [&](int place) __attribute__((always_inline)) {
         char* const to = lds + place * PLACE;
-        const uint32_t stat = attn_in_lds(to) + 2 * BYTES + wave * 8 * BM;
+        const uint32_t stat = attn_in_lds(to) + 2 * BYTES + (BIAS ? wave & 1 : 0) * 8 * BM;
         if (next < plain) {
             qs.plain(a.q, next_q, attn_in_lds(to), wave);
             os.plain(a.go, next_o, attn_in_lds(to) + BYTES, wave);
@@ -939,7 +1005,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             qs.load(a.q, next_head, i0, all.hi, a.dim, to, wave, lane);
             os.load(a.go, next_head, i0, all.hi, a.dim, to + BYTES, wave, lane);
             const int i = i0 + (lane >> 1), in = i < all.hi ? i : all.hi - 1;
-            attn_load_lds<4>(a.stats + ((int64_t)next_head * a.tokens + i0) * 2, (uint32_t)((in - i0) * 8 + (lane & 1) * 4), stat);
+            attn_load_lds<4>(stats + ((int64_t)next_head * a.tokens + i0) * 2, (uint32_t)((in - i0) * 8 + (lane & 1) * 4), stat);
         }
         if (++next == upto) {
             next = from;
@@ -966,7 +1032,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         constexpr bool MASKED = decltype(kind_)::value == ATTN_MASKED, NEAR = BIAS && decltype(kind_)::value != ATTN_FAR;
         char* const here = lds + place * PLACE;
         const uint32_t qt = attn_in_lds(here), ot = qt + BYTES;
-        const float* const st = (const float*)(here + 2 * BYTES) + wave * 2 * BM;      // (lse2, D) of each row
+        const float* const st = (const float*)(here + 2 * BYTES);       // (lse2, D) of each row
         const int i0 = walk.at(n), i = i0 + 4 * half;
         bool terms = false;
         if constexpr (MASKED) {
@@ -974,13 +1040,20 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             if (i0 >= own.hi || i0 + BM <= own.lo) return;
         }
         const bool near = NEAR && (far.apart || i0 - (key0 + 31) < a.max_distance);
-        const float cc = near ? 1.0f : c;
         f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
 #pragma unroll
         for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, at, 0, x), k[x], s);
 #pragma unroll
         for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, at, 0, x), v[x], dp);
-        if (NEAR && near) attn_add_bias<-1>(s, c, by_distance, i - key, a.max_distance);
+        if (NEAR && near) {                    // (a row's exponents as they are to be: nothing is taken from them below)
+            attn_add_bias<-1>(s, a.scale_abs, by_distance, i - key, a.max_distance);
+            const float* const near_st = st + 2 * BM;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const f32x2_t x = *(const f32x2_t*)(near_st + 2 * ((r & 3) + 8 * (r >> 2) + 4 * half));
+                s[r] = __builtin_fmaf(s[r] - x[0], ATTN_LOG2E, -x[1]);
+            }
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f32x4_t st01 = *(const f32x4_t*)(st + 16 * g + 8 * half), st23 = *(const f32x4_t*)(st + 16 * g + 8 * half + 4);
@@ -989,7 +1062,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
                 const int r = 4 * g + e;
                 const float ls = e < 2 ? st01[2 * e] : st23[2 * e - 4], de = e < 2 ? st01[2 * e + 1] : st23[2 * e - 3];
                 const bool hidden = MASKED && (uint32_t)(i + e + 8 * g - key) >= reach;
-                const float p = attn_exp2(__builtin_fmaf(s[r], cc, -ls));
+                const float p = attn_exp2(NEAR && near ? s[r] : __builtin_fmaf(s[r], c, -ls));
                 s[r] = hidden ? 0.0f : p;
                 dp[r] = hidden ? 0.0f : p * (dp[r] - de);
             }
@@ -1033,7 +1106,7 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         if (BIAS) {
             __syncthreads();                    // the table of the head before is not read any more
             attn_bias_by_distance(a, head0 + g, by_distance, tid, ATTN_THREADS);
-            far = AttnFar(attn_bias(a, head0 + g, a.buckets - 1), c);
+            far = AttnFar(attn_bias(a, head0 + g, a.buckets - 1), a.scale_abs);
             if (sums)
                 for (int n = lane; n < a.max_distance + 63; n += WAVE) on_distance[n] = 0.0f;
         }
@@ -1150,7 +1223,8 @@ inline bool attn_arguments(AttnArgs<E>& a, const size_t* md, const int32_t* offs
     a.dim = (int32_t)dim;
     a.sequences = (int32_t)sequences;
     a.scale = scale;
-    a.scale_log2 = (scale == 0.0f ? 1.0f : std::fabs(scale)) * ATTN_LOG2E;
+    a.scale_abs = scale == 0.0f ? 1.0f : std::fabs(scale);
+    a.scale_log2 = a.scale_abs * ATTN_LOG2E;
     if (table) {
         const size_t buckets = md[5], distance = md[6];
         if (buckets < 2 || buckets > (size_t)ATTN_MAX_BUCKETS) { set_status(ERR_UNSUPPORTED, "attention: a bias takes 2 to 256 buckets"); return false; }
@@ -1238,7 +1312,7 @@ inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
     const size_t bias = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
     attn_query_launch<E, DP, BIAS>(a);
     if (a.gk || a.gv || grad_table) {
-        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_WAVES * 8 * 32, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
+        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_STATS, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
         const int parts = a.head_parts * a.query_parts;
         const unsigned blocks = (unsigned)(tiles * kv * parts);
         const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && DP <= 64 && blocks > 256 ? 2 : 1);
@@ -1315,9 +1389,10 @@ inline void attention_backward_entry(const size_t* md, const int32_t* offsets, c
     const size_t stats = ((size_t)a.heads * a.tokens * 2 + 63) / 64 * 64, sums = parts > 1 ? ((size_t)a.tokens * kv * a.dim + 63) / 64 * 64 * parts : 0;
     a.partial_tiles = (int)(ATTN_WAVES * tiles) * a.query_parts;
     const size_t partials = grad_table ? (size_t)a.heads * a.partial_tiles * a.buckets : 0;
-    a.stats = (float*)scratch((stats + 2 * sums + partials) * sizeof(float));
+    a.stats = (float*)scratch((stats * (table ? 2 : 1) + 2 * sums + partials) * sizeof(float));
     if (!a.stats) return;
-    a.part_k = a.stats + stats;
+    a.near_stats = a.stats + (table ? stats : 0);
+    a.part_k = a.near_stats + stats;
     a.part_v = a.part_k + sums;
     a.partial = grad_table ? a.part_v + sums : nullptr;
     attn_by_dim(a, [&](auto dp) {

@@ -4,7 +4,7 @@ import pytest
 
 import maidenx_amd.lib as L
 from helpers import to_float, to_storage
-from language import Attention, borders
+from language import E32, UNIT, Attention, borders, bucket_of
 
 pytestmark = pytest.mark.gpu
 ALL = ["f32", "bf16", "f16"]
@@ -370,3 +370,73 @@ def test_no_tokens(dt, sequences):
     code = FIRST_CALL.format(paths=[ROOT, ROOT + "/tests"], sequences=sequences, dt=dt, np="float32" if dt == "f32" else "uint16")
     p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert p.returncode == 0 and "zeros" in p.stdout, p.stderr[-2000:]
+
+
+def uniform_rows(a, rows_of, u, e):
+    """Gradients of rows whose scores are all equal (P = 1 / n), for the rows of a sequence that rows_of(n) names, with bounds: P comes
+    from an exponential of zero and a sum of ones (a few e), dP and D are sums of dim and n terms, D with o as it was rounded (u), dS is
+    rounded to the tensors' type (u), and so is each result."""
+    t, h, g, d = a.tokens, a.heads, a.kv, a.dim
+    group, s = h // g, abs(a.scale)
+    out, lse = np.full((t, h, d), np.nan), np.full((h, t), np.nan)
+    r = {"gq": np.zeros((t, h, d)), "gk": np.zeros((t, g, d)), "gv": np.zeros((t, g, d)), "gt": np.zeros((a.buckets, h))}
+    b = {n: np.zeros_like(x) for n, x in r.items()}
+    ob = np.zeros((t, h, d))
+    for first, last in zip(a.offsets[:-1], a.offsets[1:]):
+        for n in rows_of(last - first):                      # keys that the row sees
+            i, r_ = first + n - 1, slice(first, first + n)
+            bucket = bucket_of(np.arange(n)[::-1], a.buckets, a.distance)
+            for x in range(h):
+                k, v, q, go = a.k[r_, x // group], a.v[r_, x // group], a.q[i, x], a.go[i, x]
+                o, dp = v.mean(0), v @ go
+                ds = (dp - dp.mean()) / n
+                out[i, x], lse[x, i] = o, np.log(n)
+                ob[i, x] = (2 * u + e * (n + 16)) * np.abs(v).mean(0)
+                off = ((np.abs(v) @ np.abs(go)) * (u + e * (n + d + 16)) * 2 + (2 * u + e * (n + d + 16)) * (np.abs(v) @ np.abs(go)).mean()) / n
+                r["gq"][i, x] = a.scale * (ds @ k)
+                b["gq"][i, x] = s * (off @ np.abs(k)) + u * np.abs(r["gq"][i, x])
+                r["gk"][r_, x // group] += a.scale * ds[:, None] * q
+                b["gk"][r_, x // group] += s * off[:, None] * np.abs(q)
+                r["gv"][r_, x // group] += go / n
+                b["gv"][r_, x // group] += (u + e * (n + 16)) * np.abs(go) / n
+                np.add.at(r["gt"][:, x], bucket, ds)
+                np.add.at(b["gt"][:, x], bucket, off)
+    return out, ob, lse, r, b
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,dim", [(4, 32), (4, 128), (40, 64), (90, 128), (90, 96)])
+@pytest.mark.parametrize("which,value", [("near", -2.0 ** 31), ("near", "lowest"), ("all", -2.0 ** 31), ("all", "lowest"), ("all", 2.0 ** 40)])
+def test_rows_of_one_large_bias(hip, dt, value, heads, dim, which):
+    """A bias so large that q . k is lost beside it, on the first four distances or on all of them: rows with nothing else in view spread
+    evenly, forward and backward; the others see the rest as if those pairs were out."""
+    value = {"f32": -float(np.finfo(np.float32).max), "bf16": -3.3895313892515355e38}[dt] if value == "lowest" else value
+    u, e = UNIT[dt], E32
+    a = Attention(dt, [330, 3, 90], heads, heads // 2, dim, buckets=8, distance=16, seed=33)
+    near = slice(0, 4) if which == "near" else slice(0, 8)
+    a.table[near] = -np.inf
+    want, bound = a.exact()                                  # of the rows that see more (none where all are masked)
+    a.table[near] = value
+    rows_of = (lambda n: range(1, min(4, n) + 1)) if which == "near" else (lambda n: range(1, n + 1))
+    o, ob, lse_n, r, b = uniform_rows(a, rows_of, u, e)
+    even = ~np.isnan(o[:, 0, 0])
+    want["o"][even], bound["o"][even] = o[even], ob[even]
+    want["lse"][:, even], bound["lse"][:, even] = value + lse_n[:, even], abs(value) * 2.0 ** -23
+    for n in r:
+        want[n] = want[n] + r[n]
+        bound[n] = bound[n] + b[n] + 2 * u * np.abs(r[n])
+    out, lse = a.forward(hip)
+    a.close(out, want["o"], bound["o"], "output")
+    a.close(lse, want["lse"], bound["lse"], "lse")
+    for name, got in zip(("gq", "gk", "gv", "gt"), a.backward(hip, out, lse)):
+        a.close(got, want[name], bound[name], name)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("size", [300.0, 2.0e4])
+@pytest.mark.parametrize("heads,dim", [(4, 64), (40, 128), (90, 32)])
+def test_large_biases(hip, dt, size, heads, dim):
+    """Biases of some hundreds to the reach of f16, of either sign, beside each other."""
+    a = Attention(dt, [400, 90], heads, heads // 2, dim, buckets=16, distance=64, seed=34)
+    a.table[:] = to_float(to_storage(size * a.table, dt), dt)
+    a.check(hip)
