@@ -677,7 +677,8 @@ void hip_softmax_f64(size_t num_els, size_t num_dims, size_t dim, const size_t* 
  * output [tokens, heads, dim] and lse [heads, tokens] (f32) are contiguous.  Rows of tokens that no sequence holds are
  *   not written, here and in the gradients.  Outputs must not overlap inputs.
  * Scores, statistics and sums are f32; P (and dS in the backward pass) are rounded to the tensors' type where they enter a
- * product, results once.  Same bits on every call.
+ * product (f16: scaled by a power of two first, so that output gradients of any size may be given), results once.  Same bits
+ * on every call.
  * backward: grad_output [tokens, heads, dim] contiguous; output and lse as the forward call wrote them; each of
  *   grad_query [tokens, heads, dim], grad_key and grad_value [tokens, kv_heads, dim] (contiguous; sums over the heads that share
  *   a key head) and grad_bias [buckets, heads] may be NULL. */

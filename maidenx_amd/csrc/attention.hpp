@@ -19,8 +19,10 @@
 // touches skip it, and a batch of short sequences fills its tiles.
 //
 // Rounding: scores, statistics and every accumulator are f32.  P and dS are rounded to the tensors' type where they become an
-// operand of the matrix cores (bf16 and f16; f32 tensors keep f32 there): the error is that of one more rounding of
-// every term, independent from term to term, and the sum over terms is as far off as the rounding of the result itself.
+// operand of the matrix cores (bf16 and f16; f32 tensors keep f32 there): a term t of a sum is then off by u |t| at most (u = 2^-8, 2^-11),
+// the sum by u times the sum of the |t|, and by about u times the root of the sum of their squares, the roundings being independent; the
+// result's own rounding is u times the sum.  Against 64 bits that makes 1.3 times (output) and 1.5 times (gradients) the error
+// of the same formulas with P and dS in f32.  What f16 cannot hold of dS is scaled by powers of two (AttnLift).
 #pragma once
 #include <cmath>
 #include <cstring>
@@ -66,8 +68,11 @@ struct AttnArgs {
     float scale, scale_abs, scale_log2;   // scale_log2 = |scale| * log2(e); the sign goes into an operand
     E *out, *gq, *gk, *gv;
     float *lse, *partial;
-    float* stats;              // [heads, tokens]: (lse in units of log2, D)
-    float* near_stats;         // with a bias, [heads, tokens]: (lse, log2 of what the row of P sums to with that lse)
+    // Of the rows, for the kernel of the keys: [heads, tokens] of each, stat_size apart: lse in units of log2, with the logarithm of what the row
+    // of P sums to; -D; and with a bias lse as it is, and that logarithm.  (f16: both less 14, so that P comes times 2^14.)
+    float* stats;
+    int64_t stat_size;
+    int32_t* lifts;            // f16, [heads, tokens / 32, 4]: the power of two that dS of 32 rows was held by, of each group of waves
     float *part_k, *part_v;    // with more than one part: [parts][tokens, kv_heads, dim] sums in f32
     int32_t head_parts, query_parts, partial_tiles;
     int* flag;
@@ -512,6 +517,66 @@ __device__ __forceinline__ AttnSpan attn_span_of_block(const AttnSpan& own, int*
     return all;
 }
 
+// f16 has no room for dS as it comes: a loss that is scaled up takes it beyond 65504, a mean over many tokens below 2^-24, long before the
+// gradients leave the type.  A wave holds it, and the sum it goes into, times 2^-e: the first values that are not zero come to lie
+// around 2^10, and e grows when some reach 2^15.  What gets lost in subnormals is 2^-35 of the largest.  The kernel of the queries finds e as
+// it goes and leaves it for the kernel of the keys, which takes the largest of the rows that it walks over.  (P, which is never above one,
+// is held times 2^14 there.)  8192 tokens, 16 heads: the kernel of the queries 130 -> 139 us at 64 elements, 205 -> 209 at 128, that of the
+// keys 233 -> 247 and 466 -> 470; with e found in both, 272 and 560.
+template <class E> constexpr bool attn_lifted() { return std::is_same<E, f16_t>::value; }
+template <class E> constexpr int attn_p_up() { return attn_lifted<E>() ? 14 : 0; }
+constexpr int ATTN_NO_LIFT = -1000;         // nothing but zeros
+struct AttnLift {
+    float limit = 0.0f;
+    int e = 0;
+    template <int DB>
+    __device__ __forceinline__ void hold(f32x16_t& s, f32x16_t (&sums)[DB], float& other) {
+        float top = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, __builtin_fabsf(s[r]));
+        if (__any(top > limit)) {
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
+            int up = top < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(top) : 0;      // (what is infinite stays so)
+            up = up < e - 100 ? e - 100 : up > e + 80 ? e + 80 : up;      // (dS is below 2^40: nothing overflows in f32)
+            up = __builtin_amdgcn_readfirstlane(up);
+            const float by = power(up);
+            s *= attn_start(by);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) sums[d] *= attn_start(by);
+            other *= by;
+            e -= up;
+            limit = top < INFINITY ? 32768.0f : INFINITY;
+        }
+    }
+    __device__ static __forceinline__ float power(int n) { return __builtin_ldexpf(1.0f, n); }
+};
+
+// the largest power of the rows of `heads` heads that a block walks over, found by its waves together
+template <class E>
+__device__ __forceinline__ int attn_lift_of_rows(const AttnArgs<E>& a, int head0, int heads, const AttnSpan& all, int* shared, int tid, int lane, int wave) {
+    const int from = all.lo / 32, n = all.hi > all.lo ? (all.hi - 1) / 32 + 1 - from : 0, chunks = (a.tokens + 31) / 32;
+    int e = ATTN_NO_LIFT;
+    for (int x = tid; x < n * heads; x += ATTN_THREADS) {
+        const int h = x / n;
+        const int32_t* const four = a.lifts + ((int64_t)(head0 + h) * chunks + from + x - h * n) * 4;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) e = four[g] > e ? four[g] : e;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const int other = __shfl_xor(e, d, WAVE);
+        e = other > e ? other : e;
+    }
+    __syncthreads();
+    if (lane == 0) shared[wave] = e;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < ATTN_WAVES; ++w) e = shared[w] > e ? shared[w] : e;
+    e = e < -80 ? 0 : e > 100 ? 100 : e;       // (nothing found, or offsets that do not ascend)
+    return __builtin_amdgcn_readfirstlane(e);
+}
+
 // Sums of another group of waves for the same rows, through LDS: `count` registers of a wave, four at a time.
 template <int DB>
 __device__ inline void attn_leave(float* to, const f32x16_t (&sums)[DB], float x, float y, int lane) {
@@ -821,7 +886,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
         }
         ++next;
     };
-    const bool walks = a.gq || (BIAS && (a.gk || a.partial));       // else only D_i is wanted, if that
+    const bool walks = a.gq || (BIAS && (a.gk || a.partial)) || (attn_lifted<E>() && a.gk);       // else only D_i is wanted, if that
     if (walks) ring.begin(rounds.total, fetch);
     typename T::Frag q[KS], go[KS];
     attn_own_rows<E, DP>(a.go, head, there ? row : 0, there, a.dim, lane, 1.0f, go);
@@ -838,9 +903,9 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
         lse = a.lse[(int64_t)head * a.tokens + row];
         if (lse == -INFINITY) lse = INFINITY;                    // a row of nothing but -inf: P is zero
     }
-    float* const stat = a.stats + ((int64_t)head * a.tokens + row) * 2;
+    float* const stat = a.stats + (int64_t)head * a.tokens + row;
     if (!walks) {
-        if (there && half == 0 && group == 0) { stat[0] = lse * ATTN_LOG2E; stat[1] = delta; }      // (never with a bias: the gradient of the values alone wants no D)
+        if (there && half == 0 && group == 0) { stat[0] = lse * ATTN_LOG2E - attn_p_up<E>(); stat[a.stat_size] = -delta; }      // (never with a bias: the gradient of the values alone wants no D)
         return;
     }
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
@@ -849,19 +914,19 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     const int lower = there ? first : -1;
     const uint32_t reach = there ? (uint32_t)(row - first) : 0;
     const float c = a.scale_log2;
-    const int64_t to_near = BIAS ? a.near_stats - a.stats : 0;
     if constexpr (BIAS) {                 // (kept in memory over the walk, where registers are scarce; both halves and all groups write the same)
         float z = 1.0f;
         if (__any(__builtin_fabsf(lse) > ATTN_ROUGH && lse != INFINITY)) z = attn_row_sum<E, DP>(a, head, kv, row, lane, own, lower, reach, lse, q);
         if (there) {
-            stat[to_near] = lse;
-            stat[to_near + 1] = __builtin_amdgcn_logf(z);
+            stat[2 * a.stat_size] = lse;
+            stat[3 * a.stat_size] = __builtin_amdgcn_logf(z) - attn_p_up<E>();
         }
     }
     f32x16_t acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = f32x16_t{};
     float rest = 0.0f;
+    AttnLift lift;
     auto step = [&](auto kind_, int round, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(kind_)::value == ATTN_MASKED;
         const char* const kt = mine + place * 2 * BYTES;
@@ -886,9 +951,9 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
             if (BIAS && near) {
                 attn_add_bias<1>(s, a.scale_abs, by_distance, row - j, a.max_distance);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = (s[r] - lse) * ATTN_LOG2E;
+                for (int r = 0; r < 16; ++r) s[r] = attn_lifted<E>() ? __builtin_fmaf(s[r] - lse, ATTN_LOG2E, -(float)lift.e) : (s[r] - lse) * ATTN_LOG2E;
             } else {
-                const float lse2 = lse * ATTN_LOG2E;
+                const float lse2 = attn_lifted<E>() ? __builtin_fmaf(lse, ATTN_LOG2E, (float)lift.e) : lse * ATTN_LOG2E;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], c, -lse2);
             }
@@ -897,7 +962,13 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
                 s[r] = attn_exp2(s[r]);
                 s[r] *= dp[r] - delta;
                 if (MASKED && (uint32_t)(j + (r & 3) + 8 * (r >> 2) - lower) > reach) s[r] = 0.0f;
-                if (BIAS) rest += s[r];
+                if (BIAS && !attn_lifted<E>()) rest += s[r];
+            }
+            if constexpr (attn_lifted<E>()) {
+                lift.hold(s, acc, rest);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (BIAS) rest += s[r];
             }
             if (MASKED && terms) {
                 const f32x16_t w[1] = {s};
@@ -908,6 +979,14 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
         }
     };
     attn_run_rounds<2 * AttnStage<E, DP, BN, RG>::N>(rounds, ring, fetch, step);
+    if constexpr (attn_lifted<E>()) {
+        if (lane == 0 && row0 < a.tokens)
+            for (int slot = group; slot < 4; slot += KG) a.lifts[((int64_t)head * ((a.tokens + 31) / 32) + row0 / 32) * 4 + slot] = lift.limit == 0.0f ? ATTN_NO_LIFT : lift.e;
+        const float by = AttnLift::power(lift.e);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) acc[d] *= attn_start(by);
+        rest *= by;
+    }
     if constexpr (KG > 1) {
         __syncthreads();
         float* const left = (float*)lds;
@@ -922,8 +1001,8 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     }
     if (BIAS) rest += attn_other_half(rest);
     if (!there) return;
-    const float log_z = BIAS ? *(const volatile float*)(stat + to_near + 1) : 0.0f, inv = BIAS ? attn_exp2(-log_z) : 1.0f;
-    if (half == 0) { stat[0] = __builtin_fmaf(lse, ATTN_LOG2E, log_z); stat[1] = BIAS ? __builtin_fmaf(rest, inv, delta) : delta; }
+    const float log_z = BIAS ? *(const volatile float*)(stat + 3 * a.stat_size) + attn_p_up<E>() : 0.0f, inv = BIAS ? attn_exp2(-log_z) : 1.0f;
+    if (half == 0) { stat[0] = __builtin_fmaf(lse, ATTN_LOG2E, log_z) - attn_p_up<E>(); stat[a.stat_size] = BIAS ? __builtin_fmaf(rest, -inv, -delta) : -delta; }
     if (a.gq) attn_write_row<E, DP>(a.gq + ((int64_t)row * a.heads + head) * a.dim, acc, a.scale * inv, a.dim, half, attn_whole(a.gq, a.dim));
 }
 
@@ -937,15 +1016,16 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
 // 413 us = 535 TFLOP/s; of 64, with two waves, 218 us = 508).  Two waves that share the work, one for each sum and both making P, take
 // 406, and more for the bias; the values in LDS, 475.
 __host__ __device__ inline int attn_corner(int max_distance) { return 16 * 33 + max_distance + 63; }      // floats of a wave
-// Statistics of the 32 rows of a tile: 256 bytes for (lse2, D), 256 for (lse, log2 of the row's sum), which a bias wants.  Every wave
-// brings one of the two, 4 bytes a lane: that some bring the same keeps the count of loads alike.
-constexpr int ATTN_STATS = 512;
+// Statistics of the 32 rows of a tile, two or (with a bias) four of each.  A wave brings one of them, 4 bytes a lane, twice over; where there
+// are two, two waves bring the same: all count the same loads.
+template <bool BIAS> constexpr int attn_stats() { return BIAS ? 4 : 2; }
+constexpr int ATTN_STAT_BYTES = 256;
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) void attn_grad_key_kernel(const AttnArgs<E> a, int tiles, int stages) {
     using T = AttnType<E>;
     using L = AttnTile<E, DP>;
     constexpr int BM = 32, DB = DP / 32, KS = DP / 16, BYTES = BM * L::PITCH, PER = 2 * AttnStage<E, DP, BM, ATTN_WAVES>::N + 1;
-    constexpr int PLACE = 2 * BYTES + ATTN_STATS;                // queries, gradients of the output, and their statistics
+    constexpr int PLACE = 2 * BYTES + attn_stats<BIAS>() * ATTN_STAT_BYTES;      // queries, gradients of the output, and their statistics
     extern __shared__ __attribute__((aligned(512))) char lds[];
     __shared__ int span[16];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -981,31 +1061,32 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
     const int plain = qs.plainly(a.q, a.dim) && os.plainly(a.go, a.dim) ? walk.nclean : 0;
     const int64_t to_next_q = (int64_t)BM * a.q.token, to_next_o = (int64_t)BM * a.go.token;
     const E *next_q, *next_o;
-    const float *const stats = BIAS && (wave & 1) ? a.near_stats : a.stats, *next_s;
+    const int which = wave % attn_stats<BIAS>();
+    const float *const stats = a.stats + which * a.stat_size, *next_s;
     int next_head = head0, next = from;
     auto at_next = [&]() __attribute__((always_inline)) {
         const int64_t i0 = walk.at(next);
         next_q = a.q.p + (int64_t)next_head * a.q.head + i0 * a.q.token;
         next_o = a.go.p + (int64_t)next_head * a.go.head + i0 * a.go.token;
-        next_s = stats + ((int64_t)next_head * a.tokens + i0) * 2;
+        next_s = stats + (int64_t)next_head * a.tokens + i0;
     };
     at_next();
     auto fetch = [&](int place) __attribute__((always_inline)) {
         char* const to = lds + place * PLACE;
-        const uint32_t stat = attn_in_lds(to) + 2 * BYTES + (BIAS ? wave & 1 : 0) * 8 * BM;
+        const uint32_t stat = attn_in_lds(to) + 2 * BYTES + which * ATTN_STAT_BYTES;
         if (next < plain) {
             qs.plain(a.q, next_q, attn_in_lds(to), wave);
             os.plain(a.go, next_o, attn_in_lds(to) + BYTES, wave);
-            attn_load_lds<4>(next_s, attn_lane() * 4, stat);
+            attn_load_lds<4>(next_s, (attn_lane() & 31) * 4, stat);
             next_q += to_next_q;
             next_o += to_next_o;
-            next_s += 2 * BM;
+            next_s += BM;
         } else {
             const int i0 = walk.at(next);
             qs.load(a.q, next_head, i0, all.hi, a.dim, to, wave, lane);
             os.load(a.go, next_head, i0, all.hi, a.dim, to + BYTES, wave, lane);
-            const int i = i0 + (lane >> 1), in = i < all.hi ? i : all.hi - 1;
-            attn_load_lds<4>(stats + ((int64_t)next_head * a.tokens + i0) * 2, (uint32_t)((in - i0) * 8 + (lane & 1) * 4), stat);
+            const int i = i0 + (lane & 31), in = i < all.hi ? i : all.hi - 1;
+            attn_load_lds<4>(stats + (int64_t)next_head * a.tokens + i0, (uint32_t)(in - i0) * 4, stat);
         }
         if (++next == upto) {
             next = from;
@@ -1026,13 +1107,16 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
         gk[d] = f32x16_t{};
         gv[d] = f32x16_t{};
     }
+    const int e = attn_lifted<E>() ? attn_lift_of_rows(a, head0, heads, all, span, tid, lane, wave) : 0;
+    const float by_ds = AttnLift::power(-attn_p_up<E>() - e), back = AttnLift::power(e);
     float far_sum = 0.0f;                      // of the head at hand, from max_distance on
     AttnFar far(0.0f, 1.0f);
     auto step = [&](auto kind_, int n, int place) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(kind_)::value == ATTN_MASKED, NEAR = BIAS && decltype(kind_)::value != ATTN_FAR;
         char* const here = lds + place * PLACE;
         const uint32_t qt = attn_in_lds(here), ot = qt + BYTES;
-        const float* const st = (const float*)(here + 2 * BYTES);       // (lse2, D) of each row
+        const float* const st = (const float*)(here + 2 * BYTES) + 4 * half;       // the lane's rows: eight further on from four to four
+        constexpr int NEXT = ATTN_STAT_BYTES / 4;
         const int i0 = walk.at(n), i = i0 + 4 * half;
         bool terms = false;
         if constexpr (MASKED) {
@@ -1040,31 +1124,36 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
             if (i0 >= own.hi || i0 + BM <= own.lo) return;
         }
         const bool near = NEAR && (far.apart || i0 - (key0 + 31) < a.max_distance);
-        f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp = f32x16_t{};
+        f32x16_t s = attn_start(BIAS && !near ? far.start : 0.0f), dp;      // (dP - D: the product starts at -D)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4_t d = *(const f32x4_t*)(st + NEXT + 8 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * g + e] = d[e];
+        }
 #pragma unroll
         for (int x = 0; x < KS; ++x) s = T::mma(L::rows(qt, at, 0, x), k[x], s);
 #pragma unroll
         for (int x = 0; x < KS; ++x) dp = T::mma(L::rows(ot, at, 0, x), v[x], dp);
         if (NEAR && near) {                    // (a row's exponents as they are to be: nothing is taken from them below)
             attn_add_bias<-1>(s, a.scale_abs, by_distance, i - key, a.max_distance);
-            const float* const near_st = st + 2 * BM;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const f32x2_t x = *(const f32x2_t*)(near_st + 2 * ((r & 3) + 8 * (r >> 2) + 4 * half));
-                s[r] = __builtin_fmaf(s[r] - x[0], ATTN_LOG2E, -x[1]);
+            for (int g = 0; g < 4; ++g) {
+                const f32x4_t lse = *(const f32x4_t*)(st + 2 * NEXT + 8 * g), log_z = *(const f32x4_t*)(st + 3 * NEXT + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[4 * g + e] = __builtin_fmaf(s[4 * g + e] - lse[e], ATTN_LOG2E, -log_z[e]);
             }
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const f32x4_t st01 = *(const f32x4_t*)(st + 16 * g + 8 * half), st23 = *(const f32x4_t*)(st + 16 * g + 8 * half + 4);
+            const f32x4_t lse2 = *(const f32x4_t*)(st + 8 * g);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
-                const float ls = e < 2 ? st01[2 * e] : st23[2 * e - 4], de = e < 2 ? st01[2 * e + 1] : st23[2 * e - 3];
                 const bool hidden = MASKED && (uint32_t)(i + e + 8 * g - key) >= reach;
-                const float p = attn_exp2(NEAR && near ? s[r] : __builtin_fmaf(s[r], c, -ls));
+                const float p = attn_exp2(NEAR && near ? s[r] : __builtin_fmaf(s[r], c, -lse2[e]));
                 s[r] = hidden ? 0.0f : p;
-                dp[r] = hidden ? 0.0f : p * (dp[r] - de);
+                dp[r] = hidden ? 0.0f : attn_lifted<E>() ? p * (dp[r] * by_ds) : p * dp[r];
             }
         }
         if (MASKED && terms) {
@@ -1135,17 +1224,18 @@ __global__ __launch_bounds__(ATTN_THREADS, sizeof(E) == 2 && DP <= 64 ? 2 : 1) v
                 const int ends = b + 1 == a.buckets ? a.max_distance + 63 : b + 1 <= a.exact_to ? b + 1 : (int)a.borders[b - a.exact_to];
                 float x = b + 1 == a.buckets ? far_sum : 0.0f;
                 for (int n = begins; n < ends; ++n) x += on_distance[n];
-                sums[(int64_t)g * a.partial_tiles * a.buckets + b] = x;
+                sums[(int64_t)g * a.partial_tiles * a.buckets + b] = attn_lifted<E>() ? x * back : x;
             }
             far_sum = 0.0f;
         }
     }
     if (!there) return;
+    const float by_k = attn_lifted<E>() ? a.scale * back : a.scale, by_v = attn_lifted<E>() ? AttnLift::power(-14) : 1.0f;
     const int64_t out = ((int64_t)key * kv_heads + kv) * a.dim, size = (int64_t)a.tokens * kv_heads * a.dim;
-    if (parts > 1) attn_write_row<float, DP>(a.part_k + part * size + out, gk, a.scale, a.dim, half, a.dim % 4 == 0);
-    else if (a.gk) attn_write_row<E, DP>(a.gk + out, gk, a.scale, a.dim, half, attn_whole(a.gk, a.dim));
-    if (parts > 1) attn_write_row<float, DP>(a.part_v + part * size + out, gv, 1.0f, a.dim, half, a.dim % 4 == 0);
-    else if (a.gv) attn_write_row<E, DP>(a.gv + out, gv, 1.0f, a.dim, half, attn_whole(a.gv, a.dim));
+    if (parts > 1) attn_write_row<float, DP>(a.part_k + part * size + out, gk, by_k, a.dim, half, a.dim % 4 == 0);
+    else if (a.gk) attn_write_row<E, DP>(a.gk + out, gk, by_k, a.dim, half, attn_whole(a.gk, a.dim));
+    if (parts > 1) attn_write_row<float, DP>(a.part_v + part * size + out, gv, by_v, a.dim, half, a.dim % 4 == 0);
+    else if (a.gv) attn_write_row<E, DP>(a.gv + out, gv, by_v, a.dim, half, attn_whole(a.gv, a.dim));
 }
 
 // dk and dv from their parts, in order; rows that no sequence holds are left as they are
@@ -1312,7 +1402,7 @@ inline void attn_backward_launch(const AttnArgs<E>& a, E* grad_table) {
     const size_t bias = BIAS ? ((size_t)a.max_distance + 1) * 4 : 0;
     attn_query_launch<E, DP, BIAS>(a);
     if (a.gk || a.gv || grad_table) {
-        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + ATTN_STATS, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
+        const size_t place = 2 * attn_tile_bytes<E, DP>(32) + attn_stats<BIAS>() * ATTN_STAT_BYTES, rest = bias + (BIAS && grad_table ? (size_t)ATTN_WAVES * attn_corner(a.max_distance) * 4 : 0);
         const int parts = a.head_parts * a.query_parts;
         const unsigned blocks = (unsigned)(tiles * kv * parts);
         const int stages = attn_stages(place, rest, 1, sizeof(E) == 2 && DP <= 64 && blocks > 256 ? 2 : 1);
@@ -1386,15 +1476,17 @@ inline void attention_backward_entry(const size_t* md, const int32_t* offsets, c
     while (a.head_parts < a.group && (tiles * kv * a.head_parts < 512 || a.group % a.head_parts != 0)) ++a.head_parts;
     while (tiles * kv * a.head_parts * a.query_parts < 512 && (size_t)a.tokens / 32 / a.query_parts >= 16) a.query_parts *= 2;
     const int parts = a.head_parts * a.query_parts;
-    const size_t stats = ((size_t)a.heads * a.tokens * 2 + 63) / 64 * 64, sums = parts > 1 ? ((size_t)a.tokens * kv * a.dim + 63) / 64 * 64 * parts : 0;
+    const size_t stats = ((size_t)a.heads * a.tokens + 63) / 64 * 64, sums = parts > 1 ? ((size_t)a.tokens * kv * a.dim + 63) / 64 * 64 * parts : 0;
+    const size_t all_stats = stats * (table ? 4 : 2), lifts = attn_lifted<E>() ? (size_t)a.heads * cdiv((size_t)a.tokens, 32) * 4 : 0;
     a.partial_tiles = (int)(ATTN_WAVES * tiles) * a.query_parts;
     const size_t partials = grad_table ? (size_t)a.heads * a.partial_tiles * a.buckets : 0;
-    a.stats = (float*)scratch((stats * (table ? 2 : 1) + 2 * sums + partials) * sizeof(float));
+    a.stats = (float*)scratch((all_stats + 2 * sums + partials + lifts) * sizeof(float));
     if (!a.stats) return;
-    a.near_stats = a.stats + (table ? stats : 0);
-    a.part_k = a.near_stats + stats;
+    a.stat_size = (int64_t)stats;
+    a.part_k = a.stats + all_stats;
     a.part_v = a.part_k + sums;
     a.partial = grad_table ? a.part_v + sums : nullptr;
+    a.lifts = (int32_t*)(a.part_v + sums + partials);
     attn_by_dim(a, [&](auto dp) {
         if (table) attn_backward_launch<E, decltype(dp)::value, true>(a, grad_table);
         else attn_backward_launch<E, decltype(dp)::value, false>(a, grad_table);

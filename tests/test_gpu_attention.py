@@ -440,3 +440,32 @@ def test_large_biases(hip, dt, size, heads, dim):
     a = Attention(dt, [400, 90], heads, heads // 2, dim, buckets=16, distance=64, seed=34)
     a.table[:] = to_float(to_storage(size * a.table, dt), dt)
     a.check(hip)
+
+
+@pytest.mark.parametrize("dim,heads,lengths,buckets", [(32, 2, [90, 33], 0), (128, 2, [150, 20], 0), (64, 40, [330], 16), (128, 90, [200, 150], 16), (80, 12, [700], 0), (96, 4, [64, 64], 8)])
+@pytest.mark.parametrize("power", [-14, -8, 6, 11])
+def test_f16_gradients_of_any_size(hip, dim, heads, lengths, buckets, power):
+    """Output gradients times 2^power: all gradients are as many times larger, and so are their bounds (what is held in f16 on the way is
+    scaled to the type's middle: 2^-35 of the largest dS is lost, where the bound counts 2^-25); what leaves f16 is infinite, below its
+    normal numbers a result is off by half of the last subnormal."""
+    a = Attention("f16", lengths, heads, heads // 2, dim, buckets=buckets, distance=40 if buckets else 0, seed=35)
+    go = to_float(to_storage(a.go * 2.0 ** power, "f16"), "f16").astype(np.float64)
+    a.go = go * 2.0 ** -power
+    want, bound = a.exact()
+    a.go = go
+    out, lse = a.forward(hip)
+    for name, got in zip(("gq", "gk", "gv", "gt"), a.backward(hip, out, lse)):
+        if got is None:
+            continue
+        w, b = want[name] * 2.0 ** power, bound[name] * 2.0 ** power + 2.0 ** -25
+        x = to_float(got, "f16").astype(np.float64)
+        fits = np.abs(w) + b < 65504
+        assert fits.mean() > 0.9
+        a.close(np.where(fits, x, 0), np.where(fits, w, 0), b, name)
+        assert not np.isnan(x).any()
+        beyond = np.abs(w) - b > 65520
+        assert (x[beyond] == np.sign(w[beyond]) * np.inf).all()
+
+
+def test_f16_gradients_beside_large_scores(hip):
+    Attention("f16", [150], 2, 1, 64, spread=8.0, scale=0.5, seed=11).check(hip)
