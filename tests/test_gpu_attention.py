@@ -469,3 +469,14 @@ def test_f16_gradients_of_any_size(hip, dim, heads, lengths, buckets, power):
 
 def test_f16_gradients_beside_large_scores(hip):
     Attention("f16", [150], 2, 1, 64, spread=8.0, scale=0.5, seed=11).check(hip)
+
+
+@pytest.mark.parametrize("dim,heads", [(64, 2), (128, 40), (96, 90)])
+def test_f16_gradients_whose_inner_ones_leave_the_type(hip, dim, heads):
+    """dS above 65504 on the way to gradients that f16 holds."""
+    a = Attention("f16", [30, 41], heads, heads // 2, dim, scale=2.0 ** -8, seed=36)
+    a.v = to_float(to_storage(a.v * 64.0, "f16"), "f16").astype(np.float64)
+    a.go = to_float(to_storage(a.go * 1024.0, "f16"), "f16").astype(np.float64)
+    dp = a.v[:30, 0] @ a.go[:30, 0].T                        # [keys, queries]; P is about 1 / (query + 1)
+    assert max(abs(dp[:i + 1, i] - dp[:i + 1, i].mean()).max() / (i + 1) for i in range(1, 30)) > 70000
+    a.check(hip)
