@@ -672,7 +672,8 @@ void hip_softmax_f64(size_t num_els, size_t num_dims, size_t dim, const size_t* 
  *   ln(max_distance / E))), exactly.  -inf takes a pair out; a row whose pairs are all out has an output of zeros and
  *   lse = -inf, and gives no gradient.  Any finite bias is a bias, the type's lowest value too: where it drowns q . k, a row
  *   with nothing else in view spreads evenly over its keys, forward and backward.
- * scale: any value, zero and negative ones included.  dim: 1 .. 128.
+ * scale: any value, zero and negative ones included.  dim: 1 .. 128.  tokens and sequences: below 2^31 - 1024; heads: up to 65535;
+ *   ceil(tokens / 128) * heads: below 2^24.
  * Without tokens or sequences there is nothing to do but to zero grad_bias; with tokens = 0 the tensors' addresses may be NULL.
  * output [tokens, heads, dim] and lse [heads, tokens] (f32) are contiguous.  Rows of tokens that no sequence holds are
  *   not written, here and in the gradients.  Outputs must not overlap inputs.

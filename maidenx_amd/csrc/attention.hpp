@@ -1300,7 +1300,7 @@ inline bool attn_arguments(AttnArgs<E>& a, const size_t* md, const int32_t* offs
     if (heads == 0 || kv == 0 || dim == 0 || heads % kv != 0) { set_status(ERR_INVALID, "attention: heads must be a multiple of kv_heads, and dim positive"); return false; }
     if (dim > (size_t)ATTN_MAX_DIM) { set_status(ERR_UNSUPPORTED, "attention: head dimension above 128"); return false; }
     if (tokens >= (1ull << 31) - 1024 || sequences >= (1ull << 31) - 1024 || heads > 65535) { set_status(ERR_TOO_LARGE, "attention: too many tokens, sequences or heads"); return false; }
-    if (((tokens + ATTN_ROWS - 1) / ATTN_ROWS) * heads >= (1ull << 31)) { set_status(ERR_TOO_LARGE, "attention: too many tiles"); return false; }
+    if (((tokens + ATTN_ROWS - 1) / ATTN_ROWS) * heads * ATTN_THREADS >= (1ull << 32)) { set_status(ERR_TOO_LARGE, "attention: too many tiles"); return false; }
     std::memset((void*)&a, 0, sizeof(a));
     attn_view(a.q, q, md + 7, md[16], (int)dim);
     attn_view(a.k, k, md + 10, md[17], (int)dim);

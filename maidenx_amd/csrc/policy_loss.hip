@@ -6,7 +6,7 @@ namespace mxh {
 __global__ __launch_bounds__(POLICY_SUM_THREADS) void policy_sum_kernel(const float* __restrict__ terms, int n, float* __restrict__ loss) {
     __shared__ double shared[POLICY_SUM_THREADS / WAVE];
     double sum = 0.0;
-    for (int i = threadIdx.x; i < n; i += POLICY_SUM_THREADS) sum += (double)terms[i];
+    for (int64_t i = threadIdx.x; i < n; i += POLICY_SUM_THREADS) sum += (double)terms[i];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, WAVE);
     if (threadIdx.x % WAVE == 0) shared[threadIdx.x / WAVE] = sum;

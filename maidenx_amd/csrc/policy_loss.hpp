@@ -45,7 +45,7 @@ struct PolicyArgs {
     const I* target;
     const float *old_logp, *ref_logp, *advantage, *weight, *grad_loss;
     float least, most, beta;          // 1 - low, 1 + high
-    int32_t rows, vocab;
+    int32_t rows, vocab, row0;        // row0: of a launch's first block
     float *loss, *logp, *lse, *terms;
     E* grad;
     int* flag;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E,
     using T = PolicyType<E>;
     constexpr int N = T::N;
     __shared__ PolicySum shared[THREADS / WAVE];
-    const int row = blockIdx.x, tid = threadIdx.x;
+    const int row = a.row0 + blockIdx.x, tid = threadIdx.x;
     const E* const x = a.logits + (int64_t)row * a.row;
     const int target = policy_target(a, row, tid == 0);
     const int lead = K || a.elem == 1 ? policy_lead(x) : 0, pieces = (lead + a.vocab + N - 1) / N;
@@ -367,9 +367,9 @@ __global__ __launch_bounds__(POLICY_SUM_THREADS) void policy_join_kernel(const P
 }
 // the gradient from lp and lse
 template <class E, class I>
-__global__ __launch_bounds__(POLICY_PART_THREADS) void policy_grad_kernel(const PolicyArgs<E, I> a, int per, int row0) {
+__global__ __launch_bounds__(POLICY_PART_THREADS) void policy_grad_kernel(const PolicyArgs<E, I> a, int per) {
     constexpr int N = PolicyType<E>::N;
-    const int row = row0 + blockIdx.y;
+    const int row = a.row0 + blockIdx.y;
     const int target = policy_target(a, row, blockIdx.x == 0 && threadIdx.x == 0);
     const E* const x = a.logits + (int64_t)row * a.row;
     E* const y = a.grad + (int64_t)row * a.vocab;
@@ -428,6 +428,16 @@ inline bool policy_arguments(PolicyArgs<E, I>& a, const size_t* md, const I* tar
 template <class E, class I>
 inline int policy_pieces(const PolicyArgs<E, I>& a) { return (a.vocab + 2 * (PolicyType<E>::N - 1)) / PolicyType<E>::N; }
 
+// a launch takes less than 2^32 threads, and 65535 blocks along the second axis
+template <class E, class I, class F>
+inline void policy_by_rows(const PolicyArgs<E, I>& a, int most, F&& launch) {
+    PolicyArgs<E, I> b = a;
+    for (int64_t row0 = 0; row0 < a.rows; row0 += most) {
+        b.row0 = (int32_t)row0;
+        launch(b, (unsigned)(a.rows - row0 < most ? a.rows - row0 : most));
+    }
+}
+
 template <class E, class I>
 inline void policy_grad_launch(const PolicyArgs<E, I>& a) {
     // four pieces a thread, or less where rows are few
@@ -435,18 +445,19 @@ inline void policy_grad_launch(const PolicyArgs<E, I>& a) {
     int per = 4 * POLICY_PART_THREADS;
     while (per > POLICY_PART_THREADS && (int64_t)cdiv(pieces, per) * a.rows < 512) per /= 2;
     const unsigned blocks = cdiv((size_t)pieces, (size_t)per);
-    for (int row0 = 0; row0 < a.rows; row0 += 65535) {
-        const int n = a.rows - row0 < 65535 ? a.rows - row0 : 65535;
-        hipLaunchKernelGGL((policy_grad_kernel<E, I>), dim3(blocks, (unsigned)n), dim3(POLICY_PART_THREADS), 0, stream(), a, per, row0);
+    policy_by_rows(a, 65535, [&](const PolicyArgs<E, I>& b, unsigned n) {
+        hipLaunchKernelGGL((policy_grad_kernel<E, I>), dim3(blocks, n), dim3(POLICY_PART_THREADS), 0, stream(), b, per);
         MXH_LAUNCH_CHECK("policy_loss (gradient)");
-    }
+    });
 }
 
 template <class E, class I, int THREADS, int K>
 inline void policy_row_launch(const PolicyArgs<E, I>& a) {
-    if (a.grad) hipLaunchKernelGGL((policy_row_kernel<E, I, THREADS, K, true>), dim3((unsigned)a.rows), dim3(THREADS), 0, stream(), a);
-    else hipLaunchKernelGGL((policy_row_kernel<E, I, THREADS, K, false>), dim3((unsigned)a.rows), dim3(THREADS), 0, stream(), a);
-    MXH_LAUNCH_CHECK("policy_loss");
+    policy_by_rows(a, 1 << 21, [&](const PolicyArgs<E, I>& b, unsigned n) {
+        if (a.grad) hipLaunchKernelGGL((policy_row_kernel<E, I, THREADS, K, true>), dim3(n), dim3(THREADS), 0, stream(), b);
+        else hipLaunchKernelGGL((policy_row_kernel<E, I, THREADS, K, false>), dim3(n), dim3(THREADS), 0, stream(), b);
+        MXH_LAUNCH_CHECK("policy_loss");
+    });
 }
 
 // loss, logp and lse, and the gradient where one is wanted

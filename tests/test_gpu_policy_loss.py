@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import maidenx_amd.lib as L
-from helpers import Null, Out, to_float, u64
+from helpers import In, Null, Out, to_float, u64
 from language import Policy
 
 pytestmark = pytest.mark.gpu
@@ -223,3 +223,25 @@ def test_logits_at_the_limits(hip, dt, rows, vocab, what):
     p.close(p.backward(hip, logp, lse), want["grad"], bound["grad"], "backward")
     for name, got in zip(("loss", "logp", "lse", "grad"), p.step(hip)):
         p.close(got, want[name], bound[name], "step " + name)
+
+
+def test_more_rows_than_a_launch_has_threads_for(hip):
+    """2^24 rows and some: one block of 256 threads each would be more than 2^32 threads.  Two logits a row; every row is checked by a
+    plain sum in 64 bits (a f32 logarithm, exponential and product each: 2^-21 of values below 16 is generous)."""
+    rows = 2 ** 24 + 300
+    r = np.random.default_rng(15)
+    x = r.standard_normal((rows, 2), dtype=np.float32)
+    target = r.integers(0, 2, rows).astype(np.int32)
+    weight = np.full(rows, 1.0, np.float32)
+    adv, zero = r.standard_normal(rows, dtype=np.float32), np.zeros(rows, np.float32)
+    d = (x[np.arange(rows), 1 - target].astype(np.float64) - x[np.arange(rows), target])
+    lp = -np.log1p(np.exp(d))
+    args = [u64(rows, 2, 2, 1, 0), In(target), In(x), In(lp.astype(np.float32)), Null(), In(adv), In(weight), 0.2, 0.2, 0.0]
+    loss, logp, lse, grad = hip.call("policy_loss_step_f32_i32", *args, Null(), Out(1, "f32"), Out(rows, "f32"), Out(rows, "f32"), Out(2 * rows, "f32"))
+    assert np.abs(logp - lp).max() < 2.0 ** -21 * 16
+    assert np.abs(lse - (x[np.arange(rows), target] - lp)).max() < 2.0 ** -21 * 16
+    g = -adv * -np.expm1(lp)                                  # the ratio is one to within a rounding, inside the clip range
+    assert np.abs(grad.reshape(rows, 2)[np.arange(rows), target] - g).max() < 2.0 ** -21 * 16
+    assert abs(loss[0] + adv.astype(np.float64).sum()) < rows * 2.0 ** -21
+    again = hip.call("policy_loss_backward_f32_i32", *args, In(logp), In(lse), Null(), Out(2 * rows, "f32"))[0]
+    assert np.abs(again - grad).max() < 2.0 ** -21 * 16

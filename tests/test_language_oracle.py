@@ -142,3 +142,10 @@ def test_policy_loss_refuses_null_outputs():
                 args = args[:2] + [None] + args[2:]
             got, said = status(name, *policy_args(), *args)
             assert got == INVALID and "null" in said, (name, at)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_attention_refuses_more_threads_than_a_launch_takes(dt):
+    for tokens, heads in ((2 ** 27, 16), (33000, 65028), (128 * 257, 65535), (2 ** 31 - 2048, 2)):
+        got, said = status("attention_" + dt, *attention_args(dt, tokens=tokens, heads=heads, kv=heads))
+        assert got == TOO_LARGE and "tiles" in said, (tokens, heads, got, said)
