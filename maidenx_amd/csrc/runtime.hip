@@ -53,6 +53,8 @@ struct GraphExec {                        // what hip_graph_end_capture hands ou
 // A capture that called scratch() has the block's address baked into its graph or program: while such a capture is
 // alive the block must not be freed, so a later growth retires it instead (freed with the last live capture).
 static bool g_scratch_captured[16][3] = {{false}};
+// ... and a capture that the caller makes of its own stream has it too: nothing says when that graph goes, so its block is never freed.
+static bool g_scratch_callers[16][3] = {{false}};
 static int g_live_captures = 0;
 static std::vector<void*> g_retired_scratch;
 static void* g_scratch[16][3] = {{nullptr}};
@@ -550,6 +552,13 @@ void prog_launch_seen() {
     else g_prog_ok = false;               // a launch without a command: only the HIP graph can replay this capture
 }
 
+// the caller has set a stream that it is capturing itself (the null stream cannot be captured)
+static bool caller_captures() {
+    if (g_capturing || !g_stream) return false;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(g_stream, &st) == hipSuccess && st == hipStreamCaptureStatusActive;
+}
+
 static size_t g_scratch_allocs = 0;       // hipMallocs made by scratch() (under g_scratch_mu)
 
 void* scratch(size_t bytes, int slot) {
@@ -559,11 +568,13 @@ void* scratch(size_t bytes, int slot) {
         return nullptr;
     }
     std::lock_guard<std::mutex> lk(g_scratch_mu);
+    const bool callers = caller_captures();
     if (g_scratch_bytes[dev][slot] >= bytes) {
         if (g_capturing) g_scratch_captured[dev][slot] = true;
+        if (callers) g_scratch_callers[dev][slot] = true;
         return g_scratch[dev][slot];
     }
-    if (g_capturing) {      // growing means a synchronise and a free, neither of which a capture allows
+    if (g_capturing || callers) {      // growing means a synchronise and a free, neither of which a capture allows
         set_status(ERR_INVALID, "scratch would have to grow during graph capture: run the sequence eagerly once first");
         return nullptr;
     }
@@ -571,9 +582,11 @@ void* scratch(size_t bytes, int slot) {
     if (g_scratch[dev][slot]) {
         (void)hipStreamSynchronize(g_stream);
         if (g_capture_stream) (void)hipStreamSynchronize(g_capture_stream);     // replays queued there use the block as well
-        if (g_scratch_captured[dev][slot] && g_live_captures > 0) g_retired_scratch.push_back(g_scratch[dev][slot]);
-        else (void)hipFree(g_scratch[dev][slot]);
-        g_scratch_captured[dev][slot] = false;
+        if (!g_scratch_callers[dev][slot]) {
+            if (g_scratch_captured[dev][slot] && g_live_captures > 0) g_retired_scratch.push_back(g_scratch[dev][slot]);
+            else (void)hipFree(g_scratch[dev][slot]);
+        }
+        g_scratch_captured[dev][slot] = g_scratch_callers[dev][slot] = false;
         g_scratch[dev][slot] = nullptr;
         g_scratch_bytes[dev][slot] = 0;
     }
@@ -595,7 +608,7 @@ int* index_flag() {
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) { set_status(ERR_INVALID, "index flag: bad device"); return nullptr; }
     std::lock_guard<std::mutex> lk(g_scratch_mu);
     if (!g_index_flag[dev]) {
-        if (g_capturing) { set_status(ERR_INVALID, "the first index op of a device cannot run inside a graph capture"); return nullptr; }
+        if (g_capturing || caller_captures()) { set_status(ERR_INVALID, "the first index op of a device cannot run inside a graph capture"); return nullptr; }
         int* p = nullptr;
         hipError_t e = hipMalloc((void**)&p, 256);
         if (e == hipSuccess) e = hipMemset(p, 0, 256);
@@ -613,7 +626,7 @@ static void collect_index_flag() {
     int* p;
     {
         std::lock_guard<std::mutex> lk(g_scratch_mu);
-        if (!g_index_flag_used[dev] || g_capturing) return;
+        if (!g_index_flag_used[dev] || g_capturing || caller_captures()) return;
         g_index_flag_used[dev] = false;
         p = g_index_flag[dev];
     }

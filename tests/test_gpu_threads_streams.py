@@ -132,3 +132,65 @@ def test_replay_on_a_caller_set_stream_equals_eager(lib, n, program):
         assert lib.hip_stream_synchronize(s) == 0
         assert lib.hip_stream_destroy(s) == 0
     assert lib.hip_get_last_status() == 0, lib.hip_status_string()
+
+
+CALLERS_GRAPH = """
+import sys
+sys.path[:0] = {paths!r}
+import ctypes as C
+import numpy as np
+import maidenx_amd.lib as L
+from helpers import In, to_storage
+from language import Attention
+lib, hip = L.load(), C.CDLL("libamdhip64.so")
+ok = lambda rc: rc == 0 or sys.exit("runtime error %d" % rc)
+
+def problem(**kw):
+    a = Attention("bf16", **kw)
+    dev = lambda x: L.DeviceBuffer.from_numpy(x.arr) if isinstance(x, In) else x
+    args = [dev(x) if isinstance(x, In) else None if type(x).__name__ == "Null" else x for x in a.arguments()]
+    n, m = a.tokens * a.heads * a.dim, a.tokens * a.kv * a.dim
+    outs = [L.DeviceBuffer(2 * c) for c in (n, n, m, m)]
+    lse, go = L.DeviceBuffer(4 * a.tokens * a.heads), L.DeviceBuffer.from_numpy(to_storage(a.go, "bf16").ravel())
+    def calls():
+        L.call("attention_bf16", *args, outs[0], lse)
+        L.call("attention_backward_bf16", *args, outs[0], lse, go, *outs[1:], None)
+    calls.keep = (args, lse, go)
+    return calls, outs
+
+s, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+ok(lib.hip_stream_create(C.byref(s)))
+ok(lib.hip_set_stream(s))
+small, outs = problem(lengths=[150, 50], heads=4, kv=2, dim=64)
+large, _ = problem(lengths=[16] * 5000, heads=64, kv=64, dim=1)
+small()
+L.synchronize()
+want = [o.to_numpy(np.uint16).tobytes() for o in outs]
+before = lib.hip_scratch_allocations()
+ok(hip.hipStreamBeginCapture(s, 1))
+small()
+large()                                      # would need a larger workspace: refused, and the capture goes on
+assert lib.hip_get_last_status() == 1 and b"grow" in lib.hip_status_string()
+ok(hip.hipStreamEndCapture(s, C.byref(graph)))
+ok(hip.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_ulonglong(0)))
+for turn in range(3):
+    for o in outs:
+        lib.hip_fill_bf16(o.nbytes // 2, o.ptr, 0x4000)
+    ok(hip.hipGraphLaunch(exe, s))
+    L.synchronize()
+    assert [o.to_numpy(np.uint16).tobytes() for o in outs] == want, turn
+    large()                                  # eager: grows the workspace the first time; the graph keeps the old one
+    L.synchronize()
+    assert lib.hip_scratch_allocations() == before + 1
+print("replayed")
+"""
+
+
+def test_a_graph_of_the_callers_keeps_its_workspace():
+    """A caller that captures its own stream has the workspace's address in its graph: the library does not grow it meanwhile, nor free
+    it when it grows later."""
+    import subprocess
+    import sys
+    from helpers import ROOT
+    p = subprocess.run([sys.executable, "-c", CALLERS_GRAPH.format(paths=[ROOT, ROOT + "/tests"])], capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0 and "replayed" in p.stdout, (p.stdout[-1000:], p.stderr[-2000:])
