@@ -704,7 +704,8 @@ MX_DECL_ATTENTION(mx_f16, f16)
  *   [rows]; one outside [0, vocabulary) in a row that counts leaves the row out and is reported by hip_get_last_status() like an
  *   index out of range.  old_logp, ref_logp (NULL if kl_weight is 0), advantage, weight: f32 [rows].  clip_low, clip_high >= 0.
  * Without rows the loss is zero, and the addresses of everything else may be NULL.
- * loss [1], logp [rows] (lp), lse [rows]: f32.  grad_logits [rows, vocabulary]: contiguous, of the logits' type.
+ * loss [1], logp [rows] (lp), lse [rows]: f32.  grad_logits [rows, vocabulary]: contiguous, of the logits' type,
+ *   beside them: overlapping the logits (a gradient in place) is refused.
  *   hip_policy_loss_..           the loss
  *   hip_policy_loss_backward_..  grad_logits = grad_loss[0] * (d loss / d x) from logp and lse of the forward call; grad_loss NULL: 1
  *   hip_policy_loss_step_..      both in one pass over the logits (each read once where a row fits a block's registers)

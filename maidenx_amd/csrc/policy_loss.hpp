@@ -399,7 +399,7 @@ void policy_sum(const float* terms, int n, float* loss);
 
 template <class E, class I>
 inline bool policy_arguments(PolicyArgs<E, I>& a, const size_t* md, const I* target, const E* logits, const float* old_logp, const float* ref_logp,
-                             const float* advantage, const float* weight, float low, float high, float beta) {
+                             const float* advantage, const float* weight, float low, float high, float beta, const E* grad) {
     const bool some = !md || md[0] != 0;        // (tensors of no rows have no address)
     if (!md || (some && (!target || !logits || !old_logp || !advantage || !weight))) { set_status(ERR_INVALID, "policy_loss: null argument"); return false; }
     if (some && !ref_logp && beta != 0.0f) { set_status(ERR_INVALID, "policy_loss: the KL term needs ref_logp"); return false; }
@@ -421,6 +421,12 @@ inline bool policy_arguments(PolicyArgs<E, I>& a, const size_t* md, const I* tar
     a.rows = (int32_t)md[0];
     a.vocab = (int32_t)md[1];
     if (a.rows == 0) return true;
+    if (grad) {      // a row's threads write while others still read its target
+        const int64_t ends[2] = {(int64_t)(a.rows - 1) * a.row, (int64_t)(a.vocab - 1) * a.elem};
+        const E *lo = a.logits, *hi = a.logits + 1;
+        for (int64_t end : ends) (end < 0 ? lo : hi) += end;
+        if (grad < hi && lo < grad + (size_t)a.rows * a.vocab) { set_status(ERR_INVALID, "policy_loss: grad_logits overlaps the logits"); return false; }
+    }
     a.flag = index_flag();
     return a.flag != nullptr;
 }
@@ -467,7 +473,7 @@ inline void policy_entry(const size_t* md, const I* target, const E* logits, con
     PolicyArgs<E, I> a;
     const bool some = !md || md[0] != 0;
     if (!loss || (some && (!logp || !lse || (step && !grad)))) { set_status(ERR_INVALID, "policy_loss: null output"); return; }
-    if (!policy_arguments(a, md, target, logits, old_logp, ref_logp, advantage, weight, low, high, beta)) return;
+    if (!policy_arguments(a, md, target, logits, old_logp, ref_logp, advantage, weight, low, high, beta, step ? grad : nullptr)) return;
     a.grad_loss = grad_loss;
     a.loss = loss;
     a.logp = logp;
@@ -504,7 +510,7 @@ inline void policy_backward_entry(const size_t* md, const I* target, const E* lo
                                   const float* weight, float low, float high, float beta, const float* logp, const float* lse, const float* grad_loss, E* grad) {
     PolicyArgs<E, I> a;
     if ((!logp || !lse || !grad) && !(md && md[0] == 0)) { set_status(ERR_INVALID, "policy_loss_backward: null argument"); return; }
-    if (!policy_arguments(a, md, target, logits, old_logp, ref_logp, advantage, weight, low, high, beta)) return;
+    if (!policy_arguments(a, md, target, logits, old_logp, ref_logp, advantage, weight, low, high, beta, grad)) return;
     if (a.rows == 0) return;
     a.grad_loss = grad_loss;
     a.logp = (float*)logp;

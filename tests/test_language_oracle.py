@@ -149,3 +149,19 @@ def test_attention_refuses_more_threads_than_a_launch_takes(dt):
     for tokens, heads in ((2 ** 27, 16), (33000, 65028), (128 * 257, 65535), (2 ** 31 - 2048, 2)):
         got, said = status("attention_" + dt, *attention_args(dt, tokens=tokens, heads=heads, kv=heads))
         assert got == TOO_LARGE and "tiles" in said, (tokens, heads, got, said)
+
+
+@pytest.mark.parametrize("suffix,size", [("f32_i32", 4), ("bf16_i64", 2), ("f16_i32", 2)])
+@pytest.mark.parametrize("strides", [(10, 1), (12, 1), (1, 4), (2 ** 64 - 10, 1), (10, 2 ** 64 - 1)])
+def test_policy_loss_refuses_a_gradient_in_place(suffix, size, strides):
+    """Rows and elements in either direction; the gradient begins at the logits' first byte, at their last, or ends in them."""
+    low, high = 0, 0
+    for n, s in ((4, strides[0]), (10, strides[1])):
+        end = (n - 1) * (s if s < 2 ** 63 else s - 2 ** 64)
+        low, high = low + min(end, 0), high + max(end, 0)
+    at = 2 ** 20
+    args = policy_args(x=at, md=u64(4, 10, list(strides), 0))
+    for grad in (at + low * size, at + high * size, at + (low - 39) * size):
+        for name, rest in (("policy_loss_step_", [None, 10, 20, 30, grad]), ("policy_loss_backward_", [20, 30, None, grad])):
+            got, said = status(name + suffix, *args, *rest)
+            assert got == INVALID and "overlaps" in said, (name, grad - at, got, said)
