@@ -1,27 +1,30 @@
 // Attention for f32 tensors, and the bucket borders of the relative position bias (see attention.hpp).
-#include <vector>
-
 #include "attention.hpp"
 
 namespace mxh {
 
-// x^n as whole numbers of 32-bit limbs, least first
-typedef std::vector<uint32_t> Whole;
-static void multiply(Whole& w, uint32_t x) {
-    uint64_t carry = 0;
-    for (uint32_t& limb : w) {
-        carry += (uint64_t)limb * x;
-        limb = (uint32_t)carry;
-        carry >>= 32;
+// a whole number of 32-bit limbs, least first; the largest here is 4096^128 = 2^1536
+struct Whole {
+    static constexpr int MOST = (12 * ATTN_MAX_BUCKETS / 2 + 31) / 32 + 1;
+    static_assert(ATTN_MAX_DISTANCE <= 4096, "12 bits a factor");
+    uint32_t limb[MOST] = {1};
+    int size = 1;
+    void multiply(uint32_t x) {
+        uint64_t carry = 0;
+        for (int i = 0; i < size; ++i) {
+            carry += (uint64_t)limb[i] * x;
+            limb[i] = (uint32_t)carry;
+            carry >>= 32;
+        }
+        if (carry && size < MOST) limb[size++] = (uint32_t)carry;
     }
-    if (carry) w.push_back((uint32_t)carry);
-}
-static bool less(const Whole& a, const Whole& b) {
-    if (a.size() != b.size()) return a.size() < b.size();
-    for (size_t i = a.size(); i-- > 0;)
-        if (a[i] != b[i]) return a[i] < b[i];
-    return false;
-}
+    bool below(const Whole& b) const {
+        if (size != b.size) return size < b.size;
+        for (int i = size; i-- > 0;)
+            if (limb[i] != b.limb[i]) return limb[i] < b.limb[i];
+        return false;
+    }
+};
 
 // Bucket E + m begins at the least whole n with (n / E)^M >= (X / E)^m, that is n^M >= X^m E^(M - m) (E = buckets / 2,
 // M = buckets - E, X = max_distance).  The logarithms of the definition are whole numbers exactly there, where floating
@@ -32,13 +35,13 @@ bool attn_borders(int buckets, int max_distance, uint16_t* borders) {
     const int E = buckets / 2, M = buckets - E;
     if (known_buckets != buckets || known_distance != max_distance) {
         for (int m = 1; m < M; ++m) {
-            Whole right{1};
-            for (int i = 0; i < m; ++i) multiply(right, (uint32_t)max_distance);
-            for (int i = m; i < M; ++i) multiply(right, (uint32_t)E);
+            Whole right;
+            for (int i = 0; i < m; ++i) right.multiply((uint32_t)max_distance);
+            for (int i = m; i < M; ++i) right.multiply((uint32_t)E);
             auto reaches = [&](int n) {
-                Whole left{1};
-                for (int i = 0; i < M; ++i) multiply(left, (uint32_t)n);
-                return !less(left, right);
+                Whole left;
+                for (int i = 0; i < M; ++i) left.multiply((uint32_t)n);
+                return !left.below(right);
             };
             int n = (int)std::floor((double)E * std::pow((double)max_distance / E, (double)m / M));
             while (n > 1 && reaches(n - 1)) --n;
