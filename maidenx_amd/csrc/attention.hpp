@@ -800,11 +800,11 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
 // ---- backward: gradients of the queries ------------------------------------------------------------------------------------
 // A block owns 128 queries like the forward kernel.  Writes dq (if wanted) and, for the kernel of the keys, lse and D_i: with a
 // bias the one that makes the row of dS sum to zero (formed from P and dP themselves; the rounding of o in do . o
-// would otherwise enter every pair of the far bucket with the same sign).  bf16, 8192 tokens (4096, 3000, 1096), 16 heads of 128: 204-226
-// us = 730-810 TFLOP/s, 16 heads of 64: 117 us.
+// would otherwise enter every pair of the far bucket with the same sign).  bf16, 8192 tokens (4096, 3000, 1096), 16 heads of 128: 196-217
+// us = 760-846 TFLOP/s, 16 heads of 64: 110 us.
 // The sum, the rows of q and those of do take 128 registers at 128 elements a head.  With 64 keys to a tile the rest does not suffice (a
 // register more than there are is read from memory, behind every tile on its way): 8192 tokens, 16 heads with a bias 313 us, with 32
-// keys 212.
+// keys 212.  (With a bias five registers are read back even so, for lse as it is: 214 us.)
 //
 // With a bias, scores and lse may be so large that lse has lost the logarithm of the sum to its rounding (masks by large negative numbers:
 // the row of P would sum to the number of its keys).  Beyond ATTN_ROUGH - 2^8 2^-24 = 2^-16 - a wave forms that sum first, keys straight
@@ -886,7 +886,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
         }
         ++next;
     };
-    const bool walks = a.gq || (BIAS && (a.gk || a.partial)) || (attn_lifted<E>() && a.gk);       // else only D_i is wanted, if that
+    const bool walks = a.gq || BIAS || (attn_lifted<E>() && a.gk);       // else only D_i is wanted, if that
     if (walks) ring.begin(rounds.total, fetch);
     typename T::Frag q[KS], go[KS];
     attn_own_rows<E, DP>(a.go, head, there ? row : 0, there, a.dim, lane, 1.0f, go);
@@ -905,7 +905,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     }
     float* const stat = a.stats + (int64_t)head * a.tokens + row;
     if (!walks) {
-        if (there && half == 0 && group == 0) { stat[0] = lse * ATTN_LOG2E - attn_p_up<E>(); stat[a.stat_size] = -delta; }      // (never with a bias: the gradient of the values alone wants no D)
+        if (there && half == 0 && group == 0) { stat[0] = lse * ATTN_LOG2E - attn_p_up<E>(); stat[a.stat_size] = -delta; }
         return;
     }
     attn_own_rows<E, DP>(a.q, head, there ? row : 0, there, a.dim, lane, attn_sign(a.scale), q);
@@ -1013,7 +1013,7 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
 //
 // Both sums, the keys and the values of 32 rows of 128 elements take 192 registers of a wave and leave no room for a second wave on
 // its SIMD above 64 elements a head (16 bits): one wave there is limited by what it can issue (8192 tokens, 16 heads of 128:
-// 413 us = 535 TFLOP/s; of 64, with two waves, 218 us = 508).  Two waves that share the work, one for each sum and both making P, take
+// 416 us = 531 TFLOP/s; of 64, with two waves, 223 us = 495).  Two waves that share the work, one for each sum and both making P, take
 // 406, and more for the bias; the values in LDS, 475.
 __host__ __device__ inline int attn_corner(int max_distance) { return 16 * 33 + max_distance + 63; }      // floats of a wave
 // Statistics of the 32 rows of a tile, two or (with a bias) four of each.  A wave brings one of them, 4 bytes a lane, twice over; where there
@@ -1362,7 +1362,10 @@ inline void attn_row_launch(Kernel* kernel, const AttnArgs<E>& a, size_t place, 
 // forward, 32 heads: 185 against 161 us.  With less than three blocks for four CUs, four groups share the walks of half as many
 // rows: f32, 1024 tokens, 8 heads of 64 with a bias (64 blocks) 47 -> 31 us forward, 65 -> 41 us dq, f16, 1802 tokens, 12 heads of 80 (180
 // blocks) 34 -> 29 and 40 -> 33 us; with 256 blocks they lose: bf16, 2000 tokens, 16 heads of 64: 32 -> 40 us.
-// f32 heads above 64 take too many registers for either.
+// f32 heads above 64 take too many registers for either.  At 128 elements (16 bits) four groups read up to 29 registers back from memory and
+// are ahead all the same: 1024 tokens, 16 heads (128 blocks): 25 -> 24 us forward, 34 -> 28 dq; 2048 tokens, 8 heads: 40 -> 36, 54 -> 41.
+// At 192 blocks, where twice as many of half the rows are one and a half for a CU, it goes by the walks: 2048 tokens, 12 heads of 96:
+// 40 -> 37, 48 -> 43; 1024 tokens, 24 heads: 25 -> 28, 31 -> 34 (of 128: 41 -> 43, 55 -> 50 and 26 -> 33, 36 -> 41).
 template <class E, int DP>
 inline int attn_groups(const AttnArgs<E>& a) {
     const int64_t blocks = (int64_t)((a.tokens + ATTN_ROWS - 1) / ATTN_ROWS) * a.heads;

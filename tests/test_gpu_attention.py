@@ -480,3 +480,19 @@ def test_f16_gradients_whose_inner_ones_leave_the_type(hip, dim, heads):
     dp = a.v[:30, 0] @ a.go[:30, 0].T                        # [keys, queries]; P is about 1 / (query + 1)
     assert max(abs(dp[:i + 1, i] - dp[:i + 1, i].mean()).max() / (i + 1) for i in range(1, 30)) > 70000
     a.check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("buckets", [0, 16])
+@pytest.mark.parametrize("large", [False, True])
+def test_one_gradient_alone_finds_nothing_of_an_earlier_call(hip, dt, buckets, large):
+    """Each gradient by itself, after a call of another problem of the same sizes has left its numbers in the workspace."""
+    a, other = (Attention(dt, [150, 60], 4, 2, 64, buckets=buckets, distance=64 if buckets else 0, seed=s, spread=f) for s, f in ((37, 1.0), (38, 3.0)))
+    if large and buckets:
+        a.table[:3] = to_float(to_storage(np.full((3, 4), -60000.0), dt), dt)
+    out, lse = a.forward(hip)
+    every = a.backward(hip, out, lse)
+    for n in range(4 if buckets else 3):
+        other.backward(hip, *other.forward(hip))
+        got = a.backward(hip, out, lse, tuple(m == n for m in range(4)))
+        assert got[n].tobytes() == every[n].tobytes(), n
