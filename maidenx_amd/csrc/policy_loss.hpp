@@ -199,8 +199,8 @@ __device__ inline void policy_write(const PolicyArgs<E, I>& a, int row, float lo
 // ---- one block a row -------------------------------------------------------------------------------------------------------
 // K pieces of a thread stay in registers between the sums and the gradient; K = 0: rows that do not fit, or whose elements are not
 // neighbours, are read again (from the caches, as a block's row is what its CU read last).
-// Loss and gradient, bf16: 2048 rows of 32000 (six in ten count) 50 us a call = 4.2 TB/s, 8192 rows of 50001 329 us = 4.7 TB/s, where a large
-// copy reaches 4.7; loss alone, f32, 3000 rows of 32000 (seven in ten) 50 us a call = 5.3 TB/s.
+// Loss and gradient, bf16: 2048 rows of 32000 (six in ten count) 50 us in a row of calls = 4.2 TB/s, 8192 rows of 50001 329 us = 4.7 TB/s, where a large
+// copy reaches 4.7; loss alone, f32, 3000 rows of 32000 (seven in ten) 50 us = 5.3 TB/s.
 template <class E, class I, int THREADS, int K, bool STEP>
 __global__ __launch_bounds__(THREADS) void policy_row_kernel(const PolicyArgs<E, I> a) {
     using T = PolicyType<E>;
