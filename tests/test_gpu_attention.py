@@ -496,3 +496,50 @@ def test_one_gradient_alone_finds_nothing_of_an_earlier_call(hip, dt, buckets, l
         other.backward(hip, *other.forward(hip))
         got = a.backward(hip, out, lse, tuple(m == n for m in range(4)))
         assert got[n].tobytes() == every[n].tobytes(), n
+
+
+class Mixed(Attention):
+    """Query, key and value each packed or on no 16-byte boundary."""
+
+    def stored(self):
+        kinds, out = self.layout, []
+        for n, kind in enumerate(kinds):
+            self.layout = kind
+            out.append(super().stored()[n])
+        self.layout = kinds
+        return out
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("dim", [24, 32, 64, 128])
+@pytest.mark.parametrize("kinds", [("odd", "packed", "packed"), ("packed", "odd", "packed"), ("packed", "packed", "odd"), ("odd", "odd", "packed")])
+def test_operands_that_lie_differently(hip, dt, dim, kinds):
+    """One operand of a tile straight to shared memory, the other through registers."""
+    Mixed(dt, [410, 60], 4, 2, dim, layout=kinds, buckets=8, distance=30, seed=39).check(hip)
+    Mixed(dt, [300], 40, 20, dim, layout=kinds, seed=40).check(hip)
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("stride", [2 ** 23 - 8, 2 ** 23 + 8])
+def test_offsets_beyond_32_bits(hip, dt, stride):
+    """Tokens 2^23 elements apart, on either side of the longest row that goes straight to shared memory: a sequence of 400 reaches
+    over 2^31 elements and more."""
+    lib, size = L.load(), 4 if dt == "f32" else 2
+    a = Attention(dt, [380, 20], 2, 1, 32, buckets=8, distance=30, seed=41)
+    want = [a.forward(hip)]
+    want += [a.backward(hip, *want[0])]
+    rows = to_storage(np.concatenate([a.q, a.k, a.v], axis=1), dt).reshape(400, -1)
+    big = L.DeviceBuffer((399 * stride + rows.shape[1]) * size)
+    for t in range(400):
+        assert lib.hip_memcpy_h2d(big.ptr + t * stride * size, rows[t].ctypes.data, rows[t].nbytes) == 0
+    md = a.arguments()[0].copy()
+    for n, offset in enumerate((0, 64, 96)):
+        md[7 + 3 * n], md[16 + n] = stride, offset
+    dev = [L.DeviceBuffer.from_numpy(x) for x in (a.offsets, to_storage(a.table, dt).ravel(), to_storage(a.go, dt).ravel())]
+    out, lse, gq, gk, gv, gt = (L.DeviceBuffer(x.nbytes) for x in (*want[0], *want[1]))
+    common = [md, dev[0], big, big, big, dev[1], float(a.scale)]
+    L.call("attention_" + dt, *common, out, lse)
+    L.call("attention_backward_" + dt, *common, out, lse, dev[2], gq, gk, gv, gt)
+    L.synchronize()
+    for got, w in zip((out, lse, gq, gk, gv, gt), (*want[0], *want[1])):
+        assert got.to_numpy(w.dtype).tobytes() == w.tobytes()

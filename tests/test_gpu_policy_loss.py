@@ -245,3 +245,24 @@ def test_more_rows_than_a_launch_has_threads_for(hip):
     assert abs(loss[0] + adv.astype(np.float64).sum()) < rows * 2.0 ** -21
     again = hip.call("policy_loss_backward_f32_i32", *args, In(logp), In(lse), Null(), Out(2 * rows, "f32"))[0]
     assert np.abs(again - grad).max() < 2.0 ** -21 * 16
+
+
+@pytest.mark.parametrize("rows,vocab", [(300, 1001), (3, 9001)])
+def test_rows_beyond_32_bits(hip, rows, vocab):
+    """Rows so far apart that the last lies beyond 2^31 elements.  (Not the bits of rows that lie together: how a row is cut into
+    16-byte pieces goes by its alignment, and the order of its sum by that.)"""
+    lib = L.load()
+    p = Policy("bf16", rows, vocab, seed=16)
+    want, bound = p.exact()
+    args = p.arguments()
+    stride = 2 ** 31 // (rows - 1) + 9
+    big = L.DeviceBuffer(((rows - 1) * stride + vocab) * 2)
+    x = args[2].arr.reshape(rows, vocab)
+    for t in range(rows):
+        assert lib.hip_memcpy_h2d(big.ptr + t * stride * 2, np.ascontiguousarray(x[t]).ctypes.data, 2 * vocab) == 0
+    dev = [L.DeviceBuffer.from_numpy(a.arr) for a in (args[1], *args[3:7])]
+    outs = [L.DeviceBuffer(n) for n in (4, 4 * rows, 4 * rows, 2 * rows * vocab)]
+    L.call("policy_loss_step_bf16_i64", u64(rows, vocab, stride, 1, 0), dev[0], big, *dev[1:], *args[7:], None, *outs)
+    L.synchronize()
+    for name, got in zip(("loss", "logp", "lse", "grad"), outs):
+        p.close(got.to_numpy(np.uint16 if name == "grad" else np.float32).reshape(want[name].shape), want[name], bound[name], name)
