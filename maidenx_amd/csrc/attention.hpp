@@ -535,9 +535,13 @@ struct AttnLift {
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, __builtin_fabsf(s[r]));
         if (__any(top > limit)) {
+            top = 0.0f;                         // (an infinite value stays one, and says nothing about the other rows)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = __builtin_fabsf(s[r]) < INFINITY ? fmaxf(top, __builtin_fabsf(s[r])) : top;
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, WAVE));
-            int up = top < INFINITY ? 11 - __builtin_amdgcn_frexp_expf(top) : 0;      // (what is infinite stays so)
+            if (!(top > limit)) return;
+            int up = 11 - __builtin_amdgcn_frexp_expf(top);
             up = up < e - 100 ? e - 100 : up > e + 80 ? e + 80 : up;      // (dS is below 2^40: nothing overflows in f32)
             up = __builtin_amdgcn_readfirstlane(up);
             const float by = power(up);
@@ -546,7 +550,7 @@ struct AttnLift {
             for (int d = 0; d < DB; ++d) sums[d] *= attn_start(by);
             other *= by;
             e -= up;
-            limit = top < INFINITY ? 32768.0f : INFINITY;
+            limit = 32768.0f;
         }
     }
     __device__ static __forceinline__ float power(int n) { return __builtin_ldexpf(1.0f, n); }
@@ -916,7 +920,11 @@ __global__ __launch_bounds__(64 * attn_row_waves<KG>() * KG, sizeof(E) == 4 && D
     const float c = a.scale_log2;
     if constexpr (BIAS) {                 // (kept in memory over the walk, where registers are scarce; both halves and all groups write the same)
         float z = 1.0f;
-        if (__any(__builtin_fabsf(lse) > ATTN_ROUGH && lse != INFINITY)) z = attn_row_sum<E, DP>(a, head, kv, row, lane, own, lower, reach, lse, q);
+        const bool rough = __builtin_fabsf(lse) > ATTN_ROUGH && lse != INFINITY;
+        if (__any(rough)) {
+            const float sum = attn_row_sum<E, DP>(a, head, kv, row, lane, own, lower, reach, lse, q);
+            z = rough ? sum : 1.0f;             // (the other rows are as they would be without these)
+        }
         if (there) {
             stat[2 * a.stat_size] = lse;
             stat[3 * a.stat_size] = __builtin_amdgcn_logf(z) - attn_p_up<E>();

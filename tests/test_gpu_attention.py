@@ -4,7 +4,7 @@ import pytest
 
 import maidenx_amd.lib as L
 from helpers import to_float, to_storage
-from language import E32, UNIT, Attention, borders, bucket_of
+from language import E32, TINY, UNIT, Attention, borders, bucket_of
 
 pytestmark = pytest.mark.gpu
 ALL = ["f32", "bf16", "f16"]
@@ -543,3 +543,36 @@ def test_offsets_beyond_32_bits(hip, dt, stride):
     L.synchronize()
     for got, w in zip((out, lse, gq, gk, gv, gt), (*want[0], *want[1])):
         assert got.to_numpy(w.dtype).tobytes() == w.tobytes()
+
+
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("power", [-14, 0, 11])
+def test_gradients_of_any_size_beside_infinite_ones(hip, dt, power):
+    """Sequences that share the tiles of a wave, one full of infinities and NaN: the other's gradients keep their bounds, for output gradients of
+    any size (times a power of two, as all of them then are)."""
+    a = Attention(dt, [45, 40, 70], 2, 1, 64, lead=4, tail=7, seed=42)
+    go = to_float(to_storage(a.go * 2.0 ** power, dt), dt).astype(np.float64)
+    a.go = go * 2.0 ** -power
+    want, bound = a.exact()
+    a.go = go
+    clean, dirty = np.r_[4:49, 89:159], np.r_[0:4, 49:89, a.tokens - 7:a.tokens]
+    for t in (a.q, a.k, a.v, a.go):
+        t[dirty[::2]] = np.nan
+        t[dirty[1::2]] = np.inf
+    out, lse = a.forward(hip)
+    for name, g in zip(("gq", "gk", "gv"), a.backward(hip, out, lse)):
+        a.close(g[clean], want[name][clean] * 2.0 ** power, bound[name][clean] * 2.0 ** power + TINY[dt], name)
+
+
+@pytest.mark.parametrize("dt", ALL)
+def test_rows_that_are_summed_once_more_leave_others_as_they_are(hip, dt):
+    """Large scores in one sequence: the gradients of another in the same waves keep their bits."""
+    a = Attention(dt, [45, 40, 70], 2, 1, 64, buckets=8, distance=16, seed=42)
+    clean, large = np.r_[0:45, 85:155], np.r_[45:85]
+    a.go[large] = 0
+    want = a.backward(hip, *a.forward(hip))
+    a.q[large], a.k[large] = a.q[large] * 16, a.k[large] * 16
+    out, lse = a.forward(hip)
+    assert np.abs(lse[:, large]).max() > 256
+    for w, g in zip(want[:3], a.backward(hip, out, lse)):
+        assert g[clean].tobytes() == w[clean].tobytes()
